@@ -53,12 +53,32 @@ class BankConfigV1(C.Structure):
                 ("reserved", C.c_int32 * 6)]
 
 
+class RouteConfigV1(C.Structure):
+    _fields_ = [("n_experts", C.c_int32), ("k", C.c_int32), ("score", C.c_int32), ("n_groups", C.c_int32),
+                ("top_groups", C.c_int32), ("group_score", C.c_int32), ("renormalize", C.c_int32),
+                ("scale", C.c_float), ("logits_type", C.c_int32), ("reserved", C.c_int32 * 3)]
+
+
+class BlockNormConfigV1(C.Structure):
+    _fields_ = [("dim", C.c_int32), ("post", C.c_int32), ("gate", C.c_int32), ("gate_sigmoid", C.c_int32),
+                ("h_type", C.c_int32), ("y_type", C.c_int32), ("gate_type", C.c_int32), ("x_type", C.c_int32),
+                ("post_eps", C.c_float), ("pre_eps", C.c_float), ("residual_scale", C.c_float),
+                ("block_scale", C.c_float), ("ld_h", C.c_int64), ("ld_y", C.c_int64), ("ld_gate", C.c_int64),
+                ("ld_h_out", C.c_int64), ("ld_x", C.c_int64), ("reserved", C.c_int32 * 4)]
+
+
+class Int8LinearConfigV1(C.Structure):
+    _fields_ = [("n", C.c_int32), ("k", C.c_int32), ("x_type", C.c_int32), ("out_type", C.c_int32),
+                ("ld_w", C.c_int64), ("ld_x", C.c_int64), ("ld_out", C.c_int64), ("reserved", C.c_int32 * 4)]
+
+
 HOST_EXPERT_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.c_uint32, C.c_int32, C.POINTER(C.c_float), C.c_int32,
                              C.POINTER(C.c_float))
 
 _P = C.c_void_p
 _I = C.c_int32
 _U32 = C.c_uint32
+_I64 = C.c_int64
 _F = C.c_float
 _SZ = C.c_size_t
 _PE = C.POINTER(ErrorV1)
@@ -122,6 +142,12 @@ SIGNATURES = {
     "clb_lane_config_parse": (_I, [C.c_char_p, _P, _PE]),
     "clb_bank_synchronize": (_I, [_P, _PE]),
     "clb_warm_execute": (_I, [_P, _U32, _P, _P, _I, _P, _P, HOST_EXPERT_FN, _P, _P, _PE]),
+    "clb_route_experts_device": (_I, [C.POINTER(RouteConfigV1), _P, _I64, _P, _I, _P, _P, _P, _P, _PE]),
+    "clb_block_norm_device": (_I, [C.POINTER(BlockNormConfigV1), _I, _P, _P, _P, _P, _P, _P, _P, _P, _PE]),
+    "clb_int8_quantize_device": (_I, [_I, _P, _I64, _I, _I, _P, _I64, _P, _P, _PE]),
+    "clb_int8_linear_workspace_bytes": (C.c_uint64, [_I, _I]),
+    "clb_int8_linear_device": (_I, [C.POINTER(Int8LinearConfigV1), _P, _P, _P, _I, _P, _P, _P, _P, C.c_uint64, _P, _P,
+                                    _PE]),
     "clb_expert_forward_noalloc": (_I, [_I, _P, _P, _P, _P, _P, _I, _I, _F, _P, _PE]),
 }
 

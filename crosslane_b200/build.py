@@ -24,7 +24,7 @@ LIB = os.path.join(HERE, "libcrosslane_b200.so")
 BUILD_TRACE = os.path.join(HERE, "_build_trace")
 LIB_TRACE = os.path.join(HERE, "libcrosslane_b200_trace.so")
 SOURCES = ["clb_kernels.cu", "clb_bank.cu", "clb_noalloc.cu", "clb_stack.cu", "clb_prefill.cu",
-           "clb_pack_io.cu"]
+           "clb_pack_io.cu", "clb_route.cu", "clb_block_norm.cu", "clb_int8.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-contract=off,-fno-fast-math",

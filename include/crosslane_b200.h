@@ -462,6 +462,127 @@ int32_t clb_expert_forward_noalloc(int32_t type, const void* w_gate, const void*
                                    const float* x, float* y, int32_t dim, int32_t ff, float limit, void* stream,
                                    clb_error_v1* err);
 
+/* ---- operators around the routed experts of a layer (device pointers, caller stream) ----
+ * Routing, the norms with the gated residual step, and the 8-bit integer product of the
+ * shared expert and the dense projections. They run on the current device's `stream`
+ * (NULL = legacy default stream), allocate nothing, do not synchronise, may be captured into
+ * a graph, and check every argument before they touch the GPU. Zero tokens are no work and
+ * no error. Rows are pitched: `ld_*` is the distance of two rows in elements (>= the row's
+ * length). No counterpart in crosslane's lanes. */
+
+/* Element types. */
+#define CLB_F32 0
+#define CLB_BF16 1
+#define CLB_F16 2
+#define CLB_I8 3
+
+/* Routing scores of clb_route_experts_device. */
+#define CLB_SCORE_SIGMOID 0
+#define CLB_SCORE_SOFTMAX 1
+#define CLB_SCORE_SQRT_SOFTPLUS 2
+/* A group's value: its best rank value, or the fp32 sum of its two best scores. */
+#define CLB_GROUP_MAX 1
+#define CLB_GROUP_PAIR 2
+
+typedef struct clb_route_config_v1 {
+    int32_t n_experts;    /* 1..1024 */
+    int32_t k;            /* picks per token, 1..16, <= the experts of top_groups groups */
+    int32_t score;        /* CLB_SCORE_* */
+    int32_t n_groups;     /* 1..32, divides n_experts; 1 = no groups */
+    int32_t top_groups;   /* 1..n_groups groups that stay */
+    int32_t group_score;  /* CLB_GROUP_* (read when n_groups > 1) */
+    int32_t renormalize;  /* 1: weights over the picks' sum + 1e-20 */
+    float scale;          /* factor of the weights, finite, >= 0 */
+    int32_t logits_type;  /* CLB_F32, CLB_BF16 or CLB_F16 */
+    int32_t reserved[3];  /* 0 */
+} clb_route_config_v1;
+
+/* Picks of `tokens` rows of logits [tokens][n_experts]: d_ids [tokens][k] int32, d_w
+ * [tokens][k] fp32, best first.
+ *   s = sigmoid(l), softmax(l) or sqrt(softplus(l)), correctly rounded to fp32;
+ *   rank = fl(s + d_bias[e]), or the logit itself without a bias (s rises with l);
+ *   with groups, those top_groups with the largest value stay (ties to the lower group):
+ *   CLB_GROUP_MAX the largest rank, CLB_GROUP_PAIR the fp32 sum of the two largest
+ *   s + bias (s without a bias);
+ *   the k largest ranks are picked, ties to the lower id;
+ *   w = s, divided by (sum of the picks' s + 1e-20) if renormalize, times scale.
+ * An expert whose logit or bias is -inf is not available (it still counts in the softmax
+ * if only its bias is -inf). Places left over take the remaining ids in ascending order
+ * with weight 0, so the ids of a token are always distinct and in range: a row with no
+ * available expert gives ids 0..k-1 and weights 0. A row with a NaN or +inf in its logits
+ * (or any such bias) gives ids 0..k-1 and NaN weights, and sets *d_status (int32, may be
+ * NULL) to 1; the other rows are not touched by it. */
+int32_t clb_route_experts_device(const clb_route_config_v1* cfg, const void* d_logits, int64_t ld_logits,
+                                 const float* d_bias, int32_t tokens, int32_t* d_ids, float* d_w, int32_t* d_status,
+                                 void* stream, clb_error_v1* err);
+
+/* Gate of clb_block_norm_device: none, one number per channel, per token, or for each. */
+#define CLB_GATE_NONE 0
+#define CLB_GATE_CHANNEL 1
+#define CLB_GATE_TOKEN 2
+#define CLB_GATE_FULL 3
+
+typedef struct clb_block_norm_config_v1 {
+    int32_t dim;           /* 1..32768 */
+    int32_t post;          /* 1: RMSNorm of y before it is added */
+    int32_t gate;          /* CLB_GATE_* */
+    int32_t gate_sigmoid;  /* 1: the gate is sigmoid(gate) */
+    int32_t h_type, y_type, gate_type, x_type; /* CLB_F32, CLB_BF16 or CLB_F16 */
+    float post_eps, pre_eps;             /* > 0 */
+    float residual_scale, block_scale;   /* finite */
+    int64_t ld_h, ld_y, ld_gate, ld_h_out, ld_x; /* row pitches (ld_gate for CLB_GATE_FULL) */
+    int32_t reserved[4];   /* 0 */
+} clb_block_norm_config_v1;
+
+/* The residual step between two blocks, one pass over the rows:
+ *   z  = post ? y / sqrt(mean(y^2) + post_eps) * w_post : y
+ *   h' = residual_scale * h + block_scale * g * z          (g: the gate, 1 without one)
+ *   x  = h' / sqrt(mean(h'^2) + pre_eps) * w_pre
+ * d_h [tokens][dim] is the residual stream, d_y the block's output, d_h_out receives h'
+ * (may be d_h itself) and d_x (NULL: none) the next block's input. d_y NULL: h' = h, only x
+ * is written, and d_h_out, d_gate and d_w_post have to be NULL. d_w_post, d_w_pre [dim] fp32,
+ * NULL = ones. Sums and h' are fp32 (x comes from h' before it is rounded to h_type); the
+ * order of a row's sum depends on dim and the row count's class alone, so results repeat.
+ * Apart from d_h_out = d_h with the same type and pitch, an output overlaps no input. */
+int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, int32_t tokens, const void* d_h, const void* d_y,
+                              const void* d_gate, const float* d_w_post, const float* d_w_pre, void* d_h_out,
+                              void* d_x, void* stream, clb_error_v1* err);
+
+/* Rows in 8-bit integers, a scale for each row: scale = fl(max |x| / 127), q = x / scale
+ * rounded to the nearest integer (ties to even, exact quotient), |q| <= 127. Rows: tokens of
+ * an activation, or output channels of a weight matrix. x [rows][k] of `type` (CLB_F32,
+ * CLB_BF16, CLB_F16), q [rows][ld_q] int8 with ld_q % 16 == 0 and q 16-byte aligned; columns
+ * k..ld_q-1 are not written. A row of zeros (or whose scale is 0 in fp32) has scale 0 and
+ * q = 0; a row with a NaN or an infinity has scale NaN and q = 0. k <= 131072. */
+int32_t clb_int8_quantize_device(int32_t type, const void* d_x, int64_t ld_x, int32_t rows, int32_t k, int8_t* d_q,
+                                 int64_t ld_q, float* d_scale, void* stream, clb_error_v1* err);
+
+typedef struct clb_int8_linear_config_v1 {
+    int32_t n, k;              /* weight matrix [n][k]; k <= 131072 */
+    int32_t x_type;            /* CLB_F32, CLB_BF16, CLB_F16 (quantised by the call) or CLB_I8 */
+    int32_t out_type;          /* CLB_F32, CLB_BF16 or CLB_F16 */
+    int64_t ld_w, ld_x, ld_out;/* row pitches; ld_w (and ld_x for CLB_I8) a multiple of 16 */
+    int32_t reserved[4];       /* 0 */
+} clb_int8_linear_config_v1;
+
+/* Workspace of clb_int8_linear_device: the quantised activation and its scales. */
+uint64_t clb_int8_linear_workspace_bytes(int32_t tokens, int32_t k);
+
+/* out[t][n] = x_scale[t] * w_scale[n] * sum_k q[t][k] w[n][k] + bias[n], the sum exact in
+ * 32-bit integers, the products and the bias in fp32, rounded once more to out_type.
+ * d_w [n][ld_w] int8 and d_w_scale [n] fp32 (clb_int8_quantize_device of the weights makes
+ * both), d_bias [n] fp32 or NULL. x of a floating type is quantised per token as
+ * clb_int8_quantize_device does (d_x_scale NULL); CLB_I8 x brings its scales in d_x_scale.
+ * d_w, d_ws and CLB_I8 x are 16-byte aligned. d_ws (ws_bytes >= the size above; may be NULL
+ * for CLB_I8) is the caller's: calls that overlap on the GPU need one each. A token whose
+ * scale is NaN gives a row of NaN. The result does not depend on the other tokens of the
+ * call. *d_status (int32, may be NULL) becomes 3 if a bounded wait in the kernel ran out
+ * (the output is then incomplete). */
+int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, const int8_t* d_w, const float* d_w_scale,
+                               const float* d_bias, int32_t tokens, const void* d_x, const float* d_x_scale,
+                               void* d_out, void* d_ws, uint64_t ws_bytes, int32_t* d_status, void* stream,
+                               clb_error_v1* err);
+
 /* ---- warm_execute: the three-lane join with this bank as the GPU lane ---- */
 
 /* Host lane callback: compute y[dim] of one non-resident expert (crosslane's

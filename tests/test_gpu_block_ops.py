@@ -1,0 +1,635 @@
+"""The operators around the routed experts on the GPU against plain definitions in 64 bits.
+
+Tolerances come from counting roundings: u = 2^-24 (half a step of fp32) for every fp32
+operation, and half a step of the output's type for the last one.
+"""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = ("float32", "bfloat16", "float16")
+TINY = {"float32": 2.0 ** -150, "bfloat16": 2.0 ** -134, "float16": 2.0 ** -25}  # half the least subnormal
+
+
+@pytest.fixture(scope="module")
+def cb(cuda):
+    import crosslane_b200
+    return crosslane_b200
+
+
+def half_step(torch, name):
+    return torch.finfo(getattr(torch, name)).eps / 2
+
+
+def pitched(torch, values, dtype, pad):
+    """values [T][W] in rows of a buffer that is `pad` elements wider, the rest a canary."""
+    t = torch.full((values.shape[0], values.shape[1] + pad), 7.0, dtype=dtype, device="cuda")
+    v = t[:, : values.shape[1]]
+    v.copy_(torch.as_tensor(values))
+    return v
+
+
+# ---------------------------------------------------------------------------- routing
+
+def scores64(kind, l):
+    there = ~np.isneginf(l)
+    low = np.where(there, l, 0.0)
+    with np.errstate(over="ignore"):
+        if kind == "sigmoid":
+            return 1.0 / (1.0 + np.exp(-low))
+        if kind == "sqrt_softplus":
+            return np.sqrt(np.maximum(low, 0.0) + np.log1p(np.exp(-np.abs(low))))
+    top = np.where(there, l, -np.inf).max()
+    if np.isneginf(top):
+        return np.zeros_like(l)
+    e = np.where(there, np.exp(np.where(there, l - top, 0.0)), 0.0)
+    return e / e.sum()
+
+
+def route64(l32, bias, k, kind, groups, top_groups, pair, renorm, scale):
+    """One row by the definition: (ids, weights, is the row bad)."""
+    E = l32.size
+    if not np.all(l32 < np.inf) or (bias is not None and not np.all(bias < np.inf)):
+        return np.arange(k), np.full(k, np.nan), True
+    s = scores64(kind, l32.astype(np.float64))
+    held = s.astype(np.float32)
+    there = ~np.isneginf(l32) if bias is None else ~(np.isneginf(l32) | np.isneginf(bias))
+    ninf = np.float32(-np.inf)
+    with_bias = held if bias is None else held + bias
+    rank = np.where(there, l32 if bias is None else with_bias, ninf)
+    if groups > 1:
+        per = E // groups
+        value = np.empty(groups, np.float32)
+        for g in range(groups):
+            own = np.sort(np.where(there, with_bias, ninf)[g * per:(g + 1) * per])[::-1]
+            if pair:
+                value[g] = own[0] if per == 1 or np.isneginf(own[1]) else own[0] + own[1]
+            else:
+                value[g] = rank[g * per:(g + 1) * per].max()
+        for g in np.argsort(-value, kind="stable")[top_groups:]:
+            rank[g * per:(g + 1) * per] = ninf
+    ids = np.argsort(-rank, kind="stable")[:k]
+    w = np.where(np.isneginf(rank[ids]), 0.0, s[ids])
+    if renorm:
+        w = w / (w.sum() + 1e-20)
+    return ids, w * scale, False
+
+
+def check_route(torch, op, logits, bias, ids, w, kind, groups=1, top_groups=1, pair=True, renorm=True, scale=1.0):
+    k = op.k
+    l32 = logits.float().cpu().numpy()
+    b = None if bias is None else bias.cpu().numpy()
+    gi, gw = ids.cpu().numpy(), w.cpu().numpy().astype(np.float64)
+    bad_rows = 0
+    for t in range(l32.shape[0]):
+        wi, ww, bad = route64(l32[t], b, k, kind, groups, top_groups, pair, renorm, scale)
+        bad_rows += bad
+        assert np.array_equal(gi[t], wi), (t, gi[t], wi)
+        if bad:
+            assert np.all(np.isnan(gw[t])), t
+            continue
+        # a score, the k additions of the sum, its 1e-20, the division, the scale: k + 4 roundings;
+        # scores below the normal numbers lose at most half a subnormal step each, times w / s <= scale / sum
+        tol = (k + 4) * U * np.abs(ww) + 2.0 ** -149 * max(1.0, scale)
+        if renorm:
+            s = scores64(kind, l32[t].astype(np.float64))[wi]
+            tol += 2.0 ** -150 * (k + 1) * scale / (np.where(ww > 0, s, 0.0).sum() + 1e-20)
+        assert np.all(np.abs(gw[t] - ww) <= tol), (t, gw[t], ww)
+    return bad_rows
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+@pytest.mark.parametrize("E,k,groups,top,pair", [(1, 1, 1, 1, True), (2, 2, 1, 1, True), (31, 16, 1, 1, True),
+                                                 (100, 6, 1, 1, True), (128, 8, 1, 1, True), (384, 6, 1, 1, True),
+                                                 (384, 8, 8, 4, True), (384, 8, 8, 4, False), (256, 8, 32, 3, True),
+                                                 (96, 5, 3, 2, True), (32, 3, 32, 3, True), (352, 7, 11, 2, False),
+                                                 (1024, 16, 1, 1, True), (1000, 16, 4, 1, True)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_route_matches_definition(cb, cuda, kind, E, k, groups, top, pair, with_bias):
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(E * 31 + k)
+    T = 67
+    logits = torch.randn((T, E), generator=gen, device="cuda") * 3
+    if E > 8:  # masked experts, ties, extremes, a row with few experts, an empty row
+        logits[1::5] = torch.where(torch.rand((len(range(1, T, 5)), E), generator=gen, device="cuda") < 0.4, -math.inf,
+                                   logits[1::5])
+        logits[2] = 0.25
+        logits[3, ::2] = 1.0
+        logits[4] = torch.linspace(-120, 120, E, device="cuda")
+        logits[5] = -math.inf
+        logits[6] = -math.inf
+        logits[6, E - 2] = -2.0
+        logits[7] = torch.finfo(torch.float32).min
+        logits[7, 4] = 0.0
+        logits[8, ::3] = -0.0
+        logits[8, 1::3] = 0.0
+    bias = torch.randn(E, generator=gen, device="cuda") * 0.3 if with_bias else None
+    if with_bias and E > 8:
+        bias[5] = -math.inf
+    op = cb.ExpertRoute(E, k, score=kind, n_groups=groups, top_groups=top, group_score="pair" if pair else "max",
+                        renormalize=E % 3 != 1, scale=2.5)
+    ids = torch.full((T, k), -7, dtype=torch.int32, device="cuda")
+    w = torch.full((T, k), -7.0, device="cuda")
+    op.run(logits, ids, w, d_bias=bias)
+    assert check_route(torch, op, logits, bias, ids, w, kind, groups, top, pair, E % 3 != 1, 2.5) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_route_types_and_pitches(cb, cuda, dtype, pad):
+    torch = cuda
+    T, E, k = 130, 384, 6
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    logits = pitched(torch, torch.randn((T, E), generator=gen, device="cuda") * 2, getattr(torch, dtype), pad)
+    bias = torch.randn(E, generator=gen, device="cuda") * 0.1
+    op = cb.ExpertRoute(E, k, scale=1.5)
+    back = torch.full((T + 2, k), -7, dtype=torch.int32, device="cuda")
+    wback = torch.full((T + 2, k), -7.0, device="cuda")
+    op.run(logits, back[:T], wback[:T], d_bias=bias)
+    check_route(torch, op, logits, bias, back[:T], wback[:T], "sigmoid", scale=1.5)
+    assert bool((back[T:] == -7).all()) and bool((wback[T:] == -7).all())  # rows behind the last stay
+
+
+@pytest.mark.parametrize("T", [0, 1, 2, 5, 4099])
+def test_route_token_counts(cb, cuda, T):
+    torch = cuda
+    E, k = 48, 4
+    logits = torch.randn((T, E), generator=torch.Generator(device="cuda").manual_seed(T), device="cuda")
+    ids = torch.empty((T, k), dtype=torch.int32, device="cuda")
+    w = torch.empty((T, k), device="cuda")
+    op = cb.ExpertRoute(E, k, score="softmax", renormalize=False)
+    op.run(logits, ids, w)
+    check_route(torch, op, logits, None, ids, w, "softmax", renorm=False)
+
+
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_route_flags_bad_rows_alone(cb, cuda, with_bias):
+    torch = cuda
+    T, E, k = 9, 384, 6
+    logits = torch.randn((T, E), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    logits[2, 17] = math.nan
+    logits[4, 383] = math.inf
+    bias = torch.zeros(E, device="cuda") if with_bias else None
+    ids = torch.empty((T, k), dtype=torch.int32, device="cuda")
+    w = torch.empty((T, k), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    op = cb.ExpertRoute(E, k)
+    op.run(logits, ids, w, d_bias=bias, d_status=status)
+    assert check_route(torch, op, logits, bias, ids, w, "sigmoid") == 2 and int(status) == 1
+    status.zero_()
+    op.run(logits[5:], ids[5:], w[5:], d_bias=bias, d_status=status)
+    assert int(status) == 0
+    if with_bias:
+        bias[3] = math.nan
+        op.run(logits, ids, w, d_bias=bias, d_status=status)
+        assert int(status) == 1 and bool(torch.isnan(w).all()) and bool((ids == torch.arange(k, device="cuda")).all())
+
+
+def test_route_agrees_with_the_modes_there_were(cb, cuda):
+    """Sigmoid without a bias is mode 0's choice; sqrt-softplus with a bias is mode 1's."""
+    torch = cuda
+    T, E, k = 513, 384, 6
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    logits = torch.randn((T, E), generator=gen, device="cuda") * 2
+    bias = torch.randn(E, generator=gen, device="cuda") * 0.1
+    new = lambda d: torch.empty((T, k), dtype=d, device="cuda")  # noqa: E731
+    a, aw, b, bw = new(torch.int32), new(torch.float32), new(torch.int32), new(torch.float32)
+    cb.route_device(logits, E, k, T, a, aw)
+    cb.ExpertRoute(E, k).run(logits, b, bw)
+    assert torch.equal(a, b) and torch.allclose(aw, bw, rtol=2 * (k + 4) * U, atol=0)
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cb.route_b_device(logits, bias, k, 2.5, a, aw, st)
+    cb.ExpertRoute(E, k, score="sqrt_softplus", scale=2.5).run(logits, b, bw, d_bias=bias)
+    # mode 1 rounds exp and log1p one after the other: its scores may be an ulp or two apart
+    same = (a == b).all(dim=1)
+    assert float(same.float().mean()) > 0.999
+    assert torch.allclose(aw[same], bw[same], rtol=2 * (k + 8) * U, atol=0)
+
+
+# ------------------------------------------------------------------------------ norms
+
+def norm64(h, y, g, w_post, w_pre, post, gate, sig, r, b, eps):
+    """(h', x, r h, b g z) in 64 bits."""
+    D = h.shape[1]
+    rh, bz = h, np.zeros_like(h)
+    if y is not None:
+        z = y
+        if post:
+            z = y / np.sqrt((y * y).sum(1, keepdims=True) / D + eps) * (1.0 if w_post is None else w_post)
+        if g is not None:
+            g = 1.0 / (1.0 + np.exp(-g)) if sig else g
+            z = z * (g[:, None] if gate == "token" else g)
+        rh, bz = r * h, b * z
+    new = rh + bz
+    x = new / np.sqrt((new * new).sum(1, keepdims=True) / D + eps) * (1.0 if w_pre is None else w_pre)
+    return new, x, rh, bz
+
+
+def check_norm(torch, got, want, parts, D, dtype, inv_w=None):
+    """Roundings: a row's sum of squares is a chain of at most 128 products and additions per
+    thread (dim <= 32768) and 10 tree additions; its root's reciprocal halves that relative
+    error and adds 6 operations of its own: (138 / 2 + 6) u = 75 u. z takes it once and 5 more
+    products, a sigmoid gate 8 u (expf within 2 ulp, an addition, a division), h' two
+    roundings. x takes the error of h' and its own root."""
+    rh, bz = parts
+    err_h = 90 * U * (np.abs(rh) + np.abs(bz))
+    u_t = half_step(torch, dtype)
+    if inv_w is None:
+        tol = err_h + (u_t + U) * np.abs(want)
+    else:
+        # a relative change of every h' by at most e changes the root by e * |h'|'s own share
+        share = np.sqrt((err_h ** 2).sum(1, keepdims=True) / np.maximum((inv_w[1] ** 2).sum(1, keepdims=True), 1e-300))
+        tol = err_h * np.abs(inv_w[0]) + (share + 80 * U + u_t) * np.abs(want)
+    tol = 1.01 * tol + TINY[dtype]
+    assert np.all(np.isfinite(want))
+    assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / tol).max()
+
+
+def run_norm(cb, torch, T, D, h_t="float32", y_t="float32", x_t="float32", gate="none", sig=False, post=True, pre=True,
+             weights=True, pad=0, seed=1, with_y=True, in_place=False, r=0.75, b=1.25, eps=1e-5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    dt = lambda n: getattr(torch, n)  # noqa: E731
+    h = pitched(torch, rnd(T, D) * 3, dt(h_t), pad)
+    y = pitched(torch, rnd(T, D) * 0.4, dt(y_t), pad) if with_y else None
+    shape = {"none": None, "channel": (D,), "token": (T,), "full": (T, D)}[gate]
+    g = None if shape is None or not with_y else rnd(*shape).to(dt(y_t))
+    if gate == "full" and g is not None:
+        g = pitched(torch, g, dt(y_t), pad)
+    w_post = 1 + 0.3 * rnd(D) if post and weights and with_y else None
+    w_pre = 1 + 0.3 * rnd(D) if pre and weights else None
+    h64 = h.double().cpu().numpy()
+    h_out = None if not with_y else h if in_place else pitched(torch, rnd(T, D), dt(h_t), pad)
+    x = pitched(torch, rnd(T, D), dt(x_t), pad) if pre else None
+    op = cb.BlockNorm(D, post=post, pre=pre, eps=eps, gate=gate if with_y else "none", gate_sigmoid=sig,
+                      residual_scale=r, block_scale=b)
+    op.run(h, d_y=y, d_gate=g, d_w_post=w_post, d_w_pre=w_pre, d_h_out=h_out, d_x=x)
+    n64 = lambda t: None if t is None else t.double().cpu().numpy()  # noqa: E731
+    new, xw, rh, bz = norm64(h64, n64(y), n64(g), n64(w_post), n64(w_pre), post, gate, sig, r, b, eps)
+    if with_y:
+        check_norm(torch, n64(h_out), new, (rh, bz), D, h_t)
+    if pre:
+        inv = np.abs(xw) / np.maximum(np.abs(new), 1e-300)
+        check_norm(torch, n64(x), xw, (rh, bz), D, x_t, (inv, new))
+    for t in (h_out, x):  # what lies between the rows stays
+        if t is not None and pad:
+            assert bool((t._base[:, D:] == 7).all())
+    return h_out, x
+
+
+@pytest.mark.parametrize("D", [1, 7, 8, 64, 100, 1000, 2047, 2311, 5120, 7168, 8192, 8200, 16384, 16391, 32768])
+@pytest.mark.parametrize("T", [1, 3, 150])
+def test_norm_widths(cb, cuda, T, D):
+    run_norm(cb, cuda, T, D, gate="channel")
+
+
+@pytest.mark.parametrize("h_t", TYPES)
+@pytest.mark.parametrize("y_t", TYPES)
+@pytest.mark.parametrize("x_t", TYPES)
+def test_norm_types(cb, cuda, h_t, y_t, x_t):
+    run_norm(cb, cuda, 5, 768, h_t, y_t, x_t, gate="full", sig=True, seed=2)
+    run_norm(cb, cuda, 300, 331, h_t, y_t, x_t, gate="full", sig=True, seed=3)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("sig", [False, True])
+@pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("D", [512, 515])
+def test_norm_parts(cb, cuda, gate, sig, post, pre, D):
+    run_norm(cb, cuda, 37, D, gate=gate, sig=sig, post=post, pre=pre, y_t="bfloat16")
+
+
+@pytest.mark.parametrize("pad", [1, 4, 5, 8])
+@pytest.mark.parametrize("h_t", ["float32", "bfloat16"])
+def test_norm_pitches(cb, cuda, pad, h_t):
+    run_norm(cb, cuda, 33, 1024, h_t, "float16", "bfloat16", gate="full", pad=pad)
+
+
+def test_norm_without_weights_or_block(cb, cuda):
+    run_norm(cb, cuda, 9, 1024, weights=False)
+    run_norm(cb, cuda, 9, 7168, with_y=False)
+    run_norm(cb, cuda, 2000, 640, with_y=False, x_t="bfloat16")
+
+
+@pytest.mark.parametrize("T,D", [(1, 7168), (600, 1000), (5, 16384)])
+def test_norm_in_place(cb, cuda, T, D):
+    a = run_norm(cb, cuda, T, D, in_place=True, seed=4)
+    b = run_norm(cb, cuda, T, D, in_place=False, seed=4)
+    assert cuda.equal(a[0], b[0]) and cuda.equal(a[1], b[1])
+
+
+def test_norm_zero_and_nonfinite_rows_stay_alone(cb, cuda):
+    torch = cuda
+    T, D = 6, 512
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    h = torch.randn((T, D), generator=gen, device="cuda")
+    y = torch.randn((T, D), generator=gen, device="cuda")
+    clean_h, clean_x = torch.empty_like(h), torch.empty_like(h)
+    op = cb.BlockNorm(D)
+    op.run(h, d_y=y, d_h_out=clean_h, d_x=clean_x)
+    h2, y2 = h.clone(), y.clone()
+    y2[1] = 0.0
+    h2[2], y2[2] = 0.0, 0.0
+    y2[3, 5] = math.nan
+    h2[4, 6] = math.inf
+    out_h, out_x = torch.empty_like(h), torch.empty_like(h)
+    op.run(h2, d_y=y2, d_h_out=out_h, d_x=out_x)
+    assert torch.equal(out_h[[0, 5]], clean_h[[0, 5]]) and torch.equal(out_x[[0, 5]], clean_x[[0, 5]])
+    assert torch.equal(out_h[1], h2[1])            # a zero row adds nothing: 0 / sqrt(eps)
+    assert bool((out_h[2] == 0).all()) and bool((out_x[2] == 0).all())
+    assert bool(torch.isnan(out_h[3]).all()) and bool(torch.isnan(out_x[3]).all())
+    assert float(out_h[4, 6]) == math.inf and bool(torch.isnan(out_x[4, 6]))
+
+
+# ------------------------------------------------------------------------------- int8
+
+def quant64(x):
+    """(q, scale) of rows by the definition: the scale held in fp32, the exact quotient's nearest integer."""
+    m = np.abs(x).max(axis=1)
+    s = (m / 127.0).astype(np.float32)
+    bad = ~np.isfinite(m)
+    d = np.where((s > 0) & ~bad, s, 1.0).astype(np.float64)[:, None]
+    q = np.clip(np.rint(np.where(bad[:, None], 0.0, x) / d), -127, 127)
+    q[(s == 0) | bad] = 0
+    return q, np.where(bad, np.nan, s.astype(np.float64))
+
+
+def padded_int8(torch, rows, k, extra=0):
+    return torch.full((rows, (k + 15) // 16 * 16 + extra), 99, dtype=torch.int8, device="cuda")[:, :k]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k,pad,extra", [(1, 1, 0, 0), (1, 7168, 0, 0), (3, 15, 1, 16), (5, 16, 0, 0), (9, 100, 5, 0),
+                                              (300, 1536, 0, 0), (64, 2311, 3, 32), (7, 131072, 0, 0), (2, 20000, 8, 0)])
+def test_quantize_exact(cb, cuda, dtype, rows, k, pad, extra):
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(rows + k)
+    x = torch.randn((rows, k), generator=gen, device="cuda")
+    if rows > 4:
+        x[1] = 0.0
+        x[2] *= 2.0 ** -14
+        x[3] = torch.round(x[3] * 8) * 0.5  # many quotients on or near a border
+        x[3, 0] = 127.0
+    x = pitched(torch, x, getattr(torch, dtype), pad)
+    q, s = padded_int8(torch, rows, k, extra), torch.full((rows + 1,), -7.0, device="cuda")
+    cb.int8_quantize(x, q, s[:rows])
+    wq, ws = quant64(x.double().cpu().numpy())
+    assert np.array_equal(s[:rows].double().cpu().numpy(), ws) and float(s[rows]) == -7
+    assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8))
+    assert bool((q._base[:, k:] == 99).all())  # columns behind the row stay
+
+
+def test_quantize_borders_and_small_scales(cb, cuda):
+    """Quotients a rounding away from a half, exact halves, subnormal rows and scales."""
+    torch = cuda
+    rng = np.random.default_rng(2)
+    rows, k = 400, 256
+    x = np.zeros((rows, k), np.float32)
+    for r in range(rows):
+        m = np.float32(rng.uniform(1, 2) * 2.0 ** int(rng.integers(-148, 120)))
+        s = np.float32(np.float64(m) / 127.0)
+        half = (rng.integers(-127, 127, k) + 0.5) * np.float64(s)
+        x[r] = half.astype(np.float32)  # the representable numbers next to the borders
+        x[r, ::3] = np.nextafter(x[r, ::3], np.float32(np.inf))
+        x[r, 1::3] = np.nextafter(x[r, 1::3], np.float32(-np.inf))
+        x[r] = np.clip(x[r], -m, m)
+        x[r, 7] = m
+    q, s = padded_int8(torch, rows, k), torch.empty(rows, device="cuda")
+    cb.int8_quantize(torch.from_numpy(x).cuda(), q, s)
+    wq, ws = quant64(x.astype(np.float64))
+    assert np.array_equal(s.double().cpu().numpy(), ws)
+    assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8))
+
+
+def test_quantize_nonfinite_rows(cb, cuda):
+    torch = cuda
+    x = torch.randn((4, 64), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    x[1, 3], x[2, 60] = math.nan, -math.inf
+    q, s = padded_int8(torch, 4, 64), torch.empty(4, device="cuda")
+    cb.int8_quantize(x, q, s)
+    wq, ws = quant64(x.double().cpu().numpy())
+    assert np.array_equal(s.double().cpu().numpy(), ws, equal_nan=True)
+    assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8))
+
+
+def linear_case(cb, torch, T, K, N, x_t="float32", out_t="float32", bias=False, pad=0, seed=0, ready=False, extra=0,
+                bad_row=None):
+    gen = torch.Generator(device="cuda").manual_seed(seed + T + K + N)
+    w = padded_int8(torch, N, K, extra)
+    w.copy_(torch.randint(-127, 128, (N, K), generator=gen, device="cuda").to(torch.int8))
+    ws = torch.rand(N, generator=gen, device="cuda") * 0.01 + 1e-4
+    b = torch.randn(N, generator=gen, device="cuda") if bias else None
+    x = torch.randn((T, K), generator=gen, device="cuda")
+    if bad_row is not None:
+        x[bad_row, K // 2] = math.nan
+    back = torch.full((T + 1, N + pad), 7.0, dtype=getattr(torch, out_t), device="cuda")
+    out = back[:T, :N]
+    op = cb.Int8Linear(w, ws, b)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    if ready:
+        q, xs = padded_int8(torch, T, K, extra), torch.empty(T, device="cuda")
+        cb.int8_quantize(x, q, xs)
+        op.run(q, out, d_x_scale=xs, d_status=status)
+    else:
+        x = pitched(torch, x, getattr(torch, x_t), pad)
+        wsp = torch.empty(op.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+        op.run(x, out, d_ws=wsp, d_status=status)
+    assert int(status) == 0
+    wq, wxs = quant64(x.double().cpu().numpy())
+    acc = (torch.from_numpy(wq).cuda() @ w.double().t()).cpu().numpy()  # integers below 2^53: exact
+    v = acc * wxs[:, None] * ws.double().cpu().numpy()[None, :]
+    want = v if b is None else v + b.double().cpu().numpy()[None, :]
+    got = out.double().cpu().numpy()
+    good = np.isfinite(wxs)
+    assert np.all(np.isnan(got[~good]))
+    # the sum to fp32, two products, the bias, the output type
+    tol = 1.01 * (3 * U * np.abs(v) + (U + half_step(torch, out_t)) * np.abs(want)) + TINY[out_t]
+    assert np.all(np.abs(got - want)[good] <= tol[good]), (np.abs(got - want)[good] / tol[good]).max()
+    assert bool((back[T:] == 7).all()) and bool((back[:, N:] == 7).all())  # nothing behind the rows or the last row
+    return out.clone()
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 7, 8, 9, 16, 17, 31, 33, 64, 65, 100, 128, 129, 255, 257, 500])
+def test_linear_token_counts(cb, cuda, T):
+    linear_case(cb, cuda, T, 1024, 768)
+
+
+@pytest.mark.parametrize("K", [1, 15, 16, 17, 31, 100, 127, 128, 129, 255, 1000, 2311, 7168, 20000, 131072])
+@pytest.mark.parametrize("T", [1, 6, 40, 300])
+def test_linear_depths(cb, cuda, T, K):
+    linear_case(cb, cuda, T, K, 136, extra=16 if K % 3 == 0 else 0)
+
+
+@pytest.mark.parametrize("N", [1, 2, 31, 127, 128, 129, 250, 1001, 2304])
+@pytest.mark.parametrize("T", [1, 5, 48, 270])
+def test_linear_widths(cb, cuda, T, N):
+    linear_case(cb, cuda, T, 512, N, out_t="bfloat16", bias=True)
+
+
+@pytest.mark.parametrize("x_t", TYPES)
+@pytest.mark.parametrize("out_t", TYPES)
+@pytest.mark.parametrize("T", [1, 4, 20, 200])
+@pytest.mark.parametrize("pad", [0, 3, 8])
+def test_linear_types_and_pitches(cb, cuda, x_t, out_t, T, pad):
+    linear_case(cb, cuda, T, 640, 300, x_t, out_t, bias=pad == 3, pad=pad)
+
+
+@pytest.mark.parametrize("T", [1, 3, 12, 70, 300])
+@pytest.mark.parametrize("K,extra", [(512, 0), (1000, 32)])
+def test_linear_int8_input(cb, cuda, T, K, extra):
+    a = linear_case(cb, cuda, T, K, 320, ready=True, extra=extra)
+    b = linear_case(cb, cuda, T, K, 320, ready=False, extra=extra)
+    assert cuda.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [1, 2, 30, 300])
+def test_linear_nan_row_stays_alone(cb, cuda, T):
+    linear_case(cb, cuda, T, 256, 200, bad_row=T // 2)
+
+
+def test_linear_extreme_sums(cb, cuda):
+    """The largest integer sums: 127 * 127 * 131072 is below 2^31."""
+    torch = cuda
+    K, N = 131072, 40
+    for T in (1, 5, 40):
+        w = torch.full((N, K), 127, dtype=torch.int8, device="cuda")
+        w[1::2] = -127
+        q = torch.full((T, K), 127, dtype=torch.int8, device="cuda")
+        out = torch.empty((T, N), device="cuda")
+        cb.Int8Linear(w, torch.ones(N, device="cuda")).run(q, out, d_x_scale=torch.ones(T, device="cuda"))
+        want = float(np.float32(127 * 127 * K))
+        assert bool((out[:, ::2] == want).all()) and bool((out[:, 1::2] == -want).all())
+
+
+def test_linear_does_not_depend_on_the_batch(cb, cuda):
+    """A token's row has the same bits alone and in any batch (exact sums)."""
+    torch = cuda
+    K, N = 2048, 512
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    w = torch.randint(-127, 128, (N, K), generator=gen, device="cuda").to(torch.int8)
+    op = cb.Int8Linear(w, torch.rand(N, generator=gen, device="cuda"))
+    x = torch.randn((600, K), generator=gen, device="cuda")
+    ws = torch.empty(op.workspace_bytes(600), dtype=torch.uint8, device="cuda")
+    full = torch.empty((600, N), device="cuda")
+    op.run(x, full, d_ws=ws)
+    for T in (1, 2, 5, 13, 40, 64, 150, 300):
+        part = torch.empty((T, N), device="cuda")
+        op.run(x[:T], part, d_ws=ws)
+        assert torch.equal(part, full[:T]), T
+
+
+# ----------------------------------------------------------- streams, graphs, the run of them
+
+def test_streams_and_graphs(cb, cuda):
+    """Another stream's calls, and a captured step replayed on new inputs, give the eager bits."""
+    torch = cuda
+    T, D, E, k, N = 24, 1024, 96, 4, 640
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    w = torch.randint(-127, 128, (N, D), generator=gen, device="cuda").to(torch.int8)
+    lin = cb.Int8Linear(w, torch.rand(N, generator=gen, device="cuda") * 0.01)
+    route, norm = cb.ExpertRoute(E, k, n_groups=8, top_groups=4), cb.BlockNorm(D)
+    bias = rnd(E) * 0.1
+    s = dict(h=rnd(T, D), y=rnd(T, D), l=rnd(T, E), h2=rnd(T, D), x=rnd(T, D), o=rnd(T, N), w=rnd(T, k),
+             ids=torch.empty((T, k), dtype=torch.int32, device="cuda"),
+             ws=torch.empty(lin.workspace_bytes(T), dtype=torch.uint8, device="cuda"))
+
+    def step():
+        norm.run(s["h"], d_y=s["y"], d_h_out=s["h2"], d_x=s["x"])
+        route.run(s["l"], s["ids"], s["w"], d_bias=bias)
+        lin.run(s["x"], s["o"], d_ws=s["ws"])
+
+    def outputs():
+        torch.cuda.synchronize()
+        return [s[n].clone() for n in ("h2", "x", "ids", "w", "o")]
+
+    step()
+    first = outputs()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for n in ("h2", "x", "o", "w"):
+        s[n].zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    for a, b in zip(first, outputs()):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in (1, 2):
+        g2 = torch.Generator(device="cuda").manual_seed(seed)
+        for n in ("h", "y", "l"):
+            s[n].copy_(torch.randn(s[n].shape, generator=g2, device="cuda"))
+        step()
+        want = outputs()
+        for n in ("h2", "x", "o", "w"):
+            s[n].fill_(-1)
+        graph.replay()
+        for a, b in zip(want, outputs()):
+            assert torch.equal(a, b)
+
+
+def test_moe_layer_with_its_norms_and_shared_expert(cb, orc, cuda):
+    """One layer as a stage runs it: norm, router, routing, routed experts, the 8-bit shared
+    expert, and the gated residual step with the next norm, against 64-bit arithmetic
+    and the oracle's experts."""
+    from oracle_lib import rel_l2
+    torch = cuda
+    T, dim, ff, E, k, seed, policy = 21, 2048, 512, 32, 4, 6, 2
+    gen = torch.Generator(device="cuda").manual_seed(33)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    bank = cb.ExpertBank(n_layers=1, n_experts=E, dim=dim, ff=ff, max_picks=k, device=0)
+    try:
+        bank.fill_synthetic(seed, policy)
+        h, w_pre, w_post, w_next = rnd(T, dim) * 2, 1 + 0.1 * rnd(dim), 1 + 0.1 * rnd(dim), 1 + 0.1 * rnd(dim)
+        gate_w, bias, gate = rnd(E, dim) * 0.03, rnd(E) * 0.1, rnd(T)
+        mats = {}
+        for name, (n, kk) in {"gate": (ff, dim), "up": (ff, dim), "down": (dim, ff)}.items():
+            q, sc = padded_int8(torch, n, kk), torch.empty(n, device="cuda")
+            cb.int8_quantize(rnd(n, kk) * 0.05, q, sc)
+            mats[name] = cb.Int8Linear(q, sc)
+        new = lambda *s: torch.empty(s, device="cuda")  # noqa: E731
+        x, logits, ids, w = new(T, dim), new(T, E), torch.empty((T, k), dtype=torch.int32, device="cuda"), new(T, k)
+        ws8 = torch.empty(max(m.workspace_bytes(T) for m in mats.values()), dtype=torch.uint8, device="cuda")
+        g, u, a, shared, moe, h2, x2 = new(T, ff), new(T, ff), new(T, ff), new(T, dim), new(T, dim), new(T, dim), new(T, dim)
+        pws = torch.empty(bank.prefill_workspace_bytes(T, k), dtype=torch.uint8, device="cuda")
+        s = torch.cuda.current_stream().cuda_stream
+        cb.BlockNorm(dim, post=False).run(h, d_w_pre=w_pre, d_x=x)
+        cb.router_device(x, gate_w, logits)
+        cb.ExpertRoute(E, k, n_groups=4, top_groups=2, scale=2.5).run(logits, ids, w, d_bias=bias)
+        mats["gate"].run(x, g, d_ws=ws8)
+        mats["up"].run(x, u, d_ws=ws8)
+        cb.q8k_activate(g, u, a)
+        mats["down"].run(a, shared, d_ws=ws8)
+        torch.cuda.synchronize()  # the bank runs on its own stream here
+        bank.prefill_layer_device(0, ids, w, x, moe, pws, d_resid=shared, stream=s or None)
+        bank.synchronize()
+        cb.BlockNorm(dim, gate="token", gate_sigmoid=True, block_scale=0.5).run(
+            h, d_y=moe, d_gate=gate, d_w_post=w_post, d_w_pre=w_next, d_h_out=h2, d_x=x2)
+        torch.cuda.synchronize()
+
+        n = lambda t: t.double().cpu().numpy()  # noqa: E731
+        xw = norm64(n(h), None, None, None, n(w_pre), False, "none", False, 1, 1, 1e-6)[1]
+        assert rel_l2(n(x), xw) <= 1e-6
+        check_route(torch, cb.ExpertRoute(E, k), logits, bias, ids, w, "sigmoid", 4, 2, True, True, 2.5)
+
+        def lin64(m, v):
+            q, sc = quant64(v)
+            return (q @ m.d_w.double().cpu().numpy().T) * sc[:, None] * n(m.d_w_scale)[None, :]
+
+        gw, uw = lin64(mats["gate"], n(x)), lin64(mats["up"], n(x))
+        assert rel_l2(n(g), gw) <= 1e-6 and rel_l2(n(u), uw) <= 1e-6
+        sw = lin64(mats["down"], n(a))
+        assert rel_l2(n(a), n(g) / (1 + np.exp(-n(g))) * n(u)) <= 1e-6 and rel_l2(n(shared), sw) <= 1e-6
+        xs, iw, ww = x.cpu().numpy(), ids.cpu().numpy(), w.cpu().numpy()
+        routed = np.stack([orc.layer_synth(policy, seed, 0, iw[t], ww[t], xs[t], dim, ff) for t in range(T)])
+        assert rel_l2(n(moe), routed.astype(np.float64) + n(shared)) <= 1e-3
+        hw, x2w, _, _ = norm64(n(h), n(moe), n(gate), n(w_post), n(w_next), True, "token", True, 1.0, 0.5, 1e-6)
+        assert rel_l2(n(h2), hw) <= 1e-6 and rel_l2(n(x2), x2w) <= 1e-6
+    finally:
+        bank.close()
