@@ -69,6 +69,7 @@
 
 #include "clb_device.cuh"
 #include "clb_kernels.h"
+#include "clb_tc.cuh"
 #include "clb_v2.cuh"
 
 namespace clb {
@@ -103,7 +104,6 @@ constexpr uint32_t kPfACol = 256;                       // A operand: 2 blocks x
 static_assert(kPfMaxN <= kPfAccCols && kPfMaxN <= kPfDxsStride && kPfMaxN % 16 == 0, "tile width");
 static_assert(kPfRCol + kPfAccCols <= kPfACol && kPfACol + 8 * 32 <= kPfTmemCols, "tensor memory budget");
 constexpr uint32_t kPfSpin = 1u << 22;        // drain wait polls
-constexpr uint32_t kPfSuspendNs = 20000;      // try_wait suspend hint
 constexpr uint64_t kPfTimeoutNs = 1000000000; // 1 s: a pipeline wait longer than this is an error
 constexpr int kErrPrefillWait = 3;
 constexpr int kPfColdMax = 2;                 // experts with at most this many picks take the row-dot path
@@ -158,49 +158,13 @@ static_assert(PfSmem::raw % 16 == 0 && PfSmem::dw % 16 == 0 && PfSmem::dxs % 16 
 static_assert(kPfBStage % 1024 == 0 && 2944 * 4 <= 2 * kPfRawBlock, "swizzle atoms; table staging area");
 static_assert(PfSmem::total + 16 <= 227 * 1024, "fits one CTA per SM with the 16 bytes of static prmt tables");
 
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, P1;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-__device__ __forceinline__ uint64_t pf_now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// try_wait with a suspend-time hint: the thread sleeps until the phase completes or the hint
-// elapses instead of spinning (spinning warps would take issue slots from the decoders).
-__device__ __forceinline__ bool mbar_try_sleep(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, %3;\n\t"
-        "selp.b32 %0, 1, 0, P1;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity), "r"(kPfSuspendNs)
-        : "memory");
-    return done != 0;
-}
 // Bounded wait (kPfTimeoutNs); gives up early once another thread has raised the abort flag.
 __device__ __noinline__ bool pf_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err) {
-    const uint64_t t0 = pf_now_ns();
+    const uint64_t t0 = tc_now_ns();
     for (;;) {
         if (mbar_try_sleep(bar, parity)) return true;
         if (*abort_flag) return false;
-        if (pf_now_ns() - t0 > kPfTimeoutNs) break;
+        if (tc_now_ns() - t0 > kPfTimeoutNs) break;
     }
     atomicExch(err, kErrPrefillWait);
     *abort_flag = 1;
@@ -208,9 +172,6 @@ __device__ __noinline__ bool pf_wait_slow(uint32_t bar, uint32_t parity, volatil
 }
 __device__ __forceinline__ bool pf_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err) {
     return mbar_try(bar, parity) || pf_wait_slow(bar, parity, abort_flag, err);
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // D (+)= A . B^T with A in tensor memory and B described by a shared-memory descriptor.
 template <bool ACCUMULATE>
@@ -228,39 +189,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, 
             "r"(a), "l"(bdesc), "r"(idesc)
             : "memory");
 }
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
 // Four biased bytes (value + 128) -> four fp16 (value * scale), exact because |value * scale|
 // <= 1333: (1024 + byte) * scale - 1152 * scale in one fused rounding (1152 * scale is exact
 // in fp16 for every odd scale <= 31).
@@ -1136,21 +1064,11 @@ bool prefill_shape_supported(int dim, int ff) {
 }
 
 namespace {
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // Tensor maps over B rows [P][K] fp16 (list order): box 64 values x 16 (i + 1) rows, 128-byte swizzle.
 cudaError_t encode_bmaps(CUtensorMap* maps, const __half* base, int P, int K) {
-    static EncodeTiledFn encode = nullptr;
-    if (!encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-        if (e != cudaSuccess) return e;
-        if (!fn || q != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
-        encode = reinterpret_cast<EncodeTiledFn>(fn);
-    }
+    EncodeTiledFn encode = nullptr;
+    const cudaError_t e = tc_encoder(&encode);
+    if (e != cudaSuccess) return e;
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)P};
     const cuuint64_t strides[1] = {(cuuint64_t)K * 2};
     const cuuint32_t es[2] = {1, 1};
