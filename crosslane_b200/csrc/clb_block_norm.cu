@@ -38,25 +38,7 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
 template <bool VEC>
 __device__ __forceinline__ void load8(const void* p, int type, int64_t base, int chunk, int dim, float (&v)[8]) {
     if (VEC) {
-        const int64_t i = base + (int64_t)chunk * 8;
-        if (type == CLB_F32) {
-            const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-            const float4 b = *(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (type == CLB_BF16) {
-                    v[2 * j] = __uint_as_float(w[j] << 16);
-                    v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                    v[2 * j] = f.x, v[2 * j + 1] = f.y;
-                }
-            }
-        }
+        load8_aligned(p, type, base + (int64_t)chunk * 8, v);
     } else {
         const int i = chunk / (int)blockDim.x, tid = chunk % (int)blockDim.x;
 #pragma unroll

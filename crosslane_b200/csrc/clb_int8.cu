@@ -20,7 +20,8 @@ namespace {
 constexpr int kInt8MaxK = 131072;  // 127 * 127 * k stays below 2^31
 constexpr int kErrInt8Wait = 3;
 
-__device__ __forceinline__ int quant_one(float x, float scale, float inv) {
+// The exactly rounded quotient; `inv` the fp32 reciprocal of scale.
+__device__ __forceinline__ int quant_exact(float x, float scale, float inv) {
     float q = rintf(x * inv);
     q = fminf(fmaxf(q, -127.0f), 127.0f);
     const float r = fmaf(-q, scale, x), two = r + r;
@@ -29,35 +30,137 @@ __device__ __forceinline__ int quant_one(float x, float scale, float inv) {
     return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
-// One CTA per row.
-__global__ void __launch_bounds__(256) k_int8_quantize(const void* __restrict__ x, int type, int64_t ld_x, int k,
-                                                       int8_t* __restrict__ q, int64_t ld_q, int kpad,
-                                                       float* __restrict__ scale) {
-    __shared__ float part[8];
-    __shared__ int bad_s;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product's CTAs may start loading weights
-    const int64_t row = blockIdx.x;
-    if (threadIdx.x == 0) bad_s = 0;
-    __syncthreads();
-    float m = 0.0f;
-    bool bad = false;
-    for (int i = threadIdx.x; i < k; i += 256) {
-        const float v = fabsf(ops_load(x, type, row * ld_x + i));
-        bad |= !(v < INFINITY);
-        m = fmaxf(m, v);
-    }
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-    if (bad) bad_s = 1;
-    __syncthreads();
-    m = part[0];
-    for (int i = 1; i < 8; ++i) m = fmaxf(m, part[i]);
+// What a row's values are divided by. tiny: the row is lifted by 2^100 first, and its largest
+// quotient may pass 127 (scale is a subnormal number).
+struct RowScale {
+    float scale, inv;
+    bool zero, tiny;
+};
+__device__ __forceinline__ RowScale row_scale(float m, float* stored) {
     const float s = __fdiv_rn(m, 127.0f);
-    const bool zero = bad_s || !(s > 0.0f);
-    const float lift = s < 0x1p-100f ? 0x1p100f : 1.0f, ls = s * lift, inv = zero ? 0.0f : __fdiv_rn(1.0f, ls);
-    for (int i = threadIdx.x; i < kpad; i += 256)
-        q[row * ld_q + i] = zero || i >= k ? 0 : (int8_t)quant_one(ops_load(x, type, row * ld_x + i) * lift, ls, inv);
-    if (threadIdx.x == 0) scale[row] = bad_s ? __int_as_float(0x7fffffff) : s;
+    RowScale r;
+    r.zero = !(m < INFINITY) || !(s > 0.0f);  // m: largest |x|, NaN or infinite if the row holds such a value
+    r.tiny = s < 0x1p-100f;
+    r.scale = r.tiny ? s * 0x1p100f : s;
+    r.inv = r.zero ? 0.0f : __fdiv_rn(1.0f, r.scale);
+    *stored = m < INFINITY ? s : __int_as_float(0x7fffffff);
+    return r;
+}
+// Eight quotients as bytes. x * inv is within 127 * 2^-22.4 = 2.4e-5 of the quotient, so its
+// rounding (by the addition of 1.5 * 2^23, whose low byte is the integer) stands unless it
+// lies that close to a border; only then, and for tiny rows, the exact form decides.
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], const RowScale& r) {
+    if (r.zero) return make_uint2(0u, 0u);
+    uint32_t q[8];
+    float off = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float t = v[j] * r.inv, f = t + 12582912.0f;
+        q[j] = __float_as_uint(f);
+        off = fmaxf(off, fabsf(t - (f - 12582912.0f)));
+    }
+    if (r.tiny || off > 0.49997f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = (uint32_t)quant_exact(r.tiny ? v[j] * 0x1p100f : v[j], r.scale, r.inv);
+    }
+    return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+}
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+__device__ __forceinline__ float warp_max_nan(float m) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+struct QuantArgs {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    int64_t ld_x, ld_q;
+    int type, k, chunks;  // chunks of 8 columns that are written: k / 8 rounded up, plus zeros up to a pitch
+    bool vec;             // 16-byte loads of x are aligned
+};
+
+// Eight values from column 8c on, zeros behind k.
+__device__ __forceinline__ void load_x8(const void* x, int type, int64_t row, int c, int k, bool vec, float (&v)[8]) {
+    if (vec && 8 * c + 8 <= k) {
+        load8_aligned(x, type, row + 8 * c, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 8 * c + j < k ? ops_load(x, type, row + 8 * c + j) : 0.0f;
+    }
+}
+// q is 16-byte aligned with a pitch of a multiple of 16: eight bytes at once, but columns
+// behind `limit` are not touched.
+__device__ __forceinline__ void store_q8(int8_t* q, int c, int limit, uint2 v) {
+    if (8 * c + 8 <= limit) {
+        *reinterpret_cast<uint2*>(q + 8 * c) = v;
+    } else {
+        for (int j = 0; 8 * c + j < limit; ++j) q[8 * c + j] = (int8_t)((j < 4 ? v.x >> (8 * j) : v.y >> (8 * j - 32)) & 0xffu);
+    }
+}
+
+// One CTA per row, CH chunks of 8 values a thread in registers, or (CH = 0) the row read
+// twice. Bound by the row's bytes; the product behind it may start loading its weights.
+template <int CH>
+__global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a, int limit) {
+    __shared__ float part[32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t row = (int64_t)blockIdx.x * a.ld_x;
+    int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
+    const int tid = threadIdx.x, nt = blockDim.x;
+    float v[CH ? CH : 1][8];
+    float m = 0.0f;
+    if (CH) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) load_x8(a.x, a.type, row, tid + i * nt, a.k, a.vec, v[i]);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[i][j]));
+    } else {
+        for (int c = tid; c < a.chunks; c += nt) {
+            load_x8(a.x, a.type, row, c, a.k, a.vec, v[0]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[0][j]));
+        }
+    }
+    m = warp_max_nan(m);
+    if ((tid & 31) == 0) part[tid >> 5] = m;
+    __syncthreads();
+    m = warp_max_nan((tid & 31) < (nt >> 5) ? part[tid & 31] : 0.0f);
+    float stored;
+    const RowScale r = row_scale(m, &stored);
+    if (CH) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (tid + i * nt < a.chunks) store_q8(q, tid + i * nt, limit, quant8(v[i], r));
+    } else {
+        for (int c = tid; c < a.chunks; c += nt) {
+            load_x8(a.x, a.type, row, c, a.k, a.vec, v[0]);
+            store_q8(q, c, limit, quant8(v[0], r));
+        }
+    }
+    if (tid == 0) a.scale[blockIdx.x] = stored;
+}
+
+// `limit`: columns written (k, or a pitch whose rest is zeros).
+cudaError_t launch_int8_quantize(const void* x, int type, int64_t ld_x, int rows, int k, int8_t* q, int64_t ld_q,
+                                 int limit, float* scale, cudaStream_t s) {
+    QuantArgs a{x, q, scale, ld_x, ld_q, type, k, (limit + 7) / 8, false};
+    a.vec = ops_aligned(x, 16) && ld_x * ops_type_bytes(type) % 16 == 0;
+    // few rows: as many threads as the row has chunks, for the latency; many: 4 chunks a thread, so
+    // that several rows of an SM overlap their loads and stores
+    const int ch = a.chunks > 4096 ? 0 : a.chunks > 1024 || (rows > 296 && a.chunks > 128) ? 4 : 1;
+    const int threads = ch ? std::max(32, ((a.chunks + ch - 1) / ch + 31) / 32 * 32) : 1024;
+    void (*kernel)(QuantArgs, int) = ch == 0 ? k_int8_quantize<0> : ch == 1 ? k_int8_quantize<1> : k_int8_quantize<4>;
+    return ops_launch(kernel, (unsigned)rows, threads, 0, s, a, limit);
 }
 
 struct Int8Args {
@@ -73,40 +176,145 @@ __device__ __forceinline__ float int8_value(int acc, float xs, float ws, float b
     return has_bias ? __fadd_rn(v, bias) : v;
 }
 
-// One warp per weight row and up to 8 tokens.
-__global__ void __launch_bounds__(256) k_int8_dot(const Int8Args a) {
-    const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (n >= a.n) return;
-    const int t0 = blockIdx.y * 8, nt = min(8, a.tokens - t0);
-    const int8_t* w = a.w + n * a.ld_w;
-    int acc[8] = {};
-    for (int p = lane; p < a.k >> 4; p += 32) {
-        const int4 wv = reinterpret_cast<const int4*>(w)[p];
-        for (int t = 0; t < nt; ++t) {
-            const int4 v = reinterpret_cast<const int4*>(a.q + (t0 + t) * a.ld_q)[p];
-            acc[t] = __dp4a(wv.x, v.x, __dp4a(wv.y, v.y, __dp4a(wv.z, v.z, __dp4a(wv.w, v.w, acc[t]))));
+// ------------------------------------------------------------------------------
+// Few tokens (TT >= tokens): row dots. Bound by the weights' bytes, so there is one launch
+// and the first weights are in flight before the tokens are quantised: every CTA does that
+// by itself into shared memory (x comes from L2; floating x) or copies q (int8 x). A CTA has
+// `rows` weight rows, cut into `segs` pieces of K that its warps share out; a piece's sums
+// are integers, added in shared memory in any order.
+constexpr int kDotThreads = 512;
+constexpr int kDotAhead = 4;                 // 16-byte weight pieces a lane has in flight
+constexpr int kDotSmem = 160 * 1024;         // largest tokens * pitch that is staged
+constexpr int kDotMaxSums = 8192;            // rows * tokens of a CTA
+
+struct Int8Dot {
+    Int8Args a;
+    const void* x;      // floating x, or null: a.q and a.q_scale are given
+    int64_t ld_x;
+    int x_type, rows, segs, kpad;
+    bool vec;
+};
+
+template <int TT>
+__global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
+    extern __shared__ uint4 dot_smem[];
+    __shared__ float part[TT][kDotThreads / 32], scale_s[TT];
+    const Int8Args& a = d.a;
+    int8_t* qs = reinterpret_cast<int8_t*>(dot_smem);               // [TT][kpad]
+    int* sums = reinterpret_cast<int*>(qs + (size_t)TT * d.kpad);   // [rows][TT]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int r0 = blockIdx.x * d.rows, nr = min(d.rows, a.n - r0);
+    const int pieces = a.k >> 4, per = (pieces + d.segs - 1) / d.segs;
+    // the warp's first piece of weights
+    int item = warp;
+    int4 w[kDotAhead];
+    auto fetch = [&](int it, int at) {
+        const int8_t* row = a.w + (int64_t)(r0 + it / d.segs) * a.ld_w;
+        const int end = min(pieces, (it % d.segs + 1) * per);
+#pragma unroll
+        for (int u = 0; u < kDotAhead; ++u) {
+            const int p = at + lane + 32 * u;
+            w[u] = p < end ? __ldg(reinterpret_cast<const int4*>(row) + p) : make_int4(0, 0, 0, 0);
+        }
+    };
+    if (item < nr * d.segs) fetch(item, item % d.segs * per);
+    for (int i = tid; i < d.rows * TT; i += kDotThreads) sums[i] = 0;
+    const int chunks = d.kpad >> 3;
+    if (d.x) {
+        float m[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) m[t] = 0.0f;
+        for (int c = tid; c < chunks; c += kDotThreads) {
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                if (t >= a.tokens) break;
+                float v[8];
+                load_x8(d.x, d.x_type, t * d.ld_x, c, a.k, d.vec, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m[t] = max_nan(m[t], fabsf(v[j]));
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            m[t] = warp_max_nan(m[t]);
+            if (lane == 0) part[t][warp] = m[t];
+        }
+        __syncthreads();
+        for (int t = 0; t < TT && t < a.tokens; ++t) {
+            float stored;
+            const RowScale r = row_scale(warp_max_nan(part[t][lane & (kDotThreads / 32 - 1)]), &stored);
+            for (int c = tid; c < chunks; c += kDotThreads) {
+                float v[8];
+                load_x8(d.x, d.x_type, t * d.ld_x, c, a.k, d.vec, v);
+                *reinterpret_cast<uint2*>(qs + (size_t)t * d.kpad + 8 * c) = quant8(v, r);
+            }
+            if (tid == 0) scale_s[t] = stored;
+        }
+    } else {
+        for (int t = 0; t < a.tokens; ++t) {
+            for (int p = tid; p < pieces; p += kDotThreads)
+                reinterpret_cast<int4*>(qs + (size_t)t * d.kpad)[p] = reinterpret_cast<const int4*>(a.q + t * a.ld_q)[p];
+            for (int i = 16 * pieces + tid; i < a.k; i += kDotThreads) qs[(size_t)t * d.kpad + i] = a.q[t * a.ld_q + i];
+            if (tid == 0) scale_s[t] = a.q_scale[t];
         }
     }
-    for (int i = (a.k & ~15) + lane; i < a.k; i += 32)
-        for (int t = 0; t < nt; ++t) acc[t] += (int)w[i] * (int)a.q[(t0 + t) * a.ld_q + i];
-    for (int t = 0; t < nt; ++t) {
-        const int s = __reduce_add_sync(0xffffffffu, acc[t]);
-        if (lane == 0)
-            ops_store(a.out, a.out_type, (t0 + t) * a.ld_out + n,
-                      int8_value(s, a.q_scale[t0 + t], a.w_scale[n], a.bias ? a.bias[n] : 0.0f, a.bias != nullptr));
+    __syncthreads();
+    for (; item < nr * d.segs; item += kDotThreads / 32) {
+        const int seg = item % d.segs, end = min(pieces, (seg + 1) * per);
+        int acc[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[t] = 0;
+        for (int at = seg * per; at < end; at += 32 * kDotAhead) {
+            if (at > seg * per || item != warp) fetch(item, at);
+#pragma unroll
+            for (int u = 0; u < kDotAhead; ++u) {
+                const int p = min(at + lane + 32 * u, pieces - 1);  // weights behind the end are zero
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    const int4 v = reinterpret_cast<const int4*>(qs + (size_t)t * d.kpad)[p];
+                    acc[t] = __dp4a(w[u].x, v.x, __dp4a(w[u].y, v.y, __dp4a(w[u].z, v.z, __dp4a(w[u].w, v.w, acc[t]))));
+                }
+            }
+        }
+        const int row = item / d.segs;
+        if (seg == d.segs - 1) {  // the columns behind the last whole piece
+            const int i = 16 * pieces + lane;
+            if (i < a.k) {
+                const int wv = a.w[(int64_t)(r0 + row) * a.ld_w + i];
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+                    if (t < a.tokens) acc[t] += wv * qs[(size_t)t * d.kpad + i];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+            if (lane == 0) {
+                if (d.segs == 1) sums[row * TT + t] = sum;
+                else atomicAdd(&sums[row * TT + t], sum);
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < nr * a.tokens; i += kDotThreads) {
+        const int t = i / nr, r = i % nr, n = r0 + r;
+        ops_store(a.out, a.out_type, t * a.ld_out + n,
+                  int8_value(sums[r * TT + t], scale_s[t], a.w_scale[n], a.bias ? a.bias[n] : 0.0f, a.bias != nullptr));
     }
 }
 
 // ------------------------------------------------------------------------------
 // Tensor-core product: D[128 weight rows][nt tokens] in tensor memory (int32), A = weights
 // and B = quantised tokens by TMA (128-byte rows of K, 128-byte swizzle), four
-// tcgen05.mma kind::i8 of K = 32 per 128-byte block. Warps 0-3 are the epilogue (a lane is a
-// weight row, so a warp's store of one token is contiguous), warp 4 loads, warp 5 issues.
+// tcgen05.mma kind::i8 of K = 32 per 128-byte block. Warps 0-7 are the epilogue (a lane is a
+// weight row, so a warp's store of one token is contiguous; warps 0-3 take the first half of
+// the tile's tokens, 4-7 the second), warp 8 loads, warp 9 issues.
 // SPLIT: the CTAs of a cluster share a tile's K range; their sums are added over
 // distributed shared memory (integers: the order does not matter). Otherwise a CTA walks
 // over tiles, the epilogue of one under the products of the next (two accumulators).
-constexpr int kGmThreads = 192;
-constexpr int kGmMaxStages = 12;
+constexpr int kGmEpiWarps = 8, kGmLoadWarp = 8, kGmMmaWarp = 9;
+constexpr int kGmThreads = 320;
+constexpr int kGmMaxStages = 12, kGmMaxSplit = 8;
 constexpr int kGmABytes = 128 * 128;
 constexpr int kGmSmem = 220 * 1024;           // dynamic shared memory, alignment included
 constexpr uint32_t kGmTmemCols = 512, kGmAccCols = 256;
@@ -119,7 +327,8 @@ struct Int8Gemm {
     void* out;
     int* status;
     int64_t ld_out;
-    int tokens, n, kblocks, nt, stages, mtiles, tiles, split, out_type;
+    int tokens, n, kblocks, nt, stages, mtiles, tiles, split;
+    bool pairs;  // 16-bit outputs: two rows of a token in one aligned 4-byte store
 };
 
 // D (+)= A . B^T, both operands described in shared memory.
@@ -136,6 +345,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+// Waits for the loads; the registers pass through, so that no use of them moves in front.
+__device__ __forceinline__ void tmem_wait16(int (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 // K-major operand, 128-byte swizzle, 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
@@ -157,8 +372,60 @@ __device__ __forceinline__ bool gm_wait(uint32_t bar, uint32_t parity, volatile 
     return mbar_try(bar, parity) || gm_wait_slow(bar, parity, abort_flag, status);
 }
 
-template <bool SPLIT>
+template <int OUT>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    if (OUT == CLB_BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Sixteen tokens from t0 on of one warp's 32 rows (row: this lane's), from accumulators to
+// the output. xs: the tokens' scales in shared memory.
+template <int OUT>
+__device__ __forceinline__ void gm_store16(const Int8Gemm& g, const int (&r)[16], const float* xs, int t0, int row, float ws,
+                                           float bias) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(xs + j);
+        v[j] = int8_value(r[j], x.x, ws, bias, true);
+        v[j + 1] = int8_value(r[j + 1], x.y, ws, bias, true);
+        v[j + 2] = int8_value(r[j + 2], x.z, ws, bias, true);
+        v[j + 3] = int8_value(r[j + 3], x.w, ws, bias, true);
+    }
+    const int n = min(16, g.tokens - t0);
+    if (OUT != CLB_F32 && g.pairs) {
+        // even lanes take the even tokens of rows (row, row + 1), odd lanes the odd tokens of (row - 1, row)
+        const bool odd = row & 1;
+        uint16_t* p = static_cast<uint16_t*>(g.out) + (int64_t)(t0 + odd) * g.ld_out + (row & ~1);
+        const bool ok = row < g.n;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+            const uint32_t w = odd ? pack16<OUT>(other, v[j + 1]) : pack16<OUT>(v[j], other);
+            if (ok && j + odd < n) *reinterpret_cast<uint32_t*>(p) = w;
+            p += 2 * g.ld_out;
+        }
+    } else if (row < g.n) {
+        if (OUT == CLB_F32) {
+            float* p = static_cast<float*>(g.out) + (int64_t)t0 * g.ld_out + row;
+#pragma unroll
+            for (int j = 0; j < 16; ++j, p += g.ld_out)
+                if (j < n) *p = v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < n) ops_store(g.out, OUT, (int64_t)(t0 + j) * g.ld_out + row, v[j]);
+        }
+    }
+}
+
+template <bool SPLIT, int OUT>
 __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_constant__ Int8Gemm g) {
+    __shared__ __align__(16) float xs_s[2][kGmAccCols];
     extern __shared__ uint8_t gm_smem[];
     __shared__ uint64_t bars[2 * kGmMaxStages + 5];
     __shared__ uint32_t tslot;
@@ -182,7 +449,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
 
     if (tid == 0) {
         for (int i = 0; i < g.stages; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1);
-        for (int i = 0; i < 2; ++i) mbar_init(acc_full(i), 1), mbar_init(acc_empty(i), 4);
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full(i), 1), mbar_init(acc_empty(i), kGmEpiWarps);
         mbar_init(drain, 1);
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -198,7 +465,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tslot);
 
-    if (warp == 4) {
+    if (warp == kGmLoadWarp) {
         if (lane == 0) {
             // weights do not depend on the quantising kernel in front: their first loads go out before
             // that kernel has finished, the tokens' after
@@ -233,7 +500,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
                 if (++kb == nkb) kb = 0, tile += step;
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == kGmMmaWarp) {
         if (lane == 0) {
             // D s32, A and B signed 8-bit, N and M of the instruction
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(g.nt >> 3) << 17) | (8u << 24);
@@ -260,33 +527,47 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
         }
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");  // q_scale
-        const uint32_t tlane = tmem + ((uint32_t)(32 * warp) << 16);
+        const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const int half = (g.nt / 16 + 1) / 2 * 16, c0 = warp < 4 ? 0 : half, c1 = warp < 4 ? half : g.nt;
         bool ok = true;
-        for (int i = 0; i < my_tiles && ok; ++i) {
+        for (int i = 0; i < my_tiles; ++i) {  // to the end after a failed wait too: the warps meet at a barrier
             const int acc = i & 1, tile = first + i * step;
-            const int row = (tile % g.mtiles) * 128 + tid, t0 = (tile / g.mtiles) * g.nt;
-            ok = __all_sync(0xffffffffu, gm_wait(acc_full(acc), (uint32_t)(i >> 1) & 1u, abort_flag, g.status));
-            if (!ok) break;
+            const int row = (tile % g.mtiles) * 128 + (tid & 127), t0 = (tile / g.mtiles) * g.nt;
+            float ws = 0.0f, bias = -0.0f;  // adding -0 leaves every number as it is
+            if (!SPLIT) {
+                if (tid < g.nt) xs_s[acc][tid] = t0 + tid < g.tokens ? g.q_scale[t0 + tid] : 0.0f;
+                if (row < g.n) {
+                    ws = g.w_scale[row];
+                    if (g.bias) bias = g.bias[row];
+                }
+                // the scales of a tile are written once all warps have left the tile two before it
+                asm volatile("bar.sync 1, %0;" ::"r"(32 * kGmEpiWarps) : "memory");
+            }
+            if (ok) ok = __all_sync(0xffffffffu, gm_wait(acc_full(acc), (uint32_t)(i >> 1) & 1u, abort_flag, g.status));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float ws = row < g.n ? g.w_scale[row] : 0.0f;
-            const float bias = g.bias && row < g.n ? g.bias[row] : 0.0f;
-            for (int c = 0; c < g.nt; c += 16) {
-                int r[16];
-                tmem_ld16(tlane + (uint32_t)acc * kGmAccCols + (uint32_t)c, r);
-                const int mine = t0 + c + (lane & 15);
-                const float xs = !SPLIT && mine < g.tokens ? g.q_scale[mine] : 0.0f;
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (SPLIT) {  // the sums of this K range, [token][row]; every product has completed, so the
+            if (ok) {
+                const uint32_t ta = tlane + (uint32_t)acc * kGmAccCols;
+                auto take = [&](const int (&r)[16], int c) {
+                    if (SPLIT) {  // the sums of this K range as [token][row]; every product has completed, so the
                                   // stages are free
-                        asm volatile("st.shared.s32 [%0], %1;" ::"r"(base + (uint32_t)((c + j) * 128 + tid) * 4u), "r"(r[j]));
-                    } else {
-                        const float x = __shfl_sync(0xffffffffu, xs, j);
-                        if (row < g.n && t0 + c + j < g.tokens)
-                            ops_store(g.out, g.out_type, (t0 + c + j) * g.ld_out + row,
-                                      int8_value(r[j], x, ws, bias, g.bias != nullptr));
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            asm volatile("st.shared.s32 [%0], %1;" ::"r"(base + (uint32_t)((c + j) * 128 + (tid & 127)) * 4u),
+                                         "r"(r[j])
+                                         : "memory");
+                    } else if (t0 + c < g.tokens) {
+                        gm_store16<OUT>(g, r, &xs_s[acc][c], t0 + c, row, ws, bias);
                     }
+                };
+                int ra[16], rb[16] = {};
+                if (c0 < c1) tmem_ld16(ta + (uint32_t)c0, ra);
+                for (int c = c0; c < c1; c += 32) {
+                    tmem_wait16(ra);
+                    if (c + 16 < c1) tmem_ld16(ta + (uint32_t)c + 16u, rb);
+                    take(ra, c);
+                    tmem_wait16(rb);
+                    if (c + 32 < c1) tmem_ld16(ta + (uint32_t)c + 32u, ra);
+                    if (c + 16 < c1) take(rb, c + 16);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -298,23 +579,29 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     if (SPLIT) {
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-        const int row = (first % g.mtiles) * 128 + tid, t0 = (first / g.mtiles) * g.nt;
-        if (tid < 128 && row < g.n) {
-            const float ws = g.w_scale[row], bias = g.bias ? g.bias[row] : 0.0f;
-            for (int c = g.nt * rank / g.split; c < g.nt * (rank + 1) / g.split && t0 + c < g.tokens; ++c) {
-                int sum = 0;
-#pragma unroll 8
-                for (int p = 0; p < g.split; ++p) {
-                    uint32_t addr;
-                    int v;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                                 : "=r"(addr)
-                                 : "r"(base + (uint32_t)(c * 128 + tid) * 4u), "r"(p));
-                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-                    sum += v;
+        // this CTA adds up its share of the tile's tokens over the cluster: a warp per token and
+        // quarter of the rows, all peers' loads in flight at once
+        const int tile_row = (first % g.mtiles) * 128, t0 = (first / g.mtiles) * g.nt;
+        const int cb = g.nt * rank / g.split, ce = min(g.nt * (rank + 1) / g.split, g.tokens - t0);
+        if (warp < kGmEpiWarps) {
+            for (int it = warp; it < (ce - cb) * 4; it += kGmEpiWarps) {
+                const int c = cb + it / 4, rr = (it & 3) * 32 + lane, row = tile_row + rr;
+                int v[kGmMaxSplit];
+#pragma unroll
+                for (int p = 0; p < kGmMaxSplit; ++p) {
+                    v[p] = 0;
+                    if (p < g.split) {
+                        uint32_t addr;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(base + (uint32_t)(c * 128 + rr) * 4u), "r"(p));
+                        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[p]) : "r"(addr));
+                    }
                 }
-                ops_store(g.out, g.out_type, (t0 + c) * g.ld_out + row,
-                          int8_value(sum, g.q_scale[t0 + c], ws, bias, g.bias != nullptr));
+                int sum = 0;
+#pragma unroll
+                for (int p = 0; p < kGmMaxSplit; ++p) sum += v[p];
+                if (row < g.n)
+                    ops_store(g.out, OUT, (int64_t)(t0 + c) * g.ld_out + row,
+                              int8_value(sum, g.q_scale[t0 + c], g.w_scale[row], g.bias ? g.bias[row] : 0.0f, g.bias != nullptr));
             }
         }
         asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -324,7 +611,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
         const uint64_t t0 = tc_now_ns();
         while (tc_now_ns() - t0 < 200000u) {
         }
-        if (warp == 5 && lane == 0) {
+        if (warp == kGmMmaWarp && lane == 0) {
             umma_commit(drain);
             for (uint32_t i = 0; i < kGmDrainPolls && !mbar_try(drain, 0); ++i) {
             }
@@ -351,7 +638,7 @@ GmPlan gm_plan(int tokens, int n, int kblocks, int sms) {
     for (int nt = 16; nt <= 256; nt += 16) {
         if (nt > 16 && nt - 16 >= tokens) break;
         const int64_t tiles = mt * ((tokens + nt - 1) / nt);
-        for (int split = 1; split <= 8 && split <= kblocks; split *= 2) {
+        for (int split = 1; split <= kGmMaxSplit && split <= kblocks; split *= 2) {
             if (split > 1 && (nt > 128 || tiles * split > sms)) break;
             const int64_t waves = (tiles * split + sms - 1) / sms;
             const double block = std::max(2.0 * nt, (128.0 + nt) * 128.0 / kGmLoadRate);
@@ -388,11 +675,18 @@ cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, cudaS
     if ((e = gm_encode(&g.wmap, a.w, a.n, a.k, a.ld_w, 128)) != cudaSuccess) return e;
     if ((e = gm_encode(&g.xmap, a.q, a.tokens, a.k, a.ld_q, g.nt)) != cudaSuccess) return e;
     g.w_scale = a.w_scale, g.q_scale = a.q_scale, g.bias = a.bias, g.out = a.out, g.status = status;
-    g.ld_out = a.ld_out, g.tokens = a.tokens, g.n = a.n, g.out_type = a.out_type;
+    g.ld_out = a.ld_out, g.tokens = a.tokens, g.n = a.n;
+    g.pairs = a.n % 2 == 0 && a.ld_out % 2 == 0 && ops_aligned(a.out, 4);
     g.stages = std::min(kGmMaxStages, (kGmSmem - 1024) / (kGmABytes + g.nt * 128));
     g.mtiles = (a.n + 127) / 128;
     g.tiles = g.mtiles * ((a.tokens + g.nt - 1) / g.nt);
-    void (*kernel)(Int8Gemm) = g.split > 1 ? k_int8_gemm<true> : k_int8_gemm<false>;
+    void (*kernel)(Int8Gemm) =
+        g.split > 1 ? (a.out_type == CLB_F32    ? k_int8_gemm<true, CLB_F32>
+                       : a.out_type == CLB_BF16 ? k_int8_gemm<true, CLB_BF16>
+                                                : k_int8_gemm<true, CLB_F16>)
+                    : (a.out_type == CLB_F32    ? k_int8_gemm<false, CLB_F32>
+                       : a.out_type == CLB_BF16 ? k_int8_gemm<false, CLB_BF16>
+                                                : k_int8_gemm<false, CLB_F16>);
     if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem)) != cudaSuccess) return e;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t c{};
@@ -415,8 +709,35 @@ cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, cudaS
     return cudaLaunchKernelEx(&c, kernel, g);
 }
 
-// Up to this many tokens the product is row dots, above it tensor-core tiles.
-constexpr int kDotTokens = 8;
+// Up to this many tokens the product is row dots, above it (or when the quantised tokens do
+// not fit in shared memory) tensor-core tiles.
+constexpr int kDotTokens = 4;
+
+cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_t ld_x, cudaStream_t s) {
+    int dev = 0, sms = 0;
+    cudaError_t e;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    Int8Dot d{a, x, ld_x, x_type, 0, 1, (a.k + 15) & ~15, false};
+    d.vec = x && ops_aligned(x, 16) && ld_x * ops_type_bytes(x_type) % 16 == 0;
+    const int tt = a.tokens <= 1 ? 1 : a.tokens <= 2 ? 2 : 4;
+    d.rows = std::min((a.n + sms - 1) / sms, kDotMaxSums / tt);
+    // cut the rows so that the warps' shares are even: a round is kDotThreads / 32 items
+    constexpr int warps = kDotThreads / 32;
+    double least = 1e300;
+    for (int segs = 1; segs <= 16 && a.k / segs >= 512; segs *= 2) {
+        const double cost = (double)((d.rows * segs + warps - 1) / warps) / segs + 0.02 * segs;
+        if (cost < least) least = cost, d.segs = segs;
+    }
+    void (*kernel)(Int8Dot) = tt == 1 ? k_int8_dot<1> : tt == 2 ? k_int8_dot<2> : k_int8_dot<4>;
+    const size_t smem = (size_t)tt * d.kpad + (size_t)d.rows * tt * 4;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)) != cudaSuccess) return e;
+    return ops_launch(kernel, (unsigned)((a.n + d.rows - 1) / d.rows), kDotThreads, smem, s, d);
+}
+bool dot_fits(int tokens, int k) {
+    const int tt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : 4;
+    return tokens <= kDotTokens && (int64_t)tt * ((k + 15) & ~15) <= kDotSmem;
+}
 
 int64_t round16(int64_t v) { return (v + 15) & ~(int64_t)15; }
 
@@ -436,8 +757,8 @@ extern "C" int32_t clb_int8_quantize_device(int32_t type, const void* d_x, int64
         require(clb::ops_aligned(d_x, clb::ops_type_bytes(type)) && clb::ops_aligned(d_q, 16) &&
                     clb::ops_aligned(d_scale, 4),
                 CLB_E_INVALID, "misaligned pointer argument (q is 16-byte aligned)");
-        cuda_check(clb::ops_launch(clb::k_int8_quantize, (unsigned)rows, 256, 0, static_cast<cudaStream_t>(stream), d_x,
-                                   type, ld_x, k, d_q, ld_q, k, d_scale),
+        cuda_check(clb::launch_int8_quantize(d_x, type, ld_x, rows, k, d_q, ld_q, k, d_scale,
+                                             static_cast<cudaStream_t>(stream)),
                    "int8 quantise");
     });
 }
@@ -481,21 +802,20 @@ extern "C" int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, 
             a.q = static_cast<const int8_t*>(d_x);
             a.q_scale = d_x_scale;
             a.ld_q = c.ld_x;
-        } else {
+        }
+        if (clb::dot_fits(tokens, c.k)) {
+            cuda_check(clb::launch_int8_dot(a, ready ? nullptr : d_x, c.x_type, c.ld_x, s), "int8 row dots");
+            return;
+        }
+        if (!ready) {
             a.ld_q = clb::round16(c.k);
             float* scale = reinterpret_cast<float*>(static_cast<int8_t*>(d_ws) + tokens * a.ld_q);
             a.q = static_cast<const int8_t*>(d_ws);
             a.q_scale = scale;
-            cuda_check(clb::ops_launch(clb::k_int8_quantize, (unsigned)tokens, 256, 0, s, d_x, c.x_type, c.ld_x, c.k,
-                                       static_cast<int8_t*>(d_ws), a.ld_q, (int)a.ld_q, scale),
+            cuda_check(clb::launch_int8_quantize(d_x, c.x_type, c.ld_x, tokens, c.k, static_cast<int8_t*>(d_ws), a.ld_q,
+                                                 (int)a.ld_q, scale, s),
                        "int8 quantise");
         }
-        if (tokens > clb::kDotTokens) {
-            cuda_check(clb::launch_int8_gemm(a, d_status, !ready, s), "int8 product");
-            return;
-        }
-        cuda_check(clb::ops_launch(clb::k_int8_dot, dim3((unsigned)((c.n + 7) / 8), (unsigned)((tokens + 7) / 8)), 256,
-                                   0, s, a),
-                   "int8 product");
+        cuda_check(clb::launch_int8_gemm(a, d_status, !ready, s), "int8 product");
     });
 }

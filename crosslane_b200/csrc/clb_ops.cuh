@@ -26,6 +26,28 @@ __device__ __forceinline__ void ops_store(void* p, int type, int64_t i, float v)
     else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// Eight elements from i on, 16-byte aligned (coherent loads: the tensor may be updated in place).
+__device__ __forceinline__ void load8_aligned(const void* p, int type, int64_t i, float (&v)[8]) {
+    if (type == CLB_F32) {
+        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        return;
+    }
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (type == CLB_BF16) {
+            v[2 * j] = __uint_as_float(w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+    }
+}
+
 __device__ __forceinline__ float ops_warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
