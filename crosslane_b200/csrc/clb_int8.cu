@@ -9,7 +9,9 @@
 // scale settles the neighbour. Rows whose scale is below 2^-100 are first lifted by 2^100
 // (exact, the quotients stay), so that 1 / scale and the remainders are normal numbers.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <mutex>
 
 #include "clb_ops.cuh"
 #include "clb_tc.cuh"
@@ -186,6 +188,7 @@ constexpr int kDotThreads = 512;
 constexpr int kDotAhead = 4;                 // 16-byte weight pieces a lane has in flight
 constexpr int kDotSmem = 160 * 1024;         // largest tokens * pitch that is staged
 constexpr int kDotMaxSums = 8192;            // rows * tokens of a CTA
+constexpr int kDotSmemMax = kDotSmem + 4 * kDotMaxSums;
 
 struct Int8Dot {
     Int8Args a;
@@ -304,14 +307,20 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
 }
 
 // ------------------------------------------------------------------------------
-// Tensor-core product: D[128 weight rows][nt tokens] in tensor memory (int32), A = weights
-// and B = quantised tokens by TMA (128-byte rows of K, 128-byte swizzle), four
-// tcgen05.mma kind::i8 of K = 32 per 128-byte block. Warps 0-7 are the epilogue (a lane is a
-// weight row, so a warp's store of one token is contiguous; warps 0-3 take the first half of
-// the tile's tokens, 4-7 the second), warp 8 loads, warp 9 issues.
-// SPLIT: the CTAs of a cluster share a tile's K range; their sums are added over
-// distributed shared memory (integers: the order does not matter). Otherwise a CTA walks
-// over tiles, the epilogue of one under the products of the next (two accumulators).
+// Tensor-core product: D[weight rows][nt tokens] in tensor memory (int32), A = weights and B =
+// quantised tokens by TMA (128-byte rows of K, 128-byte swizzle), four tcgen05.mma kind::i8 of
+// K = 32 per 128-byte block. Warps 0-7 are the epilogue (a lane is a weight row, so a warp's
+// store of one token is contiguous; warps 0-3 take the first half of the tile's tokens, 4-7
+// the second), warp 8 loads, warp 9 issues. Three forms:
+//  * kSingle: a CTA walks over tiles of 128 rows, the epilogue of one under the products of
+//    the next (two accumulators);
+//  * kPair: the same with the two SMs of a cluster on one tile of 256 rows (cta_group::2): each
+//    loads its 128 weight rows and half of the tokens, a third less per SM and product than
+//    kSingle's, which is bound by the loads from L2;
+//  * kSplit: the CTAs of a cluster share one tile's K range, for products with few tiles; each
+//    sends its sums to the CTA that owns the tokens, which adds them up (integers: the order
+//    does not matter).
+enum : int { kSingle = 0, kPair = 1, kSplit = 2 };
 constexpr int kGmEpiWarps = 8, kGmLoadWarp = 8, kGmMmaWarp = 9;
 constexpr int kGmThreads = 320;
 constexpr int kGmMaxStages = 12, kGmMaxSplit = 8;
@@ -322,7 +331,7 @@ constexpr uint64_t kGmTimeoutNs = 1000000000; // a pipeline wait longer than thi
 constexpr uint32_t kGmDrainPolls = 1u << 22;
 
 struct Int8Gemm {
-    CUtensorMap wmap, xmap;  // [n][k] box 128 rows, [tokens][k] box nt rows; 128 bytes wide
+    CUtensorMap wmap, xmap;  // [n][k] box 128 rows, [tokens][k] box: a CTA's token rows; 128 bytes wide
     const float *w_scale, *q_scale, *bias;
     void* out;
     int* status;
@@ -331,14 +340,53 @@ struct Int8Gemm {
     bool pairs;  // 16-bit outputs: two rows of a token in one aligned 4-byte store
 };
 
-// D (+)= A . B^T, both operands described in shared memory.
+// D (+)= A . B^T, both operands described in shared memory (PAIR: of both CTAs).
+template <bool PAIR>
 __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
+// One arrival on `bar` (PAIR: on the barrier at that place in both CTAs) once the products
+// issued so far have completed.
+template <bool PAIR>
+__device__ __forceinline__ void gm_commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        umma_commit(bar);
+}
+// A 2-D tile into this CTA; PAIR: counted on a barrier of the leading CTA.
+template <bool PAIR>
+__device__ __forceinline__ void gm_load(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+            "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        tma_2d(dst, map, x, y, bar);
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -357,10 +405,21 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
     return ((uint64_t)1 << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61) |
            (uint64_t)((addr >> 4) & 0x3FFFu);
 }
+// Parity wait whose acquire covers the peer CTA's arrivals.
+__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, P1;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(kTcSuspendNs)
+        : "memory");
+    return done != 0;
+}
 __device__ __noinline__ bool gm_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
     const uint64_t t0 = tc_now_ns();
     for (;;) {
-        if (mbar_try_sleep(bar, parity)) return true;
+        if (mbar_try_cluster(bar, parity)) return true;
         if (*abort_flag) return false;
         if (tc_now_ns() - t0 > kGmTimeoutNs) break;
     }
@@ -369,7 +428,7 @@ __device__ __noinline__ bool gm_wait_slow(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 __device__ __forceinline__ bool gm_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
-    return mbar_try(bar, parity) || gm_wait_slow(bar, parity, abort_flag, status);
+    return mbar_try_cluster(bar, parity) || gm_wait_slow(bar, parity, abort_flag, status);
 }
 
 template <int OUT>
@@ -423,10 +482,11 @@ __device__ __forceinline__ void gm_store16(const Int8Gemm& g, const int (&r)[16]
     }
 }
 
-template <bool SPLIT, int OUT>
+template <int MODE, int OUT>
 __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_constant__ Int8Gemm g) {
-    __shared__ __align__(16) float xs_s[2][kGmAccCols];
+    constexpr bool PAIR = MODE == kPair, SPLIT = MODE == kSplit;
     extern __shared__ uint8_t gm_smem[];
+    __shared__ __align__(16) float xs_s[2][kGmAccCols];
     __shared__ uint64_t bars[2 * kGmMaxStages + 5];
     __shared__ uint32_t tslot;
     __shared__ int abort_s;
@@ -439,71 +499,87 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     const uint32_t drain = bar0 + 8u * (uint32_t)(2 * kGmMaxStages + 4);
     volatile int* abort_flag = &abort_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t stage_bytes = (uint32_t)kGmABytes + (uint32_t)g.nt * 128u;
-    const int rank = SPLIT ? (int)blockIdx.x % g.split : 0;
-    const int first = SPLIT ? (int)blockIdx.x / g.split : (int)blockIdx.x, step = (int)gridDim.x;
+    // this CTA's place in its cluster, the tiles it walks over, and its K blocks
+    const int peers = PAIR ? 2 : SPLIT ? g.split : 1;
+    const int rank = MODE == kSingle ? 0 : (int)blockIdx.x % peers;
+    const int first = (int)blockIdx.x / peers, step = (int)gridDim.x / peers;
     const int my_tiles = SPLIT ? 1 : (g.tiles - 1 - first) / step + 1;
     const int kb0 = SPLIT ? (int)((int64_t)g.kblocks * rank / g.split) : 0;
     const int nkb = (SPLIT ? (int)((int64_t)g.kblocks * (rank + 1) / g.split) : g.kblocks) - kb0;
     const int64_t total = (int64_t)my_tiles * nkb;
+    const int tile_rows = PAIR ? 256 : 128, brows = PAIR ? g.nt / 2 : g.nt;
+    const uint32_t stage_bytes = (uint32_t)kGmABytes + (uint32_t)brows * 128u;
+    auto row_of = [&](int tile) { return (tile % g.mtiles) * tile_rows + (PAIR ? 128 * rank : 0); };
+    auto token_of = [&](int tile) { return (tile / g.mtiles) * g.nt; };
 
-    if (tid == 0) {
+    if (tid == 32 * kGmLoadWarp) {
         for (int i = 0; i < g.stages; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1);
-        for (int i = 0; i < 2; ++i) mbar_init(acc_full(i), 1), mbar_init(acc_empty(i), kGmEpiWarps);
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full(i), 1), mbar_init(acc_empty(i), (PAIR ? 2 : 1) * kGmEpiWarps);
         mbar_init(drain, 1);
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         (uint32_t)__cvta_generic_to_shared(&tslot)),
-                     "r"(kGmTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        const uint32_t slot = (uint32_t)__cvta_generic_to_shared(&tslot);
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(kGmTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(kGmTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        }
     }
+    // the peer's barriers and tensor memory are there
+    if (PAIR) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+    // weights do not depend on the quantising kernel in front: their first loads go out before
+    // that kernel has finished, the tokens' after
+    const int ahead = (int)min((int64_t)g.stages, total);
+    if (tid == 32 * kGmLoadWarp) {
+        int tile = first, kb = 0;
+        for (int i = 0; i < ahead; ++i) {
+            if (rank == 0 || !PAIR) mbar_expect_tx(full(i), (PAIR ? 2u : 1u) * stage_bytes);
+            gm_load<PAIR>(base + (uint32_t)i * stage_bytes, &g.wmap, (kb0 + kb) * 128, row_of(tile),
+                          PAIR ? cluster_addr(full(i), 0) : full(i));
+            if (++kb == nkb) kb = 0, tile += step;
+        }
+    }
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (SPLIT) cluster_arrive();  // waited for before the first access to a peer
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tslot);
+    // SPLIT: [source][token of this CTA's share][128 rows] behind the stages
+    const int share = SPLIT ? (g.nt + g.split - 1) / g.split : 0;
+    const uint32_t red = base + (uint32_t)g.stages * stage_bytes;
 
     if (warp == kGmLoadWarp) {
         if (lane == 0) {
-            // weights do not depend on the quantising kernel in front: their first loads go out before
-            // that kernel has finished, the tokens' after
-            const int ahead = (int)min((int64_t)g.stages, total);
-            int tile = first, kb = 0;
-            auto at = [&](int& m, int& t) {
-                m = (tile % g.mtiles) * 128;
-                t = (tile / g.mtiles) * g.nt;
-            };
-            for (int i = 0; i < ahead; ++i) {
-                int m, t;
-                at(m, t);
-                mbar_expect_tx(full(i), stage_bytes);
-                tma_2d(base + (uint32_t)i * stage_bytes, &g.wmap, (kb0 + kb) * 128, m, full(i));
-                if (++kb == nkb) kb = 0, tile += step;
-            }
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            tile = first, kb = 0;
-            int stage = 0;
+            int tile = first, kb = 0, stage = 0;
             uint32_t phase = 0;
             for (int64_t i = 0; i < total; ++i) {
-                int m, t;
-                at(m, t);
                 const uint32_t a = base + (uint32_t)stage * stage_bytes;
+                const uint32_t bar = PAIR ? cluster_addr(full(stage), 0) : full(stage);
                 if (i >= ahead) {
                     if (!gm_wait(empty(stage), phase ^ 1u, abort_flag, g.status)) break;
-                    mbar_expect_tx(full(stage), stage_bytes);
-                    tma_2d(a, &g.wmap, (kb0 + kb) * 128, m, full(stage));
+                    if (rank == 0 || !PAIR) mbar_expect_tx(full(stage), (PAIR ? 2u : 1u) * stage_bytes);
+                    gm_load<PAIR>(a, &g.wmap, (kb0 + kb) * 128, row_of(tile), bar);
                 }
-                tma_2d(a + kGmABytes, &g.xmap, (kb0 + kb) * 128, t, full(stage));
+                gm_load<PAIR>(a + kGmABytes, &g.xmap, (kb0 + kb) * 128, token_of(tile) + (PAIR ? brows * rank : 0), bar);
                 if (++stage == g.stages) stage = 0, phase ^= 1u;
                 if (++kb == nkb) kb = 0, tile += step;
             }
         }
     } else if (warp == kGmMmaWarp) {
-        if (lane == 0) {
+        if (lane == 0 && (rank == 0 || !PAIR)) {
             // D s32, A and B signed 8-bit, N and M of the instruction
-            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(g.nt >> 3) << 17) | (8u << 24);
+            const uint32_t idesc =
+                (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(g.nt >> 3) << 17) | ((uint32_t)(tile_rows >> 4) << 24);
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -518,21 +594,23 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
                     const uint64_t da = smem_desc(a), db = smem_desc(a + kGmABytes);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        umma_i8(tmem + (uint32_t)acc * kGmAccCols, da + 2u * j, db + 2u * j, idesc, kb > 0 || j > 0);
-                    umma_commit(empty(stage));
+                        umma_i8<PAIR>(tmem + (uint32_t)acc * kGmAccCols, da + 2u * j, db + 2u * j, idesc, kb > 0 || j > 0);
+                    gm_commit<PAIR>(empty(stage));
                     if (++stage == g.stages) stage = 0, phase ^= 1u;
                 }
-                if (ok) umma_commit(acc_full(acc));
+                if (ok) gm_commit<PAIR>(acc_full(acc));
             }
         }
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");  // q_scale
         const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const int half = (g.nt / 16 + 1) / 2 * 16, c0 = warp < 4 ? 0 : half, c1 = warp < 4 ? half : g.nt;
+        const uint32_t lead_empty = PAIR ? cluster_addr(acc_empty(0), 0) : 0u;
         bool ok = true;
+        if (SPLIT) cluster_wait();
         for (int i = 0; i < my_tiles; ++i) {  // to the end after a failed wait too: the warps meet at a barrier
             const int acc = i & 1, tile = first + i * step;
-            const int row = (tile % g.mtiles) * 128 + (tid & 127), t0 = (tile / g.mtiles) * g.nt;
+            const int row = row_of(tile) + (tid & 127), t0 = token_of(tile);
             float ws = 0.0f, bias = -0.0f;  // adding -0 leaves every number as it is
             if (!SPLIT) {
                 if (tid < g.nt) xs_s[acc][tid] = t0 + tid < g.tokens ? g.q_scale[t0 + tid] : 0.0f;
@@ -547,14 +625,21 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ok) {
                 const uint32_t ta = tlane + (uint32_t)acc * kGmAccCols;
+                // SPLIT: where the sums of token c go
+                int owner = SPLIT ? c0 / share : 0, off = SPLIT ? c0 % share : 0;
+                auto send_to = [&] { return cluster_addr(red + (uint32_t)((rank * share + off) * 128 + (tid & 127)) * 4u, owner); };
+                uint32_t to = SPLIT ? send_to() : 0u;
                 auto take = [&](const int (&r)[16], int c) {
-                    if (SPLIT) {  // the sums of this K range as [token][row]; every product has completed, so the
-                                  // stages are free
+                    if (SPLIT) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            asm volatile("st.shared.s32 [%0], %1;" ::"r"(base + (uint32_t)((c + j) * 128 + (tid & 127)) * 4u),
-                                         "r"(r[j])
-                                         : "memory");
+                        for (int j = 0; j < 16; ++j) {
+                            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to), "r"(r[j]) : "memory");
+                            to += 512u;
+                            if (++off == share) {
+                                off = 0;
+                                if (++owner < g.split) to = send_to();
+                            }
+                        }
                     } else if (t0 + c < g.tokens) {
                         gm_store16<OUT>(g, r, &xs_s[acc][c], t0 + c, row, ws, bias);
                     }
@@ -572,80 +657,101 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(acc));
+            if (lane == 0) {
+                if (PAIR)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_empty + 8u * acc)
+                                 : "memory");
+                else
+                    mbar_arrive(acc_empty(acc));
+            }
         }
     }
+    __syncwarp();
 
     if (SPLIT) {
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-        // this CTA adds up its share of the tile's tokens over the cluster: a warp per token and
-        // quarter of the rows, all peers' loads in flight at once
-        const int tile_row = (first % g.mtiles) * 128, t0 = (first / g.mtiles) * g.nt;
-        const int cb = g.nt * rank / g.split, ce = min(g.nt * (rank + 1) / g.split, g.tokens - t0);
-        if (warp < kGmEpiWarps) {
-            for (int it = warp; it < (ce - cb) * 4; it += kGmEpiWarps) {
-                const int c = cb + it / 4, rr = (it & 3) * 32 + lane, row = tile_row + rr;
-                int v[kGmMaxSplit];
+        if (warp >= kGmEpiWarps) cluster_wait();
+        cluster_arrive();
+        cluster_wait();
+        // every peer's sums are here: this CTA's share of the tile's tokens
+        const int t0 = token_of(first) + rank * share, row = row_of(first) + (tid & 127);
+        const int nc = min(share, min(g.nt - rank * share, g.tokens - t0));
+        if (warp < kGmEpiWarps && row < g.n && !*abort_flag) {
+            const float ws = g.w_scale[row], bias = g.bias ? g.bias[row] : -0.0f;
+            for (int c = tid >> 7; c < nc; c += 2) {
+                int v[kGmMaxSplit], sum = 0;
 #pragma unroll
                 for (int p = 0; p < kGmMaxSplit; ++p) {
                     v[p] = 0;
-                    if (p < g.split) {
-                        uint32_t addr;
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(base + (uint32_t)(c * 128 + rr) * 4u), "r"(p));
-                        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[p]) : "r"(addr));
-                    }
+                    if (p < g.split)
+                        asm volatile("ld.shared.s32 %0, [%1];"
+                                     : "=r"(v[p])
+                                     : "r"(red + (uint32_t)((p * share + c) * 128 + (tid & 127)) * 4u));
                 }
-                int sum = 0;
 #pragma unroll
                 for (int p = 0; p < kGmMaxSplit; ++p) sum += v[p];
-                if (row < g.n)
-                    ops_store(g.out, OUT, (int64_t)(t0 + c) * g.ld_out + row,
-                              int8_value(sum, g.q_scale[t0 + c], g.w_scale[row], g.bias ? g.bias[row] : 0.0f, g.bias != nullptr));
+                ops_store(g.out, OUT, (int64_t)(t0 + c) * g.ld_out + row, int8_value(sum, g.q_scale[t0 + c], ws, bias, true));
             }
         }
-        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     }
     __syncthreads();
     if (*abort_flag) {  // let copies in flight land and the issued products complete before leaving
         const uint64_t t0 = tc_now_ns();
         while (tc_now_ns() - t0 < 200000u) {
         }
-        if (warp == kGmMmaWarp && lane == 0) {
-            umma_commit(drain);
+        if (warp == kGmMmaWarp && lane == 0 && (rank == 0 || !PAIR)) {
+            gm_commit<PAIR>(drain);
             for (uint32_t i = 0; i < kGmDrainPolls && !mbar_try(drain, 0); ++i) {
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) {  // the peer's products and copies use this CTA's memory until both are done
+        cluster_arrive();
+        cluster_wait();
+    }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kGmTmemCols));
+    if (warp == 0) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kGmTmemCols));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kGmTmemCols));
+    }
 }
 
-// The tile width and the K split of a product, by an estimate of its SM cycles: a 128-byte
-// block of K costs the larger of its products (2 cycles a token column at 8192 multiply-adds
-// per cycle) and its loads (kGmLoadRate bytes per cycle and SM), a tile a fixed part; the CTAs
-// run in waves over the SMs.
-constexpr double kGmLoadRate = 48.0, kGmTileCycles = 700.0, kGmSplitCycles = 1500.0;
+// The form of a product, by an estimate of its time (us) whose constants fit measurements
+// from 16 x 7168 x 1536 to 4096 x 7168 x 7168 on a B200 to about 10 %: a 128-byte block of K
+// costs its loads and, from about 100 token columns on, its multiply-adds; a tile a fixed
+// part, a launch or a split another. CTAs run in waves over the SMs, clusters in the number that fits at
+// once. Measured at 4096 x 7168 x 7168, 256 tokens a tile: single 198 us, pair 172 us; at
+// 500 x 1536 x 7168: 10.9 and 11.2 us; at 64 x 5120 x 2304, 64 tokens: single 15.4 us, split in
+// two 13.0, in four 9.3, in six 8.6 us, in seven (more clusters than fit at once) 15.0 us.
 struct GmPlan {
-    int nt, split;
+    int mode, nt, split;
 };
-GmPlan gm_plan(int tokens, int n, int kblocks, int sms) {
-    GmPlan best{16, 1};
+constexpr int kGmDevices = 64;
+struct GmDevice {
+    int sms;
+    int clusters[kGmMaxSplit + 1];  // clusters of that many CTAs that run at once
+};
+
+GmPlan gm_plan(int tokens, int n, int kblocks, const GmDevice& d) {
+    GmPlan best{kSingle, 16, 1};
     double least = 1e300;
-    const int64_t mt = (n + 127) / 128;
+    auto consider = [&](int mode, int nt, int split) {
+        const int64_t tiles = (int64_t)((n + (mode == kPair ? 255 : 127)) / (mode == kPair ? 256 : 128)) * ((tokens + nt - 1) / nt);
+        const int64_t at_once = mode == kSingle ? d.sms : d.clusters[mode == kPair ? 2 : split];
+        if (at_once < 1) return;
+        const int64_t waves = (tiles + at_once - 1) / at_once;
+        if (mode == kSplit && waves > 1) return;
+        const double block = mode == kPair ? std::max(0.30, 0.241 + 0.00077 * nt) : std::max(0.29, 0.15 + 0.00139 * nt);
+        const double blocks = (kblocks + split - 1) / split * block;
+        const double cost = mode == kSplit ? blocks + 5.2 + 0.02 * nt : waves * (blocks + 0.8) + 4.2;
+        if (cost < least) least = cost, best = GmPlan{mode, nt, split};
+    };
     for (int nt = 16; nt <= 256; nt += 16) {
-        if (nt > 16 && nt - 16 >= tokens) break;
-        const int64_t tiles = mt * ((tokens + nt - 1) / nt);
-        for (int split = 1; split <= kGmMaxSplit && split <= kblocks; split *= 2) {
-            if (split > 1 && (nt > 128 || tiles * split > sms)) break;
-            const int64_t waves = (tiles * split + sms - 1) / sms;
-            const double block = std::max(2.0 * nt, (128.0 + nt) * 128.0 / kGmLoadRate);
-            const double per = ((kblocks + split - 1) / split) * block + kGmTileCycles + 4.0 * nt;
-            const double cost = waves * per + (split > 1 ? kGmSplitCycles : 0.0);
-            if (cost < least) least = cost, best = GmPlan{nt, split};
-        }
+        consider(kSingle, nt, 1);
+        if (nt % 32 == 0) consider(kPair, nt, 1);
+        for (int split = 2; split <= kGmMaxSplit && split <= kblocks && nt <= 128; ++split) consider(kSplit, nt, split);
+        if (nt >= tokens) break;
     }
     return best;
 }
@@ -663,65 +769,103 @@ cudaError_t gm_encode(CUtensorMap* map, const void* p, int64_t rows, int k, int6
                : cudaErrorInvalidValue;
 }
 
-cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, cudaStream_t s) {
-    int dev = 0, sms = 0;
-    cudaError_t e;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    Int8Gemm g{};
-    g.kblocks = (a.k + 127) / 128;
-    const GmPlan plan = gm_plan(a.tokens, a.n, g.kblocks, sms);
-    g.nt = plan.nt, g.split = plan.split;
-    if ((e = gm_encode(&g.wmap, a.w, a.n, a.k, a.ld_w, 128)) != cudaSuccess) return e;
-    if ((e = gm_encode(&g.xmap, a.q, a.tokens, a.k, a.ld_q, g.nt)) != cudaSuccess) return e;
-    g.w_scale = a.w_scale, g.q_scale = a.q_scale, g.bias = a.bias, g.out = a.out, g.status = status;
-    g.ld_out = a.ld_out, g.tokens = a.tokens, g.n = a.n;
-    g.pairs = a.n % 2 == 0 && a.ld_out % 2 == 0 && ops_aligned(a.out, 4);
-    g.stages = std::min(kGmMaxStages, (kGmSmem - 1024) / (kGmABytes + g.nt * 128));
-    g.mtiles = (a.n + 127) / 128;
-    g.tiles = g.mtiles * ((a.tokens + g.nt - 1) / g.nt);
-    void (*kernel)(Int8Gemm) =
-        g.split > 1 ? (a.out_type == CLB_F32    ? k_int8_gemm<true, CLB_F32>
-                       : a.out_type == CLB_BF16 ? k_int8_gemm<true, CLB_BF16>
-                                                : k_int8_gemm<true, CLB_F16>)
-                    : (a.out_type == CLB_F32    ? k_int8_gemm<false, CLB_F32>
-                       : a.out_type == CLB_BF16 ? k_int8_gemm<false, CLB_BF16>
-                                                : k_int8_gemm<false, CLB_F16>);
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem)) != cudaSuccess) return e;
+template <int MODE>
+void (*gm_kernel(int out_type))(Int8Gemm) {
+    return out_type == CLB_F32 ? k_int8_gemm<MODE, CLB_F32> : out_type == CLB_BF16 ? k_int8_gemm<MODE, CLB_BF16>
+                                                                                    : k_int8_gemm<MODE, CLB_F16>;
+}
+void (*gm_kernel(int mode, int out_type))(Int8Gemm) {
+    return mode == kSingle ? gm_kernel<kSingle>(out_type) : mode == kPair ? gm_kernel<kPair>(out_type)
+                                                                          : gm_kernel<kSplit>(out_type);
+}
+
+cudaError_t gm_launch(const Int8Gemm* g, int mode, int out_type, int clusters, int cluster, bool overlap, cudaStream_t s,
+                      int* at_once) {
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3((unsigned)(g.split > 1 ? g.tiles * g.split : std::min(g.tiles, sms)));
+    c.gridDim = dim3((unsigned)clusters * (unsigned)cluster);
     c.blockDim = dim3(kGmThreads);
     c.dynamicSmemBytes = kGmSmem;
     c.stream = s;
     c.attrs = attr;
-    if (g.split > 1) {
+    if (cluster > 1) {
         attr[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[c.numAttrs].val.clusterDim.x = (unsigned)g.split;
+        attr[c.numAttrs].val.clusterDim.x = (unsigned)cluster;
         attr[c.numAttrs].val.clusterDim.y = attr[c.numAttrs].val.clusterDim.z = 1;
         ++c.numAttrs;
     }
+    if (at_once) return cudaOccupancyMaxActiveClusters(at_once, gm_kernel(mode, out_type), &c);
     if (overlap) {
         attr[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
         ++c.numAttrs;
     }
-    return cudaLaunchKernelEx(&c, kernel, g);
+    return cudaLaunchKernelEx(&c, gm_kernel(mode, out_type), *g);
+}
+
+// The current device: its SMs and the clusters they hold, and the kernels' shared memory allowed.
+// Found once per device (the kernels are told apart by attributes that do not change).
+cudaError_t gm_device(const GmDevice** out) {
+    static GmDevice devices[kGmDevices];
+    static std::atomic<bool> ready[kGmDevices];
+    static std::mutex mutex;
+    int dev = 0;
+    cudaError_t e;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if (dev < 0 || dev >= kGmDevices) return cudaErrorInvalidDevice;
+    *out = &devices[dev];
+    if (ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    std::lock_guard<std::mutex> lock(mutex);
+    if (ready[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    GmDevice& d = devices[dev];
+    if ((e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    for (int mode = kSingle; mode <= kSplit; ++mode)
+        for (int type : {CLB_F32, CLB_BF16, CLB_F16})
+            if ((e = cudaFuncSetAttribute(gm_kernel(mode, type), cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem)) !=
+                cudaSuccess)
+                return e;
+    for (auto kernel : {k_int8_dot<1>, k_int8_dot<2>, k_int8_dot<4>})
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDotSmemMax)) != cudaSuccess)
+            return e;
+    for (int size = 2; size <= kGmMaxSplit; ++size)
+        if ((e = gm_launch(nullptr, size == 2 ? kPair : kSplit, CLB_F32, 1, size, false, nullptr, &d.clusters[size])) !=
+            cudaSuccess)
+            return e;
+    ready[dev].store(true, std::memory_order_release);
+    return cudaSuccess;
+}
+
+cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, const GmDevice& d, cudaStream_t s) {
+    cudaError_t e;
+    Int8Gemm g{};
+    g.kblocks = (a.k + 127) / 128;
+    const GmPlan plan = gm_plan(a.tokens, a.n, g.kblocks, d);
+    const bool pair = plan.mode == kPair;
+    const int brows = pair ? plan.nt / 2 : plan.nt, share = (plan.nt + plan.split - 1) / plan.split;
+    g.nt = plan.nt, g.split = plan.split;
+    if ((e = gm_encode(&g.wmap, a.w, a.n, a.k, a.ld_w, 128)) != cudaSuccess) return e;
+    if ((e = gm_encode(&g.xmap, a.q, a.tokens, a.k, a.ld_q, brows)) != cudaSuccess) return e;
+    g.w_scale = a.w_scale, g.q_scale = a.q_scale, g.bias = a.bias, g.out = a.out, g.status = status;
+    g.ld_out = a.ld_out, g.tokens = a.tokens, g.n = a.n;
+    g.pairs = a.n % 2 == 0 && a.ld_out % 2 == 0 && ops_aligned(a.out, 4);
+    const int joined = plan.mode == kSplit ? plan.split * share * 512 : 0;  // the peers' sums
+    g.stages = std::min(kGmMaxStages, (kGmSmem - 1024 - joined) / (kGmABytes + brows * 128));
+    g.mtiles = (a.n + (pair ? 255 : 127)) / (pair ? 256 : 128);
+    g.tiles = g.mtiles * ((a.tokens + g.nt - 1) / g.nt);
+    const int at_once = pair ? d.clusters[2] : d.sms;
+    return gm_launch(&g, plan.mode, a.out_type, plan.mode == kSplit ? g.tiles : std::min(g.tiles, at_once),
+                     pair ? 2 : plan.split, overlap, s, nullptr);
 }
 
 // Up to this many tokens the product is row dots, above it (or when the quantised tokens do
 // not fit in shared memory) tensor-core tiles.
 constexpr int kDotTokens = 4;
 
-cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_t ld_x, cudaStream_t s) {
-    int dev = 0, sms = 0;
-    cudaError_t e;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_t ld_x, const GmDevice& dev, cudaStream_t s) {
     Int8Dot d{a, x, ld_x, x_type, 0, 1, (a.k + 15) & ~15, false};
     d.vec = x && ops_aligned(x, 16) && ld_x * ops_type_bytes(x_type) % 16 == 0;
     const int tt = a.tokens <= 1 ? 1 : a.tokens <= 2 ? 2 : 4;
-    d.rows = std::min((a.n + sms - 1) / sms, kDotMaxSums / tt);
+    d.rows = std::min((a.n + dev.sms - 1) / dev.sms, kDotMaxSums / tt);
     // cut the rows so that the warps' shares are even: a round is kDotThreads / 32 items
     constexpr int warps = kDotThreads / 32;
     double least = 1e300;
@@ -731,7 +875,6 @@ cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_
     }
     void (*kernel)(Int8Dot) = tt == 1 ? k_int8_dot<1> : tt == 2 ? k_int8_dot<2> : k_int8_dot<4>;
     const size_t smem = (size_t)tt * d.kpad + (size_t)d.rows * tt * 4;
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)) != cudaSuccess) return e;
     return ops_launch(kernel, (unsigned)((a.n + d.rows - 1) / d.rows), kDotThreads, smem, s, d);
 }
 bool dot_fits(int tokens, int k) {
@@ -803,8 +946,10 @@ extern "C" int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, 
             a.q_scale = d_x_scale;
             a.ld_q = c.ld_x;
         }
+        const clb::GmDevice* device = nullptr;
+        cuda_check(clb::gm_device(&device), "int8 product set-up");
         if (clb::dot_fits(tokens, c.k)) {
-            cuda_check(clb::launch_int8_dot(a, ready ? nullptr : d_x, c.x_type, c.ld_x, s), "int8 row dots");
+            cuda_check(clb::launch_int8_dot(a, ready ? nullptr : d_x, c.x_type, c.ld_x, *device, s), "int8 row dots");
             return;
         }
         if (!ready) {
@@ -816,6 +961,6 @@ extern "C" int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, 
                                                  (int)a.ld_q, scale, s),
                        "int8 quantise");
         }
-        cuda_check(clb::launch_int8_gemm(a, d_status, !ready, s), "int8 product");
+        cuda_check(clb::launch_int8_gemm(a, d_status, !ready, *device, s), "int8 product");
     });
 }
