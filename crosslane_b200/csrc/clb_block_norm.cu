@@ -1,18 +1,20 @@
 // The residual step between two blocks: RMSNorm after the block, gate, scaled residual sum,
-// RMSNorm before the next block, in one pass over the rows.
-//
-// One CTA per row holds the row in registers: y and h are read once, h' and x written once,
-// so the kernel is bound by those bytes. The two sums of squares are fp32: per thread in
-// element order, then over the warp and the CTA in a fixed tree.
+// RMSNorm before the next block, in one pass over the rows: y and h are read once, h' and x
+// written once, so the kernels are bound by those bytes. A CTA holds a row in registers. The
+// two sums of squares are fp32: per thread in element order, then over the warp and the CTA
+// in a fixed tree.
 #include <algorithm>
 #include <cmath>
 
 #include "clb_ops.cuh"
+#include "clb_tc.cuh"
 
 namespace clb {
 namespace {
 
 constexpr int kNormMaxDim = 32768;
+constexpr int kNormFewRows = 296;  // two an SM
+constexpr int kRowSmem = 216 * 1024;  // shared memory for rows on an SM
 
 struct NormArgs {
     const void *h, *y, *gate;
@@ -33,115 +35,88 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
     return ops_warp_sum(lane < nw ? part[lane] : 0.0f);
 }
 
-// Eight values of a thread's chunk (coherent loads: h may be updated in place). VEC: 8 contiguous elements, 16-byte loads. Otherwise
+// Eight values of a thread's chunk c. VEC: 8 contiguous elements, 16-byte accesses. Otherwise
 // the elements are blockDim apart, so that a warp's scalar accesses stay contiguous.
 template <bool VEC>
-__device__ __forceinline__ void load8(const void* p, int type, int64_t base, int chunk, int dim, float (&v)[8]) {
-    if (VEC) {
-        load8_aligned(p, type, base + (int64_t)chunk * 8, v);
-    } else {
-        const int i = chunk / (int)blockDim.x, tid = chunk % (int)blockDim.x;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int e = (i * 8 + j) * (int)blockDim.x + tid;
-            v[j] = e < dim ? ops_load(p, type, base + e) : 0.0f;
-        }
-    }
+__device__ __forceinline__ Raw8 load8(const void* p, int type, int64_t row, int c, int dim) {
+    const void* r = static_cast<const char*>(p) + row * (type == CLB_F32 ? 4 : 2);
+    const int nt = blockDim.x, tid = threadIdx.x;
+    return VEC ? raw8_aligned(r, type, 8 * (int64_t)(tid + c * nt), tid + c * nt < dim >> 3)
+               : raw8_strided(r, type, 8 * (int64_t)c * nt + tid, nt, dim);
 }
 template <bool VEC>
-__device__ __forceinline__ void store8(void* p, int type, int64_t base, int chunk, int dim, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void* p, int type, int64_t row, int c, int dim, const float (&v)[8]) {
+    const int nt = blockDim.x, tid = threadIdx.x;
     if (VEC) {
-        const int64_t i = base + (int64_t)chunk * 8;
-        if (type == CLB_F32) {
-            float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-            q[0] = make_float4(v[0], v[1], v[2], v[3]);
-            q[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (type == CLB_BF16) {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&b);
-                } else {
-                    const __half2 b = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&b);
-                }
-            }
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        if (tid + c * nt < dim >> 3) store8_aligned(p, type, row + 8 * (int64_t)(tid + c * nt), v);
     } else {
-        const int i = chunk / (int)blockDim.x, tid = chunk % (int)blockDim.x;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int e = (i * 8 + j) * (int)blockDim.x + tid;
-            if (e < dim) ops_store(p, type, base + e, v[j]);
+            const int e = (c * 8 + j) * nt + tid;
+            if (e < dim) ops_store(p, type, row + e, v[j]);
         }
     }
 }
 
+// sigmoid: expf and a reciprocal within 2 ulp each (a gate below -87.3, whose sigmoid is under
+// 2^-126, is 0).
 __device__ __forceinline__ float gate_value(float g, int sigmoid) {
-    return sigmoid ? 1.0f / (1.0f + expf(-g)) : g;
+    return sigmoid ? __fdividef(1.0f, 1.0f + expf(-g)) : g;
 }
 
-// CH chunks of 8 values per thread.
+// One CTA per row, CH chunks of 8 values per thread: few rows, where the latency of one counts,
+// rows that are not aligned, and rows too wide for k_block_norm_rows.
 template <int CH, bool VEC>
 __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     __shared__ float part[2][32];
     const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, nt = blockDim.x;
-    const int chunks = VEC ? a.dim >> 3 : 0x7fffffff;  // scalar chunks mask element by element
-    float v[CH][8], y[CH][8];
+    const bool wide_gate = a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL;
+    Raw8 yr[CH], hr[CH], gr[CH];
+    float v[CH][8];
+    if (a.y)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) yr[c] = load8<VEC>(a.y, a.y_type, row * a.ld_y, c, a.dim);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) hr[c] = load8<VEC>(a.h, a.h_type, row * a.ld_h, c, a.dim);
+    if (CH == 1 && wide_gate) gr[0] = load8<VEC>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, 0, a.dim);
     if (a.y) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            if (tid + c * nt < chunks) load8<VEC>(a.y, a.y_type, row * a.ld_y, tid + c * nt, a.dim, y[c]);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[c][j] = 0.0f;
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        if (tid + c * nt < chunks) load8<VEC>(a.h, a.h_type, row * a.ld_h, tid + c * nt, a.dim, v[c]);
-        else
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
-    }
-    if (a.y) {
-        float inv = 1.0f;
-        if (a.post) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
-            inv = 1.0f / sqrtf(cta_sum(ss, part[0]) * a.inv_dim + a.post_eps);
-        }
         float gt = 1.0f;
         if (a.gate_kind == CLB_GATE_TOKEN) gt = gate_value(ops_load(a.gate, a.gate_type, row), a.gate_sigmoid);
+        float inv = 1.0f;
+        if (a.post) {
+            float ss = 0.0f, y[8];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                raw8_floats(yr[c], a.y_type, VEC, y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+            }
+            inv = rsqrtf(cta_sum(ss, part[0]) * a.inv_dim + a.post_eps);
+        }
         const float f = a.block_scale * gt * inv;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int ch = tid + c * nt;
-            if (ch < chunks) {
-                if (a.post && a.w_post) {
-                    float w[8];
-                    load8<VEC>(a.w_post, CLB_F32, 0, ch, a.dim, w);
+            float y[8], w[8];
+            raw8_floats(yr[c], a.y_type, VEC, y);
+            if (a.w_post) {
+                raw8_floats(load8<VEC>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, VEC, w);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[c][j] *= w[j];
-                }
-                if (a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL) {
-                    float g[8];
-                    load8<VEC>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, ch, a.dim, g);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) y[c][j] *= gate_value(g[j], a.gate_sigmoid);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[c][j] = fmaf(f, y[c][j], a.residual_scale * v[c][j]);
-                store8<VEC>(a.h_out, a.h_type, row * a.ld_h_out, ch, a.dim, v[c]);
+                for (int j = 0; j < 8; ++j) y[j] *= w[j];
             }
+            if (wide_gate) {
+                if (CH > 1) gr[c] = load8<VEC>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, c, a.dim);
+                raw8_floats(gr[c], a.gate_type, VEC, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] *= gate_value(w[j], a.gate_sigmoid);
+            }
+            raw8_floats(hr[c], a.h_type, VEC, v[c]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[c][j] = fmaf(f, y[j], a.residual_scale * v[c][j]);
+            store8<VEC>(a.h_out, a.h_type, row * a.ld_h_out, c, a.dim, v[c]);
         }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) raw8_floats(hr[c], a.h_type, VEC, v[c]);
     }
     if (a.x) {
         float ss = 0.0f;
@@ -149,24 +124,231 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss = fmaf(v[c][j], v[c][j], ss);
-        const float inv = 1.0f / sqrtf(cta_sum(ss, part[1]) * a.inv_dim + a.pre_eps);
+        const float inv = rsqrtf(cta_sum(ss, part[1]) * a.inv_dim + a.pre_eps);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int ch = tid + c * nt;
-            if (ch < chunks) {
-                float w[8];
-                if (a.w_pre) {
-                    load8<VEC>(a.w_pre, CLB_F32, 0, ch, a.dim, w);
+            float w[8];
+            if (a.w_pre) raw8_floats(load8<VEC>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, VEC, w);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] *= v[c][j] * inv;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = v[c][j] * inv;
-                }
-                store8<VEC>(a.x, a.x_type, row * a.ld_x, ch, a.dim, w);
-            }
+            for (int j = 0; j < 8; ++j) w[j] = a.w_pre ? w[j] * (v[c][j] * inv) : v[c][j] * inv;
+            store8<VEC>(a.x, a.x_type, row * a.ld_x, c, a.dim, w);
         }
     }
+}
+
+// Many rows: CTAs that stay and walk over the rows. Bulk copies bring the next rows of y, h and
+// a full gate into shared memory while one is worked on, so that HBM is busy all the time;
+// what all rows share (w_post times the channels' gate, w_pre) stays in registers. A row's
+// shared memory is asked for again as soon as the CTA has read it. The instructions a thread
+// spends on the two sums are as many as on 20 values, so it takes 4 chunks where the rows have
+// them, and several CTAs an SM hide the sums' latency.
+constexpr int kRowStages = 4;
+constexpr uint32_t kRowPolls = 1u << 20;  // waits for a copy, each with a suspend hint of 20 us
+
+// The element types of a call as constants where they are a usual set (told apart at run time,
+// they cost a bandwidth-bound kernel in 16 bits a third of its rate).
+enum : int { kTypesAny = 0, kTypesF32, kTypesBF16, kTypesF16, kTypesF32BF16, kTypesF32F16 };  // the last two: h fp32
+struct NormTypes {
+    int h, other;
+};
+__host__ __device__ constexpr NormTypes norm_types(int set) {
+    return set == kTypesF32    ? NormTypes{CLB_F32, CLB_F32}
+           : set == kTypesBF16 ? NormTypes{CLB_BF16, CLB_BF16}
+           : set == kTypesF16  ? NormTypes{CLB_F16, CLB_F16}
+           : set == kTypesF32BF16 ? NormTypes{CLB_F32, CLB_BF16}
+                                  : NormTypes{CLB_F32, CLB_F16};
+}
+
+// Eight values, number i of a row in shared memory.
+__device__ __forceinline__ void row8(uint32_t p, int type, int i, float (&v)[8]) {
+    Raw8 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    const uint32_t at = p + (uint32_t)i * (type == CLB_F32 ? 32u : 16u);
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w) : "r"(at));
+    if (type == CLB_F32)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
+                     : "r"(at + 16u));
+    raw8_floats(r, type, true, v);
+}
+
+template <int CH, int THREADS, int CTAS, int SET>
+__global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArgs a, int rows, int stages, uint32_t y_bytes,
+                                                                   uint32_t h_bytes, uint32_t g_bytes) {
+    extern __shared__ __align__(16) uint8_t row_smem[];
+    __shared__ float part[4][32];
+    __shared__ uint64_t bars[kRowStages];
+    const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
+    const int x_type = SET ? norm_types(SET).other : a.x_type, g_type = SET ? norm_types(SET).other : a.gate_type;
+    const int tid = threadIdx.x, nt = blockDim.x, units = a.dim >> 3;
+    const uint32_t stage_bytes = y_bytes + h_bytes + g_bytes;
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(row_smem), bar0 = (uint32_t)__cvta_generic_to_shared(bars);
+    auto at = [](const void* p, int type, int64_t i) { return static_cast<const char*>(p) + i * (type == CLB_F32 ? 4 : 2); };
+    auto fetch = [&](int64_t row, int stage) {
+        const uint32_t dst = base + (uint32_t)stage * stage_bytes, bar = bar0 + 8u * (uint32_t)stage;
+        mbar_expect_tx(bar, stage_bytes);
+        if (y_bytes) bulk_g2s(dst, at(a.y, y_type, row * a.ld_y), y_bytes, bar);
+        bulk_g2s(dst + y_bytes, at(a.h, h_type, row * a.ld_h), h_bytes, bar);
+        if (g_bytes) bulk_g2s(dst + y_bytes + h_bytes, at(a.gate, g_type, row * a.ld_gate), g_bytes, bar);
+    };
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(bar0 + 8u * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int s = 0; s < stages; ++s)
+            if (blockIdx.x + (int64_t)s * gridDim.x < rows) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+    }
+    float wp[CH][8], wq[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) wp[c][j] = 1.0f, wq[c][j] = 1.0f;
+        if (a.w_post) raw8_floats(load8<true>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, true, wp[c]);
+        if (a.w_pre) raw8_floats(load8<true>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, true, wq[c]);
+        if (a.gate_kind == CLB_GATE_CHANNEL) {
+            float g[8];
+            raw8_floats(load8<true>(a.gate, a.gate_type, 0, c, a.dim), a.gate_type, true, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wp[c][j] *= gate_value(g[j], a.gate_sigmoid);
+        }
+    }
+    __syncthreads();
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    for (uint32_t row = blockIdx.x; row < (uint32_t)rows; row += gridDim.x) {
+        float gt = a.block_scale;
+        if (a.gate_kind == CLB_GATE_TOKEN) gt *= gate_value(ops_load(a.gate, a.gate_type, row), a.gate_sigmoid);
+        bool here = mbar_try(bar0 + 8u * stage, phase);
+        for (uint32_t i = 0; !here && i < kRowPolls; ++i) here = mbar_try_sleep(bar0 + 8u * stage, phase);
+        const uint32_t sy = base + (uint32_t)stage * stage_bytes, sh = sy + y_bytes, sg = sh + h_bytes;
+        // a copy that never came (the wait ran out) shows as a row of NaN
+        const float ok = here ? 1.0f : __int_as_float(0x7fffffff);
+        float v[CH][8];
+        if (y_bytes) {
+            float f = gt * ok;
+            if (a.post) {
+                float ss = 0.0f, y[8];
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+                    if (tid + c * nt < units) {
+                        row8(sy, y_type, tid + c * nt, y);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+                    }
+                f *= rsqrtf(cta_sum(ss, part[2 * turn]) * a.inv_dim + a.post_eps);
+            }
+            char* out = const_cast<char*>(at(a.h_out, h_type, row * a.ld_h_out));
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int u = tid + c * nt;
+                if (u < units) {
+                    float y[8], g[8];
+                    row8(sy, y_type, u, y);
+                    row8(sh, h_type, u, v[c]);
+                    if (g_bytes) {
+                        row8(sg, g_type, u, g);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) y[j] *= gate_value(g[j], a.gate_sigmoid);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[c][j] = fmaf(f, y[j] * wp[c][j], a.residual_scale * v[c][j]);
+                    store8_aligned(out, h_type, 8 * u, v[c]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                if (tid + c * nt < units) row8(sh, h_type, tid + c * nt, v[c]);
+        }
+        float inv = ok;
+        if (a.x) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                if (tid + c * nt < units)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) ss = fmaf(v[c][j], v[c][j], ss);
+            inv *= rsqrtf(cta_sum(ss, part[2 * turn + 1]) * a.inv_dim + a.pre_eps);
+        } else {
+            __syncthreads();
+        }
+        // the CTA has read the stage
+        if (tid == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, stage);
+        if (a.x) {
+            char* out = const_cast<char*>(at(a.x, x_type, row * a.ld_x));
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int u = tid + c * nt;
+                if (u < units) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = wq[c][j] * (v[c][j] * inv);
+                    store8_aligned(out, x_type, 8 * u, w);
+                }
+            }
+        }
+        turn ^= 1;  // a row may have one sum and so one barrier only: rows take turns with the buffers
+        if (++stage == stages) stage = 0, phase ^= 1u;
+    }
+}
+
+template <int SET>
+void (*rows_kernel(int ch, int threads))(NormArgs, int, int, uint32_t, uint32_t, uint32_t) {
+    return ch == 1          ? k_block_norm_rows<1, 32, 16, SET>
+           : ch == 2        ? (threads <= 32 ? k_block_norm_rows<2, 32, 16, SET> : k_block_norm_rows<2, 512, 1, SET>)
+           : threads <= 256 ? k_block_norm_rows<4, 256, 2, SET>
+                            : k_block_norm_rows<4, 512, 1, SET>;
+}
+
+decltype(rows_kernel<kTypesAny>(0, 0)) rows_kernel(int set, int ch, int threads) {
+    return set == kTypesF32       ? rows_kernel<kTypesF32>(ch, threads)
+           : set == kTypesBF16    ? rows_kernel<kTypesBF16>(ch, threads)
+           : set == kTypesF16     ? rows_kernel<kTypesF16>(ch, threads)
+           : set == kTypesF32BF16 ? rows_kernel<kTypesF32BF16>(ch, threads)
+           : set == kTypesF32F16  ? rows_kernel<kTypesF32F16>(ch, threads)
+                                  : rows_kernel<kTypesAny>(ch, threads);
+}
+
+cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStream_t s) {
+    const int units = (a.dim + 7) / 8;
+    const uint32_t y_bytes = a.y ? a.dim * ops_type_bytes(a.y_type) : 0, h_bytes = a.dim * ops_type_bytes(a.h_type);
+    const uint32_t g_bytes = a.gate_kind == CLB_GATE_FULL ? a.dim * ops_type_bytes(a.gate_type) : 0;
+    const uint32_t stage = y_bytes + h_bytes + g_bytes;
+    if (vec && tokens > kNormFewRows && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
+        int ch = units <= 32 ? 1 : units <= 64 ? 2 : 4;
+        auto threads_of = [&](int chunks) { return std::max(32, ((units + chunks - 1) / chunks + 31) / 32 * 32); };
+        // CTAs on an SM: by the registers (128 a thread), with two rows of shared memory each or more
+        int ctas = std::min(16, 512 / threads_of(ch));
+        while (ctas > 1 && kRowSmem / ctas / (int)stage < 2) --ctas;
+        if (ctas == 1 && units > 512 && units <= 1024) ch = 2;  // one CTA: more warps
+        const int threads = threads_of(ch), stages = std::min(kRowStages, kRowSmem / ctas / (int)stage);
+        int set = kTypesAny;
+        for (int i = kTypesF32; i <= kTypesF32F16; ++i) {
+            const NormTypes t = norm_types(i);
+            if (a.h_type == t.h && (!a.y || a.y_type == t.other) && (!a.x || a.x_type == t.other) &&
+                (!g_bytes || a.gate_type == t.other))
+                set = i;
+        }
+        int sms = 0;
+        const cudaError_t e = ops_device(&sms, [] {
+            cudaError_t e = cudaSuccess;
+            for (int set = kTypesAny; set <= kTypesF32F16; ++set)
+                for (int ch : {1, 2, 4})
+                    for (int threads : {32, 512})
+                        if (e == cudaSuccess)
+                            e = cudaFuncSetAttribute(rows_kernel(set, ch, threads),
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
+            return e;
+        });
+        if (e != cudaSuccess) return e;
+        return ops_launch(rows_kernel(set, ch, threads), (unsigned)std::min<int64_t>(tokens, (int64_t)sms * ctas), threads,
+                          (size_t)stages * stage, s, a, tokens, stages, y_bytes, h_bytes, g_bytes);
+    }
+    const int ch = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
+    const int threads = std::max(32, ((units + ch - 1) / ch + 31) / 32 * 32);
+    void (*kernel)(NormArgs) = vec ? (ch == 1 ? k_block_norm<1, true> : ch == 2 ? k_block_norm<2, true> : k_block_norm<4, true>)
+                                   : (ch == 1   ? k_block_norm<1, false>
+                                      : ch == 2 ? k_block_norm<2, false>
+                                                : k_block_norm<4, false>);
+    return ops_launch(kernel, (unsigned)tokens, threads, 0, s, a);
 }
 
 }  // namespace
@@ -214,13 +396,13 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
             const size_t b = clb::ops_type_bytes(t.type);
             require(t.ld >= c.dim && t.ld <= (int64_t)1 << 40, CLB_E_INVALID, "row pitch of %s below dim", t.name);
             require(clb::ops_aligned(t.p, b), CLB_E_INVALID, "%s is misaligned", t.name);
-            vec = vec && clb::ops_aligned(t.p, 16) && t.ld * b % 16 == 0;
+            vec = vec && clb::ops_vec8(t.p, t.type, t.ld);
         }
         for (const Tensor& t : vecs) {
             if (!t.p) continue;
             require(clb::ops_aligned(t.p, clb::ops_type_bytes(t.type)), CLB_E_INVALID, "%s is misaligned", t.name);
             // a gate for each token is read one number at a time
-            if (t.p != d_gate || c.gate == CLB_GATE_CHANNEL) vec = vec && clb::ops_aligned(t.p, 16);
+            if (t.p != d_gate || c.gate == CLB_GATE_CHANNEL) vec = vec && clb::ops_vec8(t.p, t.type, 0);
         }
         // an output over an input: only h_out in h's place, row by row
         const Tensor outs[] = {rows[3], rows[4]};
@@ -253,16 +435,7 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
         a.gate_kind = d_gate ? c.gate : CLB_GATE_NONE, a.gate_sigmoid = c.gate_sigmoid, a.post = c.post;
         a.post_eps = c.post_eps, a.pre_eps = c.pre_eps, a.residual_scale = c.residual_scale;
         a.block_scale = c.block_scale, a.inv_dim = 1.0f / (float)c.dim;
-        const int units = (c.dim + 7) / 8;
-        const int ch = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
-        const int threads = std::max(32, ((units + ch - 1) / ch + 31) / 32 * 32);
-        void (*kernel)(clb::NormArgs) = vec ? (ch == 1   ? clb::k_block_norm<1, true>
-                                               : ch == 2 ? clb::k_block_norm<2, true>
-                                                         : clb::k_block_norm<4, true>)
-                                            : (ch == 1   ? clb::k_block_norm<1, false>
-                                               : ch == 2 ? clb::k_block_norm<2, false>
-                                                         : clb::k_block_norm<4, false>);
-        cuda_check(clb::ops_launch(kernel, (unsigned)tokens, threads, 0, static_cast<cudaStream_t>(stream), a),
+        cuda_check(clb::launch_block_norm(a, tokens, vec, static_cast<cudaStream_t>(stream)),
                    "block norm");
     });
 }

@@ -9,9 +9,7 @@
 // scale settles the neighbour. Rows whose scale is below 2^-100 are first lifted by 2^100
 // (exact, the quotients stay), so that 1 / scale and the remainders are normal numbers.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
-#include <mutex>
 
 #include "clb_ops.cuh"
 #include "clb_tc.cuh"
@@ -86,17 +84,23 @@ struct QuantArgs {
     float* scale;
     int64_t ld_x, ld_q;
     int type, k, chunks;  // chunks of 8 columns that are written: k / 8 rounded up, plus zeros up to a pitch
-    bool vec;             // 16-byte loads of x are aligned
 };
 
 // Eight values from column 8c on, zeros behind k.
-__device__ __forceinline__ void load_x8(const void* x, int type, int64_t row, int c, int k, bool vec, float (&v)[8]) {
-    if (vec && 8 * c + 8 <= k) {
-        load8_aligned(x, type, row + 8 * c, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 8 * c + j < k ? ops_load(x, type, row + 8 * c + j) : 0.0f;
+template <bool VEC>
+__device__ __forceinline__ Raw8 raw_x8(const void* row, int type, int c, int k) {
+    if (!VEC) return raw8_strided(row, type, 8 * (int64_t)c, 1, k);
+    Raw8 r = raw8_aligned(row, type, 8 * (int64_t)c, 8 * c + 8 <= k);
+    if (8 * c < k && 8 * c + 8 > k) {  // the row's last chunk, into the aligned form
+        r = raw8_strided(row, type, 8 * (int64_t)c, 1, k);
+        if (type != CLB_F32)
+            r = Raw8{make_uint4(r.a.x | r.a.y << 16, r.a.z | r.a.w << 16, r.b.x | r.b.y << 16, r.b.z | r.b.w << 16),
+                     make_uint4(0, 0, 0, 0)};
     }
+    return r;
+}
+__device__ __forceinline__ const void* row_at(const void* x, int type, int64_t element) {
+    return static_cast<const char*>(x) + element * (type == CLB_F32 ? 4 : 2);
 }
 // q is 16-byte aligned with a pitch of a multiple of 16: eight bytes at once, but columns
 // behind `limit` are not touched.
@@ -110,28 +114,27 @@ __device__ __forceinline__ void store_q8(int8_t* q, int c, int limit, uint2 v) {
 
 // One CTA per row, CH chunks of 8 values a thread in registers, or (CH = 0) the row read
 // twice. Bound by the row's bytes; the product behind it may start loading its weights.
-template <int CH>
+template <int CH, bool VEC>
 __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a, int limit) {
     __shared__ float part[32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t row = (int64_t)blockIdx.x * a.ld_x;
+    const void* row = row_at(a.x, a.type, (int64_t)blockIdx.x * a.ld_x);
     int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
     const int tid = threadIdx.x, nt = blockDim.x;
-    float v[CH ? CH : 1][8];
-    float m = 0.0f;
+    Raw8 raw[CH ? CH : 1];
+    float v[8], m = 0.0f;
+    auto largest = [&](const Raw8& r) {
+        raw8_floats(r, a.type, VEC, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+    };
     if (CH) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) load_x8(a.x, a.type, row, tid + i * nt, a.k, a.vec, v[i]);
+        for (int i = 0; i < CH; ++i) raw[i] = raw_x8<VEC>(row, a.type, tid + i * nt, a.k);
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[i][j]));
+        for (int i = 0; i < CH; ++i) largest(raw[i]);
     } else {
-        for (int c = tid; c < a.chunks; c += nt) {
-            load_x8(a.x, a.type, row, c, a.k, a.vec, v[0]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[0][j]));
-        }
+        for (int c = tid; c < a.chunks; c += nt) largest(raw_x8<VEC>(row, a.type, c, a.k));
     }
     m = warp_max_nan(m);
     if ((tid & 31) == 0) part[tid >> 5] = m;
@@ -142,11 +145,14 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a, int l
     if (CH) {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (tid + i * nt < a.chunks) store_q8(q, tid + i * nt, limit, quant8(v[i], r));
+            if (tid + i * nt < a.chunks) {
+                raw8_floats(raw[i], a.type, VEC, v);
+                store_q8(q, tid + i * nt, limit, quant8(v, r));
+            }
     } else {
         for (int c = tid; c < a.chunks; c += nt) {
-            load_x8(a.x, a.type, row, c, a.k, a.vec, v[0]);
-            store_q8(q, c, limit, quant8(v[0], r));
+            raw8_floats(raw_x8<VEC>(row, a.type, c, a.k), a.type, VEC, v);
+            store_q8(q, c, limit, quant8(v, r));
         }
     }
     if (tid == 0) a.scale[blockIdx.x] = stored;
@@ -155,13 +161,15 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a, int l
 // `limit`: columns written (k, or a pitch whose rest is zeros).
 cudaError_t launch_int8_quantize(const void* x, int type, int64_t ld_x, int rows, int k, int8_t* q, int64_t ld_q,
                                  int limit, float* scale, cudaStream_t s) {
-    QuantArgs a{x, q, scale, ld_x, ld_q, type, k, (limit + 7) / 8, false};
-    a.vec = ops_aligned(x, 16) && ld_x * ops_type_bytes(type) % 16 == 0;
+    const QuantArgs a{x, q, scale, ld_x, ld_q, type, k, (limit + 7) / 8};
+    const bool vec = ops_vec8(x, type, ld_x);
     // few rows: as many threads as the row has chunks, for the latency; many: 4 chunks a thread, so
     // that several rows of an SM overlap their loads and stores
     const int ch = a.chunks > 4096 ? 0 : a.chunks > 1024 || (rows > 296 && a.chunks > 128) ? 4 : 1;
     const int threads = ch ? std::max(32, ((a.chunks + ch - 1) / ch + 31) / 32 * 32) : 1024;
-    void (*kernel)(QuantArgs, int) = ch == 0 ? k_int8_quantize<0> : ch == 1 ? k_int8_quantize<1> : k_int8_quantize<4>;
+    void (*kernel)(QuantArgs, int) =
+        vec ? (ch == 0 ? k_int8_quantize<0, true> : ch == 1 ? k_int8_quantize<1, true> : k_int8_quantize<4, true>)
+            : (ch == 0 ? k_int8_quantize<0, false> : ch == 1 ? k_int8_quantize<1, false> : k_int8_quantize<4, false>);
     return ops_launch(kernel, (unsigned)rows, threads, 0, s, a, limit);
 }
 
@@ -195,10 +203,9 @@ struct Int8Dot {
     const void* x;      // floating x, or null: a.q and a.q_scale are given
     int64_t ld_x;
     int x_type, rows, segs, kpad;
-    bool vec;
 };
 
-template <int TT>
+template <int TT, bool VEC>
 __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     extern __shared__ uint4 dot_smem[];
     __shared__ float part[TT][kDotThreads / 32], scale_s[TT];
@@ -224,15 +231,17 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     for (int i = tid; i < d.rows * TT; i += kDotThreads) sums[i] = 0;
     const int chunks = d.kpad >> 3;
     if (d.x) {
-        float m[TT];
+        float m[TT], v[8];
 #pragma unroll
         for (int t = 0; t < TT; ++t) m[t] = 0.0f;
         for (int c = tid; c < chunks; c += kDotThreads) {
+            Raw8 raw[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                raw[t] = raw_x8<VEC>(row_at(d.x, d.x_type, min(t, a.tokens - 1) * d.ld_x), d.x_type, c, a.k);
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-                if (t >= a.tokens) break;
-                float v[8];
-                load_x8(d.x, d.x_type, t * d.ld_x, c, a.k, d.vec, v);
+                raw8_floats(raw[t], d.x_type, VEC, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m[t] = max_nan(m[t], fabsf(v[j]));
             }
@@ -247,8 +256,7 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
             float stored;
             const RowScale r = row_scale(warp_max_nan(part[t][lane & (kDotThreads / 32 - 1)]), &stored);
             for (int c = tid; c < chunks; c += kDotThreads) {
-                float v[8];
-                load_x8(d.x, d.x_type, t * d.ld_x, c, a.k, d.vec, v);
+                raw8_floats(raw_x8<VEC>(row_at(d.x, d.x_type, t * d.ld_x), d.x_type, c, a.k), d.x_type, VEC, v);
                 *reinterpret_cast<uint2*>(qs + (size_t)t * d.kpad + 8 * c) = quant8(v, r);
             }
             if (tid == 0) scale_s[t] = stored;
@@ -727,7 +735,6 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
 struct GmPlan {
     int mode, nt, split;
 };
-constexpr int kGmDevices = 64;
 struct GmDevice {
     int sms;
     int clusters[kGmMaxSplit + 1];  // clusters of that many CTAs that run at once
@@ -803,36 +810,34 @@ cudaError_t gm_launch(const Int8Gemm* g, int mode, int out_type, int clusters, i
     return cudaLaunchKernelEx(&c, gm_kernel(mode, out_type), *g);
 }
 
-// The current device: its SMs and the clusters they hold, and the kernels' shared memory allowed.
-// Found once per device (the kernels are told apart by attributes that do not change).
+// The current device: its SMs and the clusters they hold (found once, with the kernels' shared
+// memory allowed).
 cudaError_t gm_device(const GmDevice** out) {
-    static GmDevice devices[kGmDevices];
-    static std::atomic<bool> ready[kGmDevices];
-    static std::mutex mutex;
-    int dev = 0;
-    cudaError_t e;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-    if (dev < 0 || dev >= kGmDevices) return cudaErrorInvalidDevice;
-    *out = &devices[dev];
-    if (ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
-    std::lock_guard<std::mutex> lock(mutex);
-    if (ready[dev].load(std::memory_order_relaxed)) return cudaSuccess;
-    GmDevice& d = devices[dev];
-    if ((e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    for (int mode = kSingle; mode <= kSplit; ++mode)
-        for (int type : {CLB_F32, CLB_BF16, CLB_F16})
-            if ((e = cudaFuncSetAttribute(gm_kernel(mode, type), cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem)) !=
+    static GmDevice devices[64];
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    e = ops_device(&sms, [&] {
+        GmDevice& d = devices[dev];
+        cudaError_t e;
+        if ((e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+        for (int mode = kSingle; mode <= kSplit; ++mode)
+            for (int type : {CLB_F32, CLB_BF16, CLB_F16})
+                if ((e = cudaFuncSetAttribute(gm_kernel(mode, type), cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem)) !=
+                    cudaSuccess)
+                    return e;
+        for (auto kernel : {k_int8_dot<1, true>, k_int8_dot<2, true>, k_int8_dot<4, true>, k_int8_dot<1, false>,
+                            k_int8_dot<2, false>, k_int8_dot<4, false>})
+            if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDotSmemMax)) != cudaSuccess)
+                return e;
+        for (int size = 2; size <= kGmMaxSplit; ++size)
+            if ((e = gm_launch(nullptr, size == 2 ? kPair : kSplit, CLB_F32, 1, size, false, nullptr, &d.clusters[size])) !=
                 cudaSuccess)
                 return e;
-    for (auto kernel : {k_int8_dot<1>, k_int8_dot<2>, k_int8_dot<4>})
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDotSmemMax)) != cudaSuccess)
-            return e;
-    for (int size = 2; size <= kGmMaxSplit; ++size)
-        if ((e = gm_launch(nullptr, size == 2 ? kPair : kSplit, CLB_F32, 1, size, false, nullptr, &d.clusters[size])) !=
-            cudaSuccess)
-            return e;
-    ready[dev].store(true, std::memory_order_release);
-    return cudaSuccess;
+        return cudaSuccess;
+    });
+    *out = &devices[dev];
+    return e;
 }
 
 cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, const GmDevice& d, cudaStream_t s) {
@@ -862,8 +867,8 @@ cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, const
 constexpr int kDotTokens = 4;
 
 cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_t ld_x, const GmDevice& dev, cudaStream_t s) {
-    Int8Dot d{a, x, ld_x, x_type, 0, 1, (a.k + 15) & ~15, false};
-    d.vec = x && ops_aligned(x, 16) && ld_x * ops_type_bytes(x_type) % 16 == 0;
+    Int8Dot d{a, x, ld_x, x_type, 0, 1, (a.k + 15) & ~15};
+    const bool vec = !x || ops_vec8(x, x_type, ld_x);
     const int tt = a.tokens <= 1 ? 1 : a.tokens <= 2 ? 2 : 4;
     d.rows = std::min((a.n + dev.sms - 1) / dev.sms, kDotMaxSums / tt);
     // cut the rows so that the warps' shares are even: a round is kDotThreads / 32 items
@@ -873,7 +878,8 @@ cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_
         const double cost = (double)((d.rows * segs + warps - 1) / warps) / segs + 0.02 * segs;
         if (cost < least) least = cost, d.segs = segs;
     }
-    void (*kernel)(Int8Dot) = tt == 1 ? k_int8_dot<1> : tt == 2 ? k_int8_dot<2> : k_int8_dot<4>;
+    void (*kernel)(Int8Dot) = vec ? (tt == 1 ? k_int8_dot<1, true> : tt == 2 ? k_int8_dot<2, true> : k_int8_dot<4, true>)
+                                  : (tt == 1 ? k_int8_dot<1, false> : tt == 2 ? k_int8_dot<2, false> : k_int8_dot<4, false>);
     const size_t smem = (size_t)tt * d.kpad + (size_t)d.rows * tt * 4;
     return ops_launch(kernel, (unsigned)((a.n + d.rows - 1) / d.rows), kDotThreads, smem, s, d);
 }

@@ -6,6 +6,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
+
 #include "clb_host.h"
 
 namespace clb {
@@ -13,6 +16,10 @@ namespace clb {
 inline bool ops_float_type(int t) { return t == CLB_F32 || t == CLB_BF16 || t == CLB_F16; }
 inline int ops_type_bytes(int t) { return t == CLB_F32 ? 4 : t == CLB_I8 ? 1 : 2; }
 inline bool ops_aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Whether eight elements from a multiple of 8 on can be moved at once in every row (32 bytes of
+// fp32, 16 of the others).
+inline bool ops_vec8(const void* p, int type, int64_t ld) { return ops_aligned(p, type == CLB_F32 ? 32 : 16) && ld % 8 == 0; }
 
 // One element of a floating tensor; `type` is uniform over the grid.
 __device__ __forceinline__ float ops_load(const void* p, int type, int64_t i) {
@@ -26,32 +33,122 @@ __device__ __forceinline__ void ops_store(void* p, int type, int64_t i, float v)
     else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// Eight elements from i on, 16-byte aligned (coherent loads: the tensor may be updated in place).
-__device__ __forceinline__ void load8_aligned(const void* p, int type, int64_t i, float (&v)[8]) {
+// Eight elements as they lie in memory. Loading and converting are two steps, so that a thread
+// has all its loads in flight before it touches the first: the element type is a value of the
+// launch, and a conversion right behind each load would wait for it.
+struct Raw8 {
+    uint4 a, b;  // 16-bit types, aligned: in a; otherwise one element a word
+};
+// The loads are predicated, not branched around, and coherent: the tensor may be updated in place.
+__device__ __forceinline__ void ld16_if(uint4& v, const void* p, bool ok) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+                 : "l"(p), "r"((uint32_t)ok));
+}
+__device__ __forceinline__ void ld32_if(uint4& a, uint4& b, const void* p, bool ok) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %9, 0;\n\t"
+        "@p ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t}"
+        : "+r"(a.x), "+r"(a.y), "+r"(a.z), "+r"(a.w), "+r"(b.x), "+r"(b.y), "+r"(b.z), "+r"(b.w)
+        : "l"(p), "r"((uint32_t)ok));
+}
+__device__ __forceinline__ void ld_elem_if(uint32_t& v, const void* row, int type, int64_t i, bool ok) {
+    const char* p = static_cast<const char*>(row) + i * (type == CLB_F32 ? 4 : 2);
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u16 h;\n\tsetp.ne.u32 p, %2, 0;\n\tsetp.ne.u32 q, %3, 0;\n\t"
+        "@p ld.global.u32 %0, [%1];\n\t@q ld.global.u16 h, [%1];\n\t@q cvt.u32.u16 %0, h;\n\t}"
+        : "+r"(v)
+        : "l"(p), "r"((uint32_t)(ok && type == CLB_F32)), "r"((uint32_t)(ok && type != CLB_F32)));
+}
+// Aligned (ops_vec8): elements i .. i + 7 of `row`, where ok; zeros otherwise.
+__device__ __forceinline__ Raw8 raw8_aligned(const void* row, int type, int64_t i, bool ok) {
+    Raw8 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    const char* p = static_cast<const char*>(row) + i * (type == CLB_F32 ? 4 : 2);
+    ld32_if(r.a, r.b, p, ok && type == CLB_F32);
+    ld16_if(r.a, p, ok && type != CLB_F32);
+    return r;
+}
+// Any alignment: elements i + j * step for the j with i + j * step < n; zeros otherwise.
+__device__ __forceinline__ Raw8 raw8_strided(const void* row, int type, int64_t i, int step, int n) {
+    Raw8 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    ld_elem_if(r.a.x, row, type, i, i < n);
+    ld_elem_if(r.a.y, row, type, i + step, i + step < n);
+    ld_elem_if(r.a.z, row, type, i + 2 * step, i + 2 * step < n);
+    ld_elem_if(r.a.w, row, type, i + 3 * step, i + 3 * step < n);
+    ld_elem_if(r.b.x, row, type, i + 4 * step, i + 4 * step < n);
+    ld_elem_if(r.b.y, row, type, i + 5 * step, i + 5 * step < n);
+    ld_elem_if(r.b.z, row, type, i + 6 * step, i + 6 * step < n);
+    ld_elem_if(r.b.w, row, type, i + 7 * step, i + 7 * step < n);
+    return r;
+}
+// `packed`: from raw8_aligned.
+__device__ __forceinline__ void raw8_floats(const Raw8& r, int type, bool packed, float (&v)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
     if (type == CLB_F32) {
-        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        return;
-    }
-    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (type == CLB_BF16) {
-            v[2 * j] = __uint_as_float(w[j] << 16);
-            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    } else if (type == CLB_BF16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = __uint_as_float(!packed || !(j & 1) ? w[packed ? j / 2 : j] << 16 : w[j / 2] & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const uint32_t pair = packed ? w[j / 2] : w[j] | w[j + 1] << 16;
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+            v[j] = f.x, v[j + 1] = f.y;
         }
     }
+}
+
+// Eight elements from i on, aligned as for raw8_aligned.
+__device__ __forceinline__ void store8_aligned(void* p, int type, int64_t i, const float (&v)[8]) {
+    if (type == CLB_F32) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<float*>(p) + i), "f"(v[0]),
+                     "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+        return;
+    }
+    uint32_t w[4];
+    if (type == CLB_BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2 b = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ float ops_warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// SMs of the current device; `setup` (kernel attributes) runs once per device and call site.
+template <class Setup>
+cudaError_t ops_device(int* sms, Setup setup) {
+    constexpr int kDevices = 64;
+    static std::atomic<int> known[kDevices];  // 0: not set up yet
+    static std::mutex mutex;
+    int dev = 0;
+    cudaError_t e;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if (dev < 0 || dev >= kDevices) return cudaErrorInvalidDevice;
+    if ((*sms = known[dev].load(std::memory_order_acquire)) > 0) return cudaSuccess;
+    std::lock_guard<std::mutex> lock(mutex);
+    int count = 0;
+    if ((e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    if ((e = setup()) != cudaSuccess) return e;
+    known[dev].store(*sms = count, std::memory_order_release);
+    return cudaSuccess;
 }
 
 // Launch through cudaLaunchKernelEx, whose own status is the launch's (cudaGetLastError would

@@ -1,10 +1,13 @@
 // Routing to experts for models whose routing is neither of clb_route_device's modes: scores
 // of three kinds, a bias for balance, groups of experts, top-k, renormalised weights.
 //
-// Ranks are compared as fp32 values that are the same on every machine: a score is evaluated
-// in double and rounded once (the correctly rounded float, up to double's own last bits), the
-// bias is added in fp32, and ties go to the lower id. Without a bias the rank is the logit,
-// since every score rises with it, and only the picks' scores are evaluated.
+// Ranks are compared as fp32 values that are the same on every machine: a score is the
+// correctly rounded float, the bias is added in fp32, and ties go to the lower id. Without a
+// bias the rank is the logit, since every score rises with it. Evaluating every score in
+// double costs more than all the rest, so scores are first evaluated in fp32 with a known
+// error; if the picks (and the groups) are further apart than that error they are the same
+// as with exact scores, else the row is ranked again in double (about one row in a thousand
+// with continuous logits).
 #include <cmath>
 
 #include "clb_ops.cuh"
@@ -17,6 +20,7 @@ constexpr int kRouteMaxPicks = 16;
 constexpr int kRouteMaxGroups = 32;
 constexpr int kRouteWarps = 4;
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // rank_key(-inf): an expert that is not available
+constexpr float kHalfUlp = 0x1p-24f;
 
 struct RouteArgs {
     const void* logits;
@@ -26,7 +30,8 @@ struct RouteArgs {
     int* status;
     int64_t ld;
     int tokens, type, E, k, score, groups, top_groups, pair, renorm;
-    float scale;
+    int lanes_per_group;  // power of two, groups * lanes_per_group <= 32
+    float scale, per_inv;  // per_inv: groups / E
 };
 
 // Order-preserving map of a float to unsigned (-0 as +0); 0 is below every key.
@@ -34,112 +39,259 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
     const uint32_t u = __float_as_uint(__fadd_rn(v, 0.0f));
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ double score_of(int kind, double l, double top, double sum) {
-    if (kind == CLB_SCORE_SIGMOID) return 1.0 / (1.0 + exp(-l));
-    if (kind == CLB_SCORE_SOFTMAX) return exp(l - top) / sum;
-    return sqrt(fmax(l, 0.0) + log1p(exp(-fabs(l))));
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+
+// exp(l - top): the rounding of the difference, which the exponential would carry as a relative
+// error of |l - top| half ulps, is found exactly (the two-sum of l and -top) and put back.
+__device__ __forceinline__ float exp_diff(float l, float top) {
+    const float d = __fsub_rn(l, top), bb = __fsub_rn(d, l);
+    const float r = __fsub_rn(__fsub_rn(l, __fsub_rn(d, bb)), __fadd_rn(top, bb));
+    const float e = expf(d);
+    return d < -200.0f ? 0.0f : fmaf(e, r, e);  // e is 0 there, and d may be infinite
+}
+// A score in fp32. Error: expf and log1pf are within 2 ulp (4 half ulps each), __fdividef
+// within 2 ulp, the additions and the root half an ulp, so sigmoid and sqrt(softplus) are
+// within 9 half ulps; softmax divides by a sum of E terms whose chains are at most 37
+// additions long: within 6 + 6 + 37 + 4 half ulps.
+__device__ __forceinline__ float score_f32(int kind, float l, float top, float sum) {
+    if (kind == CLB_SCORE_SIGMOID) return __fdividef(1.0f, 1.0f + expf(-l));
+    if (kind == CLB_SCORE_SOFTMAX) return __fdividef(exp_diff(l, top), sum);
+    return sqrtf(fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))));
+}
+__device__ __noinline__ float score_exact(int kind, double l, double top, double sum) {
+    if (kind == CLB_SCORE_SIGMOID) return (float)(1.0 / (1.0 + exp(-l)));
+    if (kind == CLB_SCORE_SOFTMAX) return (float)(exp(l - top) / sum);
+    return (float)sqrt(fmax(l, 0.0) + log1p(exp(-fabs(l))));
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 
-// One warp per token; the row's keys and scores in shared memory.
-__global__ void __launch_bounds__(32 * kRouteWarps) k_route_experts(const RouteArgs a) {
-    extern __shared__ float route_smem[];
+// One warp per token, expert e = 32 i + lane in the lane's i-th register. SCORED: the ranks or the
+// groups' values need scores. Bound by latency and instructions (a token's 1.5 KB of logits
+// are read once).
+template <int NPL, bool SCORED>
+__global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 5 : 3) k_route_experts(const RouteArgs a) {
+    __shared__ uint2 cand_s[kRouteWarps][32];
+    __shared__ float vals_s[SCORED ? kRouteWarps : 1][SCORED ? NPL * 32 : 1];  // scores, then with their bias
+    const unsigned all = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * kRouteWarps + warp;
     if (t >= a.tokens) return;
-    uint32_t* key = reinterpret_cast<uint32_t*>(route_smem) + (size_t)warp * 2 * a.E;
-    float* sc = reinterpret_cast<float*>(key + a.E);
     const int64_t row = (int64_t)t * a.ld;
-    const unsigned all = 0xffffffffu;
+    int* ids = a.ids + (int64_t)t * a.k;
+    float* w = a.w + (int64_t)t * a.k;
 
+    uint32_t raw[NPL];
+    float l[NPL], b[NPL];
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+        raw[i] = 0;
+        b[i] = 0.0f;
+        const int e = 32 * i + lane;
+        ld_elem_if(raw[i], a.logits, a.type, row + e, e < a.E);
+        if (a.bias && e < a.E) b[i] = __ldg(a.bias + e);
+    }
     bool bad = false;
     float top = -INFINITY;
-    for (int e = lane; e < a.E; e += 32) {
-        const float l = ops_load(a.logits, a.type, row + e);
-        const float b = a.bias ? __ldg(a.bias + e) : 0.0f;
-        bad |= !(l < INFINITY) || !(b < INFINITY);
-        top = fmaxf(top, l);
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+        const bool in = 32 * i + lane < a.E;
+        l[i] = a.type == CLB_F32    ? __uint_as_float(raw[i])
+               : a.type == CLB_BF16 ? __uint_as_float(raw[i] << 16)
+                                    : __half2float(__ushort_as_half((uint16_t)raw[i]));
+        bad |= !(l[i] < INFINITY) || !(b[i] < INFINITY);
+        if (!in) l[i] = -INFINITY;
+        top = fmaxf(top, l[i]);
     }
     if (__any_sync(all, bad)) {
         if (lane == 0 && a.status) atomicExch(a.status, 1);
-        for (int i = lane; i < a.k; i += 32) {
-            a.ids[(int64_t)t * a.k + i] = i;
-            a.w[(int64_t)t * a.k + i] = __int_as_float(0x7fffffff);
+        if (lane < a.k) {
+            ids[lane] = lane;
+            w[lane] = __int_as_float(0x7fffffff);
         }
         return;
     }
-    double sum = 0.0;
+    float sum = 1.0f;
     if (a.score == CLB_SCORE_SOFTMAX) {
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(all, top, o));
-        for (int e = lane; e < a.E; e += 32) {
-            const float l = ops_load(a.logits, a.type, row + e);
-            if (l > -INFINITY) sum += exp((double)l - (double)top);
-        }
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(all, sum, o);
+        top = warp_max(top);
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+            if (l[i] > -INFINITY) sum += exp_diff(l[i], top);
+        sum = ops_warp_sum(sum);
     }
-    const bool pair = a.groups > 1 && a.pair;
-    for (int e = lane; e < a.E; e += 32) {
-        const float l = ops_load(a.logits, a.type, row + e);
-        const float b = a.bias ? __ldg(a.bias + e) : 0.0f;
-        uint32_t u = kKeyNegInf;
-        float s = 0.0f;
-        if (l > -INFINITY && b > -INFINITY) {
-            if (a.bias || pair) s = (float)score_of(a.score, l, top, sum);
-            u = rank_key(a.bias ? __fadd_rn(s, b) : l);
-        }
-        key[e] = u;
-        sc[e] = a.bias ? __fadd_rn(s, b) : s;  // what a pair of a group adds up
-    }
-    __syncwarp();
-    if (a.groups > 1) {
-        const int per = a.E / a.groups;
-        uint32_t gkey = 0;
-        if (lane < a.groups) {
-            uint32_t best = kKeyNegInf;
-            float v1 = -INFINITY, v2 = -INFINITY;
-            for (int i = 0; i < per; ++i) {
-                const uint32_t u = key[lane * per + i];
-                best = max(best, u);
-                if (u != kKeyNegInf) {
-                    const float v = sc[lane * per + i];
-                    v2 = fmaxf(v2, fminf(v1, v));
-                    v1 = fmaxf(v1, v);
-                }
-            }
-            gkey = !a.pair ? best : rank_key(v2 > -INFINITY ? __fadd_rn(v1, v2) : v1);
-        }
-        uint32_t kept = 0;
-        for (int i = 0; i < a.top_groups; ++i) {
-            const uint32_t m = __reduce_max_sync(all, gkey);
-            const int g = __ffs(__ballot_sync(all, gkey == m)) - 1;
-            kept |= 1u << g;
-            if (lane == g) gkey = 0;
-        }
-        for (int e = lane; e < a.E; e += 32)
-            if (!((kept >> (e / per)) & 1u)) key[e] = kKeyNegInf;
-        __syncwarp();
-    }
-    float mine = 0.0f;
+
+    uint32_t mine = 0;  // lane j: the key and id of the j-th largest rank
     int id = 0;
-    float total = 0.0f;
-    for (int i = 0; i < a.k; ++i) {
-        uint32_t best = 0;
-        int be = 0;
-        for (int e = lane; e < a.E; e += 32)
-            if (key[e] > best) best = key[e], be = e;
-        const uint32_t m = __reduce_max_sync(all, best);
-        const int e = (int)__reduce_min_sync(all, best == m ? (unsigned)be : 0xffffffffu);
-        if (e % 32 == lane) key[e] = 0;
-        float s = 0.0f;
-        if (m != kKeyNegInf) s = (float)score_of(a.score, ops_load(a.logits, a.type, row + e), top, sum);
-        total = __fadd_rn(total, s);
-        if (lane == i) mine = s, id = e;
+    float lj, s;        // lane j < k: logit and score of its pick
+    int exact = 0;
+#pragma unroll 1
+    for (;;) {
+        uint32_t key[NPL];
+        float off = 0.0f;  // largest error of a rank in this lane
+        if (SCORED) {
+            if (!exact) {
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) vals_s[warp][32 * i + lane] = score_f32(a.score, l[i], top, sum);
+            } else {  // rare: nothing kept in registers for it
+                double dsum = 1.0;
+                if (a.score == CLB_SCORE_SOFTMAX) {
+                    dsum = 0.0;
+#pragma unroll 1
+                    for (int e = lane; e < a.E; e += 32) {
+                        const float le = ops_load(a.logits, a.type, row + e);
+                        if (le > -INFINITY) dsum += exp((double)le - (double)top);
+                    }
+                    for (int o = 16; o > 0; o >>= 1) dsum += __shfl_xor_sync(all, dsum, o);
+                }
+#pragma unroll 1
+                for (int e = lane; e < a.E; e += 32)
+                    vals_s[warp][e] = score_exact(a.score, ops_load(a.logits, a.type, row + e), top, dsum);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            const int e = 32 * i + lane;
+            uint32_t u = e < a.E ? kKeyNegInf : 0u;
+            float v = -INFINITY;
+            if (l[i] > -INFINITY && b[i] > -INFINITY) {
+                if (SCORED) {
+                    const float sc = vals_s[warp][e];
+                    v = a.bias ? __fadd_rn(sc, b[i]) : sc;
+                    // one half ulp of the sum too, and the scores below the normal numbers
+                    off = fmaxf(off, fmaf(sc, (a.score == CLB_SCORE_SOFTMAX ? 64.0f : 16.0f) * kHalfUlp,
+                                          fmaf(fabsf(v), 2.0f * kHalfUlp, 1e-18f)));
+                }
+                u = rank_key(SCORED && a.bias ? v : l[i]);
+            }
+            key[i] = u;
+            if (SCORED && a.groups > 1) vals_s[warp][e] = v;
+        }
+        if (SCORED) off = exact ? 0.0f : __uint_as_float(__reduce_max_sync(all, __float_as_uint(off)));
+        bool unsure = false;
+        if (a.groups > 1) {
+            // lanes_per_group lanes find the two best of a group
+            const int per = a.E / a.groups, L = a.lanes_per_group, g = lane / L;
+            float v1 = -INFINITY, v2 = -INFINITY;
+            __syncwarp();
+            if (SCORED) {
+                if (g < a.groups)
+                    for (int i = lane % L; i < per; i += L) {
+                        const float v = vals_s[warp][g * per + i];
+                        v2 = fmaxf(v2, fminf(v1, v));
+                        v1 = fmaxf(v1, v);
+                    }
+            } else if (g < a.groups) {
+                for (int i = lane % L; i < per; i += L) v1 = fmaxf(v1, ops_load(a.logits, a.type, row + g * per + i));
+            }
+            __syncwarp();
+            for (int o = 1; o < L; o <<= 1) {
+                const float o1 = __shfl_xor_sync(all, v1, o), o2 = __shfl_xor_sync(all, v2, o);
+                v2 = fmaxf(fmaxf(v2, o2), fminf(v1, o1));
+                v1 = fmaxf(v1, o1);
+            }
+            const float value = a.pair && v2 > -INFINITY ? __fadd_rn(v1, v2) : v1;
+            uint32_t gkey = g < a.groups && lane % L == 0 ? rank_key(value) : 0u;
+            uint32_t kept = 0, last = 0;
+            for (int i = 0; i < a.top_groups; ++i) {
+                last = __reduce_max_sync(all, gkey);
+                const int at = __ffs(__ballot_sync(all, gkey == last)) - 1;
+                kept |= 1u << (at / L);
+                if (lane == at) gkey = 0;
+            }
+            if (SCORED && !exact && a.top_groups < a.groups) {
+                const uint32_t next = __reduce_max_sync(all, gkey);
+                const float lo = key_value(last), hi = key_value(next);
+                unsure = next != kKeyNegInf && !(lo - hi > 4.0f * off + 4.0f * kHalfUlp * (fabsf(lo) + fabsf(hi)));
+            }
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                const int e = 32 * i + lane, ge = (int)(((float)e + 0.5f) * a.per_inv);
+                if (e < a.E && !((kept >> ge) & 1u)) key[i] = kKeyNegInf;
+            }
+        }
+        // The k + 1 largest keys. The (k + 1)-th largest of the lanes' maxima is a lower bound of
+        // them: the few keys from there on are collected, one to a lane, and ranked by counting.
+        const int want = min(a.k + 1, a.E);
+        uint32_t cur = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) cur = max(cur, key[i]);
+        uint32_t bound = 0;
+        for (int i = 0; i < want; ++i) {
+            bound = __reduce_max_sync(all, cur);
+            if (cur == bound) cur = 0;
+        }
+        bound = max(bound, 1u);  // keys of 0 are no experts
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            const unsigned m = __ballot_sync(all, key[i] >= bound);
+            if (m) {
+                const int at = n + __popc(m & ((1u << lane) - 1u));
+                if (key[i] >= bound && at < 32) cand_s[warp][at] = make_uint2(key[i], (uint32_t)(32 * i + lane));
+                n += __popc(m);
+            }
+        }
         __syncwarp();
+        mine = 0, id = 0;
+        if (n <= 32) {
+            const uint2 c = lane < n ? cand_s[warp][lane] : make_uint2(0u, 0x7fffffffu);
+            int place = 0;
+            for (int j = 0; j < n; ++j) {
+                const uint2 o = cand_s[warp][j];
+                place += o.x > c.x || (o.x == c.x && o.y < c.y);
+            }
+            __syncwarp();
+            if (lane < n) cand_s[warp][place] = c;
+            __syncwarp();
+            if (lane < want) mine = cand_s[warp][lane].x, id = (int)cand_s[warp][lane].y;
+        } else {  // many equal keys: one pick at a time
+            for (int j = 0; j < want; ++j) {
+                uint32_t best = 0, at = 0xffffffffu;
+#pragma unroll
+                for (int i = 0; i < NPL; ++i)
+                    if (key[i] > best) best = key[i], at = (uint32_t)(32 * i + lane);
+                const uint32_t m = __reduce_max_sync(all, best);
+                const uint32_t e = __reduce_min_sync(all, best == m ? at : 0xffffffffu);
+#pragma unroll
+                for (int i = 0; i < NPL; ++i)
+                    if ((uint32_t)(32 * i + lane) == e) key[i] = 0;
+                if (lane == j) mine = m, id = (int)e;
+            }
+        }
+        __syncwarp();
+        lj = lane < want ? ops_load(a.logits, a.type, row + id) : 0.0f;
+        s = lane < a.k && mine != kKeyNegInf ? score_f32(a.score, lj, top, sum) : 0.0f;
+        if (!SCORED || exact) break;
+        // do the picks stand? Two experts of one logit and one bias have one rank, exactly
+        if (a.bias) {
+            const float bj = lane < want ? a.bias[id] : 0.0f, v = key_value(mine);
+            const uint32_t nkey = __shfl_down_sync(all, mine, 1);
+            const float nl = __shfl_down_sync(all, lj, 1), nb = __shfl_down_sync(all, bj, 1), nv = key_value(nkey);
+            if (lane + 1 < want && nkey != kKeyNegInf && !(lj == nl && bj == nb)) unsure |= !(v - nv > 2.0f * off);
+        }
+        if (!__any_sync(all, unsure)) break;
+        exact = 1;
     }
+    float total = 0.0f;
+    for (int i = 0; i < a.k; ++i) total = __fadd_rn(total, __shfl_sync(all, s, i));
     if (lane < a.k) {
-        if (a.renorm) mine = __fdiv_rn(mine, __fadd_rn(total, 1e-20f));
-        a.ids[(int64_t)t * a.k + lane] = id;
-        a.w[(int64_t)t * a.k + lane] = __fmul_rn(mine, a.scale);
+        if (a.renorm) s = __fdiv_rn(s, __fadd_rn(total, 1e-20f));
+        ids[lane] = id;
+        w[lane] = __fmul_rn(s, a.scale);
     }
+}
+
+template <bool SCORED>
+void (*route_kernel(int per_lane))(RouteArgs) {
+    return per_lane <= 4    ? k_route_experts<4, SCORED>
+           : per_lane <= 8  ? k_route_experts<8, SCORED>
+           : per_lane <= 12 ? k_route_experts<12, SCORED>
+           : per_lane <= 16 ? k_route_experts<16, SCORED>
+                            : k_route_experts<32, SCORED>;
 }
 
 }  // namespace
@@ -176,9 +328,13 @@ extern "C" int32_t clb_route_experts_device(const clb_route_config_v1* cfg, cons
                     clb::ops_aligned(d_ids, 4) && clb::ops_aligned(d_w, 4) && clb::ops_aligned(d_status, 4),
                 CLB_E_INVALID, "misaligned pointer argument");
         clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, c.score,
-                         c.n_groups, c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, c.scale};
-        cuda_check(clb::ops_launch(clb::k_route_experts, (unsigned)((tokens + clb::kRouteWarps - 1) / clb::kRouteWarps),
-                                   32 * clb::kRouteWarps, (size_t)clb::kRouteWarps * 2 * c.n_experts * 4,
+                         c.n_groups, c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, 1, c.scale,
+                         (float)c.n_groups / (float)c.n_experts};
+        while (2 * a.lanes_per_group * a.groups <= 32) a.lanes_per_group *= 2;
+        const bool scored = d_bias || (a.groups > 1 && a.pair);
+        const int per_lane = (c.n_experts + 31) / 32;
+        cuda_check(clb::ops_launch(scored ? clb::route_kernel<true>(per_lane) : clb::route_kernel<false>(per_lane),
+                                   (unsigned)((tokens + clb::kRouteWarps - 1) / clb::kRouteWarps), 32 * clb::kRouteWarps, 0,
                                    static_cast<cudaStream_t>(stream), a),
                    "routing");
     });
