@@ -6,8 +6,8 @@
 // bias the rank is the logit, since every score rises with it. Evaluating every score in
 // double costs more than all the rest, so scores are first evaluated in fp32 with a known
 // error; if the picks (and the groups) are further apart than that error they are the same
-// as with exact scores, else the row is ranked again in double (about one row in a thousand
-// with continuous logits).
+// as with exact scores, else (about one row in a thousand with continuous logits) the experts
+// in question are ranked in double.
 #include <cmath>
 
 #include "clb_ops.cuh"
@@ -29,7 +29,7 @@ struct RouteArgs {
     float* w;
     int* status;
     int64_t ld;
-    int tokens, type, E, k, score, groups, top_groups, pair, renorm;
+    int tokens, type, E, k, groups, top_groups, pair, renorm;
     int lanes_per_group;  // power of two, groups * lanes_per_group <= 32
     float scale, per_inv;  // per_inv: groups / E
 };
@@ -53,14 +53,16 @@ __device__ __forceinline__ float exp_diff(float l, float top) {
 // within 2 ulp, the additions and the root half an ulp, so sigmoid and sqrt(softplus) are
 // within 9 half ulps; softmax divides by a sum of E terms whose chains are at most 37
 // additions long: within 6 + 6 + 37 + 4 half ulps.
-__device__ __forceinline__ float score_f32(int kind, float l, float top, float sum) {
-    if (kind == CLB_SCORE_SIGMOID) return __fdividef(1.0f, 1.0f + expf(-l));
-    if (kind == CLB_SCORE_SOFTMAX) return __fdividef(exp_diff(l, top), sum);
+template <int KIND>
+__device__ __forceinline__ float score_f32(float l, float top, float sum) {
+    if (KIND == CLB_SCORE_SIGMOID) return __fdividef(1.0f, 1.0f + expf(-l));
+    if (KIND == CLB_SCORE_SOFTMAX) return __fdividef(exp_diff(l, top), sum);
     return sqrtf(fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))));
 }
-__device__ __noinline__ float score_exact(int kind, double l, double top, double sum) {
-    if (kind == CLB_SCORE_SIGMOID) return (float)(1.0 / (1.0 + exp(-l)));
-    if (kind == CLB_SCORE_SOFTMAX) return (float)(exp(l - top) / sum);
+template <int KIND>
+__device__ __noinline__ float score_exact(double l, double top, double sum) {
+    if (KIND == CLB_SCORE_SIGMOID) return (float)(1.0 / (1.0 + exp(-l)));
+    if (KIND == CLB_SCORE_SOFTMAX) return (float)(exp(l - top) / sum);
     return (float)sqrt(fmax(l, 0.0) + log1p(exp(-fabs(l))));
 }
 __device__ __forceinline__ float warp_max(float v) {
@@ -72,9 +74,9 @@ __device__ __forceinline__ float warp_max(float v) {
 // One warp per token, expert e = 32 i + lane in the lane's i-th register. SCORED: the ranks or the
 // groups' values need scores. Bound by latency and instructions (a token's 1.5 KB of logits
 // are read once).
-template <int NPL, bool SCORED>
+template <int NPL, int KIND, bool SCORED>
 __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 5 : 3) k_route_experts(const RouteArgs a) {
-    __shared__ uint2 cand_s[kRouteWarps][32];
+    __shared__ uint4 cand_s[kRouteWarps][32];                                      // key, id, logit, bias
     __shared__ float vals_s[SCORED ? kRouteWarps : 1][SCORED ? NPL * 32 : 1];  // scores, then with their bias
     const unsigned all = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -84,29 +86,42 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
     int* ids = a.ids + (int64_t)t * a.k;
     float* w = a.w + (int64_t)t * a.k;
 
-    uint32_t raw[NPL];
     float l[NPL], b[NPL];
+    {
+        uint32_t raw[NPL];
+        if (a.type == CLB_F32) {
+            const uint32_t* p = static_cast<const uint32_t*>(a.logits) + row;
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-        raw[i] = 0;
-        b[i] = 0.0f;
-        const int e = 32 * i + lane;
-        ld_elem_if(raw[i], a.logits, a.type, row + e, e < a.E);
-        if (a.bias && e < a.E) b[i] = __ldg(a.bias + e);
+            for (int i = 0; i < NPL; ++i) raw[i] = __ldg(p + min(32 * i + lane, a.E - 1));
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(a.logits) + row;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) raw[i] = __ldg(p + min(32 * i + lane, a.E - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) b[i] = 0.0f;
+        if (a.bias)
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) b[i] = __ldg(a.bias + min(32 * i + lane, a.E - 1));
+        if (a.type == CLB_F32) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) l[i] = __uint_as_float(raw[i]);
+        } else if (a.type == CLB_BF16) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) l[i] = __uint_as_float(raw[i] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) l[i] = __half2float(__ushort_as_half((uint16_t)raw[i]));
+        }
     }
-    bool bad = false;
+    bool fine = true;
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-        const bool in = 32 * i + lane < a.E;
-        l[i] = a.type == CLB_F32    ? __uint_as_float(raw[i])
-               : a.type == CLB_BF16 ? __uint_as_float(raw[i] << 16)
-                                    : __half2float(__ushort_as_half((uint16_t)raw[i]));
-        bad |= !(l[i] < INFINITY) || !(b[i] < INFINITY);
-        if (!in) l[i] = -INFINITY;
+        fine = fine && l[i] < INFINITY && b[i] < INFINITY;
         top = fmaxf(top, l[i]);
     }
-    if (__any_sync(all, bad)) {
+    if (!__all_sync(all, fine)) {
         if (lane == 0 && a.status) atomicExch(a.status, 1);
         if (lane < a.k) {
             ids[lane] = lane;
@@ -115,30 +130,33 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         return;
     }
     float sum = 1.0f;
-    if (a.score == CLB_SCORE_SOFTMAX) {
-        top = warp_max(top);
+    if (KIND == CLB_SCORE_SOFTMAX || SCORED) top = warp_max(top);
+    if (KIND == CLB_SCORE_SOFTMAX) {
         sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-            if (l[i] > -INFINITY) sum += exp_diff(l[i], top);
+            if (32 * i + lane < a.E && l[i] > -INFINITY) sum += exp_diff(l[i], top);
         sum = ops_warp_sum(sum);
     }
+    // the largest error of a score (s rises with l), and of the scores below the normal numbers
+    const float off = !SCORED ? 0.0f
+                              : fmaf(KIND == CLB_SCORE_SOFTMAX ? 64.0f * kHalfUlp : 16.0f * kHalfUlp,
+                                     KIND == CLB_SCORE_SQRT_SOFTPLUS ? score_f32<KIND>(top, 0.0f, 1.0f) : 1.0f, 1e-18f);
 
-    uint32_t mine = 0;  // lane j: the key and id of the j-th largest rank
+    uint32_t mine = 0;      // lane j: the key and id of the j-th largest rank
     int id = 0;
-    float lj, s;        // lane j < k: logit and score of its pick
+    float lj = 0.0f, s;     // lane j < k: logit and score of its pick
     int exact = 0;
 #pragma unroll 1
     for (;;) {
         uint32_t key[NPL];
-        float off = 0.0f;  // largest error of a rank in this lane
         if (SCORED) {
             if (!exact) {
 #pragma unroll
-                for (int i = 0; i < NPL; ++i) vals_s[warp][32 * i + lane] = score_f32(a.score, l[i], top, sum);
+                for (int i = 0; i < NPL; ++i) vals_s[warp][32 * i + lane] = score_f32<KIND>(l[i], top, sum);
             } else {  // rare: nothing kept in registers for it
                 double dsum = 1.0;
-                if (a.score == CLB_SCORE_SOFTMAX) {
+                if (KIND == CLB_SCORE_SOFTMAX) {
                     dsum = 0.0;
 #pragma unroll 1
                     for (int e = lane; e < a.E; e += 32) {
@@ -149,44 +167,33 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
                 }
 #pragma unroll 1
                 for (int e = lane; e < a.E; e += 32)
-                    vals_s[warp][e] = score_exact(a.score, ops_load(a.logits, a.type, row + e), top, dsum);
+                    vals_s[warp][e] = score_exact<KIND>(ops_load(a.logits, a.type, row + e), top, dsum);
             }
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
             const int e = 32 * i + lane;
-            uint32_t u = e < a.E ? kKeyNegInf : 0u;
-            float v = -INFINITY;
-            if (l[i] > -INFINITY && b[i] > -INFINITY) {
-                if (SCORED) {
-                    const float sc = vals_s[warp][e];
-                    v = a.bias ? __fadd_rn(sc, b[i]) : sc;
-                    // one half ulp of the sum too, and the scores below the normal numbers
-                    off = fmaxf(off, fmaf(sc, (a.score == CLB_SCORE_SOFTMAX ? 64.0f : 16.0f) * kHalfUlp,
-                                          fmaf(fabsf(v), 2.0f * kHalfUlp, 1e-18f)));
-                }
-                u = rank_key(SCORED && a.bias ? v : l[i]);
+            float v = l[i];
+            if (SCORED) {
+                const float sc = __fadd_rn(vals_s[warp][e], b[i]);  // without a bias b is 0
+                const bool there = l[i] > -INFINITY && b[i] > -INFINITY;
+                v = !there ? -INFINITY : a.bias ? sc : l[i];
+                if (a.groups > 1) vals_s[warp][e] = there ? sc : -INFINITY;
             }
-            key[i] = u;
-            if (SCORED && a.groups > 1) vals_s[warp][e] = v;
+            key[i] = e < a.E ? rank_key(v) : 0u;
         }
-        if (SCORED) off = exact ? 0.0f : __uint_as_float(__reduce_max_sync(all, __float_as_uint(off)));
         bool unsure = false;
         if (a.groups > 1) {
             // lanes_per_group lanes find the two best of a group
             const int per = a.E / a.groups, L = a.lanes_per_group, g = lane / L;
             float v1 = -INFINITY, v2 = -INFINITY;
             __syncwarp();
-            if (SCORED) {
-                if (g < a.groups)
-                    for (int i = lane % L; i < per; i += L) {
-                        const float v = vals_s[warp][g * per + i];
-                        v2 = fmaxf(v2, fminf(v1, v));
-                        v1 = fmaxf(v1, v);
-                    }
-            } else if (g < a.groups) {
-                for (int i = lane % L; i < per; i += L) v1 = fmaxf(v1, ops_load(a.logits, a.type, row + g * per + i));
-            }
+            if (g < a.groups)
+                for (int i = lane % L; i < per; i += L) {
+                    const float v = SCORED ? vals_s[warp][g * per + i] : ops_load(a.logits, a.type, row + g * per + i);
+                    v2 = fmaxf(v2, fminf(v1, v));
+                    v1 = fmaxf(v1, v);
+                }
             __syncwarp();
             for (int o = 1; o < L; o <<= 1) {
                 const float o1 = __shfl_xor_sync(all, v1, o), o2 = __shfl_xor_sync(all, v2, o);
@@ -203,9 +210,10 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
                 if (lane == at) gkey = 0;
             }
             if (SCORED && !exact && a.top_groups < a.groups) {
+                // a value's error: of two scores, of their ranks' roundings and of the sum's
                 const uint32_t next = __reduce_max_sync(all, gkey);
                 const float lo = key_value(last), hi = key_value(next);
-                unsure = next != kKeyNegInf && !(lo - hi > 4.0f * off + 4.0f * kHalfUlp * (fabsf(lo) + fabsf(hi)));
+                unsure = next != kKeyNegInf && !(lo - hi > 4.0f * (off + 2.0f * kHalfUlp * (fabsf(lo) + fabsf(hi))));
             }
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
@@ -224,74 +232,115 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
             bound = __reduce_max_sync(all, cur);
             if (cur == bound) cur = 0;
         }
-        bound = max(bound, 1u);  // keys of 0 are no experts
-        int n = 0;
+        // the keys from `from` on into shared memory, in the order of the ids; their number
+        auto collect = [&](uint32_t from) {
+            int n = 0;
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-            const unsigned m = __ballot_sync(all, key[i] >= bound);
-            if (m) {
-                const int at = n + __popc(m & ((1u << lane) - 1u));
-                if (key[i] >= bound && at < 32) cand_s[warp][at] = make_uint2(key[i], (uint32_t)(32 * i + lane));
-                n += __popc(m);
+            for (int i = 0; i < NPL; ++i) {
+                const unsigned m = __ballot_sync(all, key[i] >= from);
+                if (m) {
+                    const int at = n + __popc(m & ((1u << lane) - 1u));
+                    if (key[i] >= from && at < 32)
+                        cand_s[warp][at] =
+                            make_uint4(key[i], (uint32_t)(32 * i + lane), __float_as_uint(l[i]), __float_as_uint(b[i]));
+                    n += __popc(m);
+                }
             }
-        }
-        __syncwarp();
-        mine = 0, id = 0;
-        if (n <= 32) {
-            const uint2 c = lane < n ? cand_s[warp][lane] : make_uint2(0u, 0x7fffffffu);
+            __syncwarp();
+            return n;
+        };
+        // lane j < n brings a candidate, collected as its j-th, and takes the j-th largest
+        float bj = 0.0f;
+        auto order = [&](uint4 c, int n) {
             int place = 0;
             for (int j = 0; j < n; ++j) {
-                const uint2 o = cand_s[warp][j];
-                place += o.x > c.x || (o.x == c.x && o.y < c.y);
+                const uint32_t ok = cand_s[warp][j].x;
+                place += ok > c.x || (ok == c.x && j < lane);
             }
             __syncwarp();
             if (lane < n) cand_s[warp][place] = c;
             __syncwarp();
-            if (lane < want) mine = cand_s[warp][lane].x, id = (int)cand_s[warp][lane].y;
+            c = cand_s[warp][lane];
+            mine = c.x, id = (int)c.y, lj = __uint_as_float(c.z), bj = __uint_as_float(c.w);
+            __syncwarp();
+        };
+        const int n = collect(max(bound, 1u));  // keys of 0 are no experts
+        if (n <= 32) {
+            order(cand_s[warp][lane], n);
         } else {  // many equal keys: one pick at a time
+            uint32_t left[NPL];
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) left[i] = key[i];
             for (int j = 0; j < want; ++j) {
                 uint32_t best = 0, at = 0xffffffffu;
 #pragma unroll
                 for (int i = 0; i < NPL; ++i)
-                    if (key[i] > best) best = key[i], at = (uint32_t)(32 * i + lane);
+                    if (left[i] > best) best = left[i], at = (uint32_t)(32 * i + lane);
                 const uint32_t m = __reduce_max_sync(all, best);
                 const uint32_t e = __reduce_min_sync(all, best == m ? at : 0xffffffffu);
 #pragma unroll
                 for (int i = 0; i < NPL; ++i)
-                    if ((uint32_t)(32 * i + lane) == e) key[i] = 0;
+                    if ((uint32_t)(32 * i + lane) == e) left[i] = 0;
                 if (lane == j) mine = m, id = (int)e;
             }
+            if (lane < want) {
+                lj = ops_load(a.logits, a.type, row + id);
+                if (a.bias) bj = a.bias[id];
+            }
         }
-        __syncwarp();
-        lj = lane < want ? ops_load(a.logits, a.type, row + id) : 0.0f;
-        s = lane < a.k && mine != kKeyNegInf ? score_f32(a.score, lj, top, sum) : 0.0f;
         if (!SCORED || exact) break;
-        // do the picks stand? Two experts of one logit and one bias have one rank, exactly
-        if (a.bias) {
-            const float bj = lane < want ? a.bias[id] : 0.0f, v = key_value(mine);
-            const uint32_t nkey = __shfl_down_sync(all, mine, 1);
-            const float nl = __shfl_down_sync(all, lj, 1), nb = __shfl_down_sync(all, bj, 1), nv = key_value(nkey);
-            if (lane + 1 < want && nkey != kKeyNegInf && !(lj == nl && bj == nb)) unsure |= !(v - nv > 2.0f * off);
+        if (__any_sync(all, unsure)) {  // of the groups
+            exact = 1;
+            continue;
         }
+        if (!a.bias) break;
+        // do the picks stand? Two experts of one logit and one bias have one rank, exactly
+        const uint32_t nkey = __shfl_down_sync(all, mine, 1);
+        const float nl = __shfl_down_sync(all, lj, 1), nb = __shfl_down_sync(all, bj, 1);
+        const float v = key_value(mine), nv = key_value(nkey);
+        if (lane + 1 < want && nkey != kKeyNegInf && !(lj == nl && bj == nb))
+            unsure = !(v - nv > 2.0f * (off + kHalfUlp * (fabsf(v) + fabsf(nv))));
         if (!__any_sync(all, unsure)) break;
-        exact = 1;
+        // whoever can be among the picks: an exact rank for each, a lane apiece
+        const float least = __shfl_sync(all, v, a.k - 1), margin = 4.0f * (off + 2.0f * kHalfUlp * fabsf(least));
+        const int close = KIND == CLB_SCORE_SOFTMAX || !(least > -INFINITY) ? 33 : collect(rank_key(least - margin));
+        if (close > 32) {
+            exact = 1;
+            continue;
+        }
+        uint4 c = cand_s[warp][lane];
+        if (lane < close && c.x != kKeyNegInf)
+            c.x = rank_key(__fadd_rn(score_exact<KIND>(__uint_as_float(c.z), 0.0, 1.0), __uint_as_float(c.w)));
+        if (lane < close) cand_s[warp][lane].x = c.x;
+        __syncwarp();
+        order(c, close);
+        break;
     }
-    float total = 0.0f;
-    for (int i = 0; i < a.k; ++i) total = __fadd_rn(total, __shfl_sync(all, s, i));
+    s = lane < a.k && mine != kKeyNegInf ? score_f32<KIND>(lj, top, sum) : 0.0f;
+    if (a.renorm) {
+        float total = 0.0f;
+        for (int i = 0; i < a.k; ++i) total = __fadd_rn(total, __shfl_sync(all, s, i));
+        s = __fdiv_rn(s, __fadd_rn(total, 1e-20f));
+    }
     if (lane < a.k) {
-        if (a.renorm) s = __fdiv_rn(s, __fadd_rn(total, 1e-20f));
         ids[lane] = id;
         w[lane] = __fmul_rn(s, a.scale);
     }
 }
 
-template <bool SCORED>
+template <int KIND, bool SCORED>
 void (*route_kernel(int per_lane))(RouteArgs) {
-    return per_lane <= 4    ? k_route_experts<4, SCORED>
-           : per_lane <= 8  ? k_route_experts<8, SCORED>
-           : per_lane <= 12 ? k_route_experts<12, SCORED>
-           : per_lane <= 16 ? k_route_experts<16, SCORED>
-                            : k_route_experts<32, SCORED>;
+    return per_lane <= 4    ? k_route_experts<4, KIND, SCORED>
+           : per_lane <= 8  ? k_route_experts<8, KIND, SCORED>
+           : per_lane <= 12 ? k_route_experts<12, KIND, SCORED>
+           : per_lane <= 16 ? k_route_experts<16, KIND, SCORED>
+                            : k_route_experts<32, KIND, SCORED>;
+}
+template <bool SCORED>
+void (*route_kernel(int kind, int per_lane))(RouteArgs) {
+    return kind == CLB_SCORE_SIGMOID   ? route_kernel<CLB_SCORE_SIGMOID, SCORED>(per_lane)
+           : kind == CLB_SCORE_SOFTMAX ? route_kernel<CLB_SCORE_SOFTMAX, SCORED>(per_lane)
+                                       : route_kernel<CLB_SCORE_SQRT_SOFTPLUS, SCORED>(per_lane);
 }
 
 }  // namespace
@@ -327,13 +376,13 @@ extern "C" int32_t clb_route_experts_device(const clb_route_config_v1* cfg, cons
         require(clb::ops_aligned(d_logits, clb::ops_type_bytes(c.logits_type)) && clb::ops_aligned(d_bias, 4) &&
                     clb::ops_aligned(d_ids, 4) && clb::ops_aligned(d_w, 4) && clb::ops_aligned(d_status, 4),
                 CLB_E_INVALID, "misaligned pointer argument");
-        clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, c.score,
-                         c.n_groups, c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, 1, c.scale,
+        clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, c.n_groups,
+                         c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, 1, c.scale,
                          (float)c.n_groups / (float)c.n_experts};
         while (2 * a.lanes_per_group * a.groups <= 32) a.lanes_per_group *= 2;
         const bool scored = d_bias || (a.groups > 1 && a.pair);
         const int per_lane = (c.n_experts + 31) / 32;
-        cuda_check(clb::ops_launch(scored ? clb::route_kernel<true>(per_lane) : clb::route_kernel<false>(per_lane),
+        cuda_check(clb::ops_launch(scored ? clb::route_kernel<true>(c.score, per_lane) : clb::route_kernel<false>(c.score, per_lane),
                                    (unsigned)((tokens + clb::kRouteWarps - 1) / clb::kRouteWarps), 32 * clb::kRouteWarps, 0,
                                    static_cast<cudaStream_t>(stream), a),
                    "routing");
