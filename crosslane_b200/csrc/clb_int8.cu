@@ -546,13 +546,13 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     // weights do not depend on the quantising kernel in front: their first loads go out before
     // that kernel has finished, the tokens' after
     const int ahead = (int)min((int64_t)g.stages, total);
+    const uint32_t lead = PAIR ? cluster_addr(full(0), 0) : full(0);  // the stages' full barriers
     if (tid == 32 * kGmLoadWarp) {
-        int tile = first, kb = 0;
+        int tile = first, kb = 0, row = row_of(tile);
         for (int i = 0; i < ahead; ++i) {
             if (rank == 0 || !PAIR) mbar_expect_tx(full(i), (PAIR ? 2u : 1u) * stage_bytes);
-            gm_load<PAIR>(base + (uint32_t)i * stage_bytes, &g.wmap, (kb0 + kb) * 128, row_of(tile),
-                          PAIR ? cluster_addr(full(i), 0) : full(i));
-            if (++kb == nkb) kb = 0, tile += step;
+            gm_load<PAIR>(base + (uint32_t)i * stage_bytes, &g.wmap, (kb0 + kb) * 128, row, lead + 8u * (uint32_t)i);
+            if (++kb == nkb) kb = 0, tile += step, row = row_of(tile);
         }
     }
     __syncwarp();
@@ -568,19 +568,25 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     if (warp == kGmLoadWarp) {
         if (lane == 0) {
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            int tile = first, kb = 0, stage = 0;
+            // the place of a tile is found once a tile: the divisions in front of every copy would cost
+            // more than the block's products
+            int stage = 0, left = ahead;
             uint32_t phase = 0;
-            for (int64_t i = 0; i < total; ++i) {
-                const uint32_t a = base + (uint32_t)stage * stage_bytes;
-                const uint32_t bar = PAIR ? cluster_addr(full(stage), 0) : full(stage);
-                if (i >= ahead) {
-                    if (!gm_wait(empty(stage), phase ^ 1u, abort_flag, g.status)) break;
-                    if (rank == 0 || !PAIR) mbar_expect_tx(full(stage), (PAIR ? 2u : 1u) * stage_bytes);
-                    gm_load<PAIR>(a, &g.wmap, (kb0 + kb) * 128, row_of(tile), bar);
+            bool ok = true;
+            for (int i = 0; i < my_tiles && ok; ++i) {
+                const int row = row_of(first + i * step), token = token_of(first + i * step) + (PAIR ? brows * rank : 0);
+                for (int x = kb0 * 128; x < (kb0 + nkb) * 128; x += 128) {
+                    const uint32_t a = base + (uint32_t)stage * stage_bytes, bar = lead + 8u * (uint32_t)stage;
+                    if (left > 0) {  // the weights are on their way
+                        --left;
+                    } else {
+                        if (!(ok = gm_wait(empty(stage), phase ^ 1u, abort_flag, g.status))) break;
+                        if (rank == 0 || !PAIR) mbar_expect_tx(full(stage), (PAIR ? 2u : 1u) * stage_bytes);
+                        gm_load<PAIR>(a, &g.wmap, x, row, bar);
+                    }
+                    gm_load<PAIR>(a + kGmABytes, &g.xmap, x, token, bar);
+                    if (++stage == g.stages) stage = 0, phase ^= 1u;
                 }
-                gm_load<PAIR>(a + kGmABytes, &g.xmap, (kb0 + kb) * 128, token_of(tile) + (PAIR ? brows * rank : 0), bar);
-                if (++stage == g.stages) stage = 0, phase ^= 1u;
-                if (++kb == nkb) kb = 0, tile += step;
             }
         }
     } else if (warp == kGmMmaWarp) {
