@@ -29,6 +29,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 class _Local(threading.local):
     def __init__(self):
         self.err = ErrorV1()
@@ -91,7 +94,7 @@ def _call(fn, index, stream, *args):
     """fn(*args, stream, err) with device `index` current."""
     if stream is None:
         stream = _raw_stream(index)
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, stream, _local.ref)
     else:
         with torch.cuda.device(index):

@@ -64,10 +64,26 @@ __device__ __forceinline__ float gate_value(float g, int sigmoid) {
     return sigmoid ? __fdividef(1.0f, 1.0f + expf(-g)) : g;
 }
 
+// The element types of a call as constants where they are a usual set (told apart at run time,
+// they cost a bandwidth-bound kernel in 16 bits a third of its rate).
+enum : int { kTypesAny = 0, kTypesF32, kTypesBF16, kTypesF16, kTypesF32BF16, kTypesF32F16 };  // the last two: h fp32
+struct NormTypes {
+    int h, other;
+};
+__host__ __device__ constexpr NormTypes norm_types(int set) {
+    return set == kTypesF32    ? NormTypes{CLB_F32, CLB_F32}
+           : set == kTypesBF16 ? NormTypes{CLB_BF16, CLB_BF16}
+           : set == kTypesF16  ? NormTypes{CLB_F16, CLB_F16}
+           : set == kTypesF32BF16 ? NormTypes{CLB_F32, CLB_BF16}
+                                  : NormTypes{CLB_F32, CLB_F16};
+}
+
 // One CTA per row, CH chunks of 8 values per thread: few rows, where the latency of one counts,
 // rows that are not aligned, and rows too wide for k_block_norm_rows.
-template <int CH, bool VEC>
+template <int CH, bool VEC, int SET>
 __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
+    const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
+    const int x_type = SET ? norm_types(SET).other : a.x_type;
     __shared__ float part[2][32];
     const int64_t row = blockIdx.x;
     const bool wide_gate = a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL;
@@ -75,9 +91,9 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     float v[CH][8];
     if (a.y)
 #pragma unroll
-        for (int c = 0; c < CH; ++c) yr[c] = load8<VEC>(a.y, a.y_type, row * a.ld_y, c, a.dim);
+        for (int c = 0; c < CH; ++c) yr[c] = load8<VEC>(a.y, y_type, row * a.ld_y, c, a.dim);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) hr[c] = load8<VEC>(a.h, a.h_type, row * a.ld_h, c, a.dim);
+    for (int c = 0; c < CH; ++c) hr[c] = load8<VEC>(a.h, h_type, row * a.ld_h, c, a.dim);
     if (CH == 1 && wide_gate) gr[0] = load8<VEC>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, 0, a.dim);
     if (a.y) {
         float gt = 1.0f;
@@ -87,7 +103,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
             float ss = 0.0f, y[8];
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                raw8_floats(yr[c], a.y_type, VEC, y);
+                raw8_floats(yr[c], y_type, VEC, y);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
             }
@@ -97,7 +113,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             float y[8], w[8];
-            raw8_floats(yr[c], a.y_type, VEC, y);
+            raw8_floats(yr[c], y_type, VEC, y);
             if (a.w_post) {
                 raw8_floats(load8<VEC>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, VEC, w);
 #pragma unroll
@@ -109,14 +125,14 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] *= gate_value(w[j], a.gate_sigmoid);
             }
-            raw8_floats(hr[c], a.h_type, VEC, v[c]);
+            raw8_floats(hr[c], h_type, VEC, v[c]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[c][j] = fmaf(f, y[j], a.residual_scale * v[c][j]);
-            store8<VEC>(a.h_out, a.h_type, row * a.ld_h_out, c, a.dim, v[c]);
+            store8<VEC>(a.h_out, h_type, row * a.ld_h_out, c, a.dim, v[c]);
         }
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) raw8_floats(hr[c], a.h_type, VEC, v[c]);
+        for (int c = 0; c < CH; ++c) raw8_floats(hr[c], h_type, VEC, v[c]);
     }
     if (a.x) {
         float ss = 0.0f;
@@ -131,7 +147,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
             if (a.w_pre) raw8_floats(load8<VEC>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, VEC, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = a.w_pre ? w[j] * (v[c][j] * inv) : v[c][j] * inv;
-            store8<VEC>(a.x, a.x_type, row * a.ld_x, c, a.dim, w);
+            store8<VEC>(a.x, x_type, row * a.ld_x, c, a.dim, w);
         }
     }
 }
@@ -144,20 +160,6 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 // them, and several CTAs an SM hide the sums' latency.
 constexpr int kRowStages = 4;
 constexpr uint32_t kRowPolls = 1u << 20;  // waits for a copy, each with a suspend hint of 20 us
-
-// The element types of a call as constants where they are a usual set (told apart at run time,
-// they cost a bandwidth-bound kernel in 16 bits a third of its rate).
-enum : int { kTypesAny = 0, kTypesF32, kTypesBF16, kTypesF16, kTypesF32BF16, kTypesF32F16 };  // the last two: h fp32
-struct NormTypes {
-    int h, other;
-};
-__host__ __device__ constexpr NormTypes norm_types(int set) {
-    return set == kTypesF32    ? NormTypes{CLB_F32, CLB_F32}
-           : set == kTypesBF16 ? NormTypes{CLB_BF16, CLB_BF16}
-           : set == kTypesF16  ? NormTypes{CLB_F16, CLB_F16}
-           : set == kTypesF32BF16 ? NormTypes{CLB_F32, CLB_BF16}
-                                  : NormTypes{CLB_F32, CLB_F16};
-}
 
 // Eight values, number i of a row in shared memory.
 __device__ __forceinline__ void row8(uint32_t p, int type, int i, float (&v)[8]) {
@@ -307,11 +309,34 @@ decltype(rows_kernel<kTypesAny>(0, 0)) rows_kernel(int set, int ch, int threads)
                                   : rows_kernel<kTypesAny>(ch, threads);
 }
 
+template <int SET>
+void (*row_kernel(int ch, bool vec))(NormArgs) {
+    return vec ? (ch == 1 ? k_block_norm<1, true, SET> : ch == 2 ? k_block_norm<2, true, SET> : k_block_norm<4, true, SET>)
+               : (ch == 1   ? k_block_norm<1, false, SET>
+                  : ch == 2 ? k_block_norm<2, false, SET>
+                            : k_block_norm<4, false, SET>);
+}
+void (*row_kernel(int set, int ch, bool vec))(NormArgs) {
+    return set == kTypesF32       ? row_kernel<kTypesF32>(ch, vec)
+           : set == kTypesBF16    ? row_kernel<kTypesBF16>(ch, vec)
+           : set == kTypesF16     ? row_kernel<kTypesF16>(ch, vec)
+           : set == kTypesF32BF16 ? row_kernel<kTypesF32BF16>(ch, vec)
+           : set == kTypesF32F16  ? row_kernel<kTypesF32F16>(ch, vec)
+                                  : row_kernel<kTypesAny>(ch, vec);
+}
+
 cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStream_t s) {
     const int units = (a.dim + 7) / 8;
     const uint32_t y_bytes = a.y ? a.dim * ops_type_bytes(a.y_type) : 0, h_bytes = a.dim * ops_type_bytes(a.h_type);
     const uint32_t g_bytes = a.gate_kind == CLB_GATE_FULL ? a.dim * ops_type_bytes(a.gate_type) : 0;
     const uint32_t stage = y_bytes + h_bytes + g_bytes;
+    int set = kTypesAny;
+    for (int i = kTypesF32; i <= kTypesF32F16; ++i) {
+        const NormTypes t = norm_types(i);
+        if (a.h_type == t.h && (!a.y || a.y_type == t.other) && (!a.x || a.x_type == t.other) &&
+            (!g_bytes || a.gate_type == t.other))
+            set = i;
+    }
     if (vec && tokens > kNormFewRows && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
         int ch = units <= 32 ? 1 : units <= 64 ? 2 : 4;
         auto threads_of = [&](int chunks) { return std::max(32, ((units + chunks - 1) / chunks + 31) / 32 * 32); };
@@ -320,13 +345,6 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStrea
         while (ctas > 1 && kRowSmem / ctas / (int)stage < 2) --ctas;
         if (ctas == 1 && units > 512 && units <= 1024) ch = 2;  // one CTA: more warps
         const int threads = threads_of(ch), stages = std::min(kRowStages, kRowSmem / ctas / (int)stage);
-        int set = kTypesAny;
-        for (int i = kTypesF32; i <= kTypesF32F16; ++i) {
-            const NormTypes t = norm_types(i);
-            if (a.h_type == t.h && (!a.y || a.y_type == t.other) && (!a.x || a.x_type == t.other) &&
-                (!g_bytes || a.gate_type == t.other))
-                set = i;
-        }
         int sms = 0;
         const cudaError_t e = ops_device(&sms, [] {
             cudaError_t e = cudaSuccess;
@@ -344,10 +362,7 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStrea
     }
     const int ch = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
     const int threads = std::max(32, ((units + ch - 1) / ch + 31) / 32 * 32);
-    void (*kernel)(NormArgs) = vec ? (ch == 1 ? k_block_norm<1, true> : ch == 2 ? k_block_norm<2, true> : k_block_norm<4, true>)
-                                   : (ch == 1   ? k_block_norm<1, false>
-                                      : ch == 2 ? k_block_norm<2, false>
-                                                : k_block_norm<4, false>);
+    void (*kernel)(NormArgs) = row_kernel(set, ch, vec);
     return ops_launch(kernel, (unsigned)tokens, threads, 0, s, a);
 }
 

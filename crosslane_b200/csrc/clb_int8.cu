@@ -46,25 +46,52 @@ __device__ __forceinline__ RowScale row_scale(float m, float* stored) {
     *stored = m < INFINITY ? s : __int_as_float(0x7fffffff);
     return r;
 }
-// Eight quotients as bytes. x * inv is within 127 * 2^-22.4 = 2.4e-5 of the quotient, so its
-// rounding (by the addition of 1.5 * 2^23, whose low byte is the integer) stands unless it
-// lies that close to a border; only then, and for tiny rows, the exact form decides.
-__device__ __forceinline__ uint2 quant8(const float (&v)[8], const RowScale& r) {
-    if (r.zero) return make_uint2(0u, 0u);
+// Eight quotients as bytes, of rows whose scale is a subnormal number (out of line).
+__device__ __noinline__ uint2 quant8_exact(float v0, float v1, float v2, float v3, float v4, float v5, float v6, float v7,
+                                           float scale, float inv, float lift) {
+    const float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
     uint32_t q[8];
-    float off = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = (uint32_t)quant_exact(v[j] * lift, scale, inv) & 0xffu;
+    return make_uint2(q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24);
+}
+// The low byte of the result is the integer nearest to x / scale, for a quotient t = x * inv that is
+// within 127 * 2^-22.4 = 2.4e-5 of it and was rounded by adding 1.5 * 2^23 (f): where t lies so
+// close to a border, the exact remainder moves the integer by one if it has to be.
+__device__ __forceinline__ uint32_t quant_settle(float x, float f, float scale) {
+    const float r = fmaf(-(f - 12582912.0f), scale, x), two = fabsf(r + r);
+    const uint32_t q = __float_as_uint(f);
+    const bool move = two > scale || (two == scale && (q & 1u));
+    return !move ? q : r > 0.0f ? q + 1u : q - 1u;
+}
+constexpr float kQuantSure = 0.49997f;  // a rounding to a distance below this stands
+
+// Eight quotients as bytes. Values of 16 bits hit the borders exactly every few hundred times, so
+// that path is short too; tiny rows take the general form.
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], const RowScale& r) {
+    float f[8], off = 0.0f;
+    uint32_t q[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float t = v[j] * r.inv, f = t + 12582912.0f;
-        q[j] = __float_as_uint(f);
-        off = fmaxf(off, fabsf(t - (f - 12582912.0f)));
+        const float t = v[j] * r.inv;
+        f[j] = t + 12582912.0f;
+        q[j] = __float_as_uint(f[j]);
+        off = fmaxf(off, fabsf(t - (f[j] - 12582912.0f)));
     }
-    if (r.tiny || off > 0.49997f) {
+    if (off > kQuantSure)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = (uint32_t)quant_exact(r.tiny ? v[j] * 0x1p100f : v[j], r.scale, r.inv);
-    }
-    return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
-                      __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+        for (int j = 0; j < 8; ++j) q[j] = quant_settle(v[j], f[j], r.scale);
+    uint2 b = make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                         __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+    if (r.zero) b = make_uint2(0u, 0u);
+    else if (r.tiny) b = quant8_exact(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], r.scale, r.inv, 0x1p100f);
+    return b;
+}
+__device__ __forceinline__ int8_t quant1(float v, const RowScale& r) {
+    if (r.zero) return 0;
+    if (r.tiny) return (int8_t)quant_exact(v * 0x1p100f, r.scale, r.inv);
+    const float t = v * r.inv, f = t + 12582912.0f;
+    return (int8_t)(fabsf(t - (f - 12582912.0f)) > kQuantSure ? quant_settle(v, f, r.scale) : __float_as_uint(f));
 }
 // The larger magnitude; NaN if either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -83,94 +110,116 @@ struct QuantArgs {
     int8_t* q;
     float* scale;
     int64_t ld_x, ld_q;
-    int type, k, chunks;  // chunks of 8 columns that are written: k / 8 rounded up, plus zeros up to a pitch
+    int k, limit;  // columns of x; columns of q that are written (zeros behind k)
 };
-
-// Eight values from column 8c on, zeros behind k.
-template <bool VEC>
-__device__ __forceinline__ Raw8 raw_x8(const void* row, int type, int c, int k) {
-    if (!VEC) return raw8_strided(row, type, 8 * (int64_t)c, 1, k);
-    Raw8 r = raw8_aligned(row, type, 8 * (int64_t)c, 8 * c + 8 <= k);
-    if (8 * c < k && 8 * c + 8 > k) {  // the row's last chunk, into the aligned form
-        r = raw8_strided(row, type, 8 * (int64_t)c, 1, k);
-        if (type != CLB_F32)
-            r = Raw8{make_uint4(r.a.x | r.a.y << 16, r.a.z | r.a.w << 16, r.b.x | r.b.y << 16, r.b.z | r.b.w << 16),
-                     make_uint4(0, 0, 0, 0)};
-    }
-    return r;
-}
 __device__ __forceinline__ const void* row_at(const void* x, int type, int64_t element) {
     return static_cast<const char*>(x) + element * (type == CLB_F32 ? 4 : 2);
 }
-// q is 16-byte aligned with a pitch of a multiple of 16: eight bytes at once, but columns
-// behind `limit` are not touched.
-__device__ __forceinline__ void store_q8(int8_t* q, int c, int limit, uint2 v) {
-    if (8 * c + 8 <= limit) {
-        *reinterpret_cast<uint2*>(q + 8 * c) = v;
-    } else {
-        for (int j = 0; 8 * c + j < limit; ++j) q[8 * c + j] = (int8_t)((j < 4 ? v.x >> (8 * j) : v.y >> (8 * j - 32)) & 0xffu);
-    }
+// The largest magnitude of a row from the threads' own, the same in every thread.
+__device__ __forceinline__ float cta_max_nan(float m, float* part) {
+    m = warp_max_nan(m);
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+    return warp_max_nan(lane < (int)(blockDim.x >> 5) ? part[lane] : 0.0f);
+}
+__device__ __forceinline__ float max8_nan(const float (&v)[8], float m) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+    return m;
 }
 
-// One CTA per row, CH chunks of 8 values a thread in registers, or (CH = 0) the row read
-// twice. Bound by the row's bytes; the product behind it may start loading its weights.
-template <int CH, bool VEC>
-__global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a, int limit) {
+// Aligned rows over the CTAs, CH chunks of 8 values a thread in registers; or (CH = 0) rows too
+// long for that, each read twice. The columns behind the last whole chunk are single values of
+// the first threads. Bound by the rows' bytes; the product behind it may start loading its
+// weights.
+template <int CH, int TYPE>
+__global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
     __shared__ float part[32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const void* row = row_at(a.x, a.type, (int64_t)blockIdx.x * a.ld_x);
+    const int tid = threadIdx.x, nt = blockDim.x, chunks = a.k >> 3, last = 8 * chunks + tid;
+    const void* x = row_at(a.x, TYPE, (int64_t)blockIdx.x * a.ld_x);
     int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
-    const int tid = threadIdx.x, nt = blockDim.x;
     Raw8 raw[CH ? CH : 1];
     float v[8], m = 0.0f;
-    auto largest = [&](const Raw8& r) {
-        raw8_floats(r, a.type, VEC, v);
+    if (CH)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
-    };
+        for (int i = 0; i < CH; ++i) raw[i] = raw8_aligned(x, TYPE, 8 * (int64_t)(tid + i * nt), tid + i * nt < chunks);
+    const float tail = last < a.k ? ops_load(x, TYPE, last) : 0.0f;
     if (CH) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) raw[i] = raw_x8<VEC>(row, a.type, tid + i * nt, a.k);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) largest(raw[i]);
+        for (int i = 0; i < CH; ++i) {
+            raw8_floats(raw[i], TYPE, true, v);
+            m = max8_nan(v, m);
+        }
     } else {
-        for (int c = tid; c < a.chunks; c += nt) largest(raw_x8<VEC>(row, a.type, c, a.k));
+#pragma unroll 4
+        for (int c = tid; c < chunks; c += nt) {
+            raw8_floats(raw8_aligned(x, TYPE, 8 * (int64_t)c, true), TYPE, true, v);
+            m = max8_nan(v, m);
+        }
     }
-    m = warp_max_nan(m);
-    if ((tid & 31) == 0) part[tid >> 5] = m;
-    __syncthreads();
-    m = warp_max_nan((tid & 31) < (nt >> 5) ? part[tid & 31] : 0.0f);
     float stored;
-    const RowScale r = row_scale(m, &stored);
+    const RowScale r = row_scale(cta_max_nan(max_nan(m, fabsf(tail)), part), &stored);
     if (CH) {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (tid + i * nt < a.chunks) {
-                raw8_floats(raw[i], a.type, VEC, v);
-                store_q8(q, tid + i * nt, limit, quant8(v, r));
+            if (tid + i * nt < chunks) {
+                raw8_floats(raw[i], TYPE, true, v);
+                *reinterpret_cast<uint2*>(q + 8 * (tid + i * nt)) = quant8(v, r);
             }
     } else {
-        for (int c = tid; c < a.chunks; c += nt) {
-            raw8_floats(raw_x8<VEC>(row, a.type, c, a.k), a.type, VEC, v);
-            store_q8(q, c, limit, quant8(v, r));
+#pragma unroll 2
+        for (int c = tid; c < chunks; c += nt) {
+            raw8_floats(raw8_aligned(x, TYPE, 8 * (int64_t)c, true), TYPE, true, v);
+            *reinterpret_cast<uint2*>(q + 8 * c) = quant8(v, r);
         }
     }
+    if (last < a.limit) q[last] = last < a.k ? quant1(tail, r) : 0;  // limit - 8 chunks < 24 values
     if (tid == 0) a.scale[blockIdx.x] = stored;
 }
 
-// `limit`: columns written (k, or a pitch whose rest is zeros).
+// Rows of any alignment, value by value, read twice (the second time from L1 or L2).
+template <int TYPE>
+__global__ void __launch_bounds__(1024) k_int8_quantize_any(const QuantArgs a) {
+    __shared__ float part[32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, nt = blockDim.x;
+    const void* x = row_at(a.x, TYPE, (int64_t)blockIdx.x * a.ld_x);
+    int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
+    float m = 0.0f;
+#pragma unroll 8
+    for (int i = tid; i < a.k; i += nt) m = max_nan(m, fabsf(ops_load(x, TYPE, i)));
+    float stored;
+    const RowScale r = row_scale(cta_max_nan(m, part), &stored);
+#pragma unroll 4
+    for (int i = tid; i < a.limit; i += nt) q[i] = i < a.k ? quant1(ops_load(x, TYPE, i), r) : 0;
+    if (tid == 0) a.scale[blockIdx.x] = stored;
+}
+
+template <int TYPE>
+void (*quantize_kernel(int ch, bool vec))(QuantArgs) {
+    return !vec      ? k_int8_quantize_any<TYPE>
+           : ch == 0 ? k_int8_quantize<0, TYPE>
+           : ch == 1 ? k_int8_quantize<1, TYPE>
+                     : k_int8_quantize<4, TYPE>;
+}
+
+// `limit`: columns written (k, or a pitch of a multiple of 16 whose rest is zeros).
 cudaError_t launch_int8_quantize(const void* x, int type, int64_t ld_x, int rows, int k, int8_t* q, int64_t ld_q,
                                  int limit, float* scale, cudaStream_t s) {
-    const QuantArgs a{x, q, scale, ld_x, ld_q, type, k, (limit + 7) / 8};
+    const QuantArgs a{x, q, scale, ld_x, ld_q, k, limit};
     const bool vec = ops_vec8(x, type, ld_x);
-    // few rows: as many threads as the row has chunks, for the latency; many: 4 chunks a thread, so
-    // that several rows of an SM overlap their loads and stores
-    const int ch = a.chunks > 4096 ? 0 : a.chunks > 1024 || (rows > 296 && a.chunks > 128) ? 4 : 1;
-    const int threads = ch ? std::max(32, ((a.chunks + ch - 1) / ch + 31) / 32 * 32) : 1024;
-    void (*kernel)(QuantArgs, int) =
-        vec ? (ch == 0 ? k_int8_quantize<0, true> : ch == 1 ? k_int8_quantize<1, true> : k_int8_quantize<4, true>)
-            : (ch == 0 ? k_int8_quantize<0, false> : ch == 1 ? k_int8_quantize<1, false> : k_int8_quantize<4, false>);
-    return ops_launch(kernel, (unsigned)rows, threads, 0, s, a, limit);
+    const int units = (limit + 7) / 8;
+    // few rows: as many threads as the row has chunks, for the latency; many: 4 chunks a thread, so that
+    // several rows of an SM overlap their loads and stores
+    const int ch = units > 4096 ? 0 : units > 1024 || (rows > 296 && units > 128) ? 4 : 1;
+    const int per = vec ? (ch ? ch : 128) : 8;
+    const int threads = std::min(1024, std::max(32, ((units * (vec ? 1 : 8) + per - 1) / per + 31) / 32 * 32));
+    void (*kernel)(QuantArgs) = type == CLB_F32    ? quantize_kernel<CLB_F32>(ch, vec)
+                                : type == CLB_BF16 ? quantize_kernel<CLB_BF16>(ch, vec)
+                                                   : quantize_kernel<CLB_F16>(ch, vec);
+    return ops_launch(kernel, (unsigned)rows, threads, 0, s, a);
 }
 
 struct Int8Args {
@@ -202,10 +251,11 @@ struct Int8Dot {
     Int8Args a;
     const void* x;      // floating x, or null: a.q and a.q_scale are given
     int64_t ld_x;
-    int x_type, rows, segs, kpad;
+    int rows, segs, kpad;
 };
 
-template <int TT, bool VEC>
+// TYPE: of a floating x.
+template <int TT, bool VEC, int TYPE>
 __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     extern __shared__ uint4 dot_smem[];
     __shared__ float part[TT][kDotThreads / 32], scale_s[TT];
@@ -229,23 +279,26 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     };
     if (item < nr * d.segs) fetch(item, item % d.segs * per);
     for (int i = tid; i < d.rows * TT; i += kDotThreads) sums[i] = 0;
-    const int chunks = d.kpad >> 3;
     if (d.x) {
+        // whole chunks, and the columns behind them as single values of the first threads (zeros behind k)
+        const int whole = VEC ? a.k >> 3 : 0, last = 8 * whole + tid;
         float m[TT], v[8];
 #pragma unroll
         for (int t = 0; t < TT; ++t) m[t] = 0.0f;
-        for (int c = tid; c < chunks; c += kDotThreads) {
+        auto source = [&](int t) { return row_at(d.x, TYPE, min(t, a.tokens - 1) * d.ld_x); };
+        for (int c = tid; c < whole; c += kDotThreads) {
             Raw8 raw[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-                raw[t] = raw_x8<VEC>(row_at(d.x, d.x_type, min(t, a.tokens - 1) * d.ld_x), d.x_type, c, a.k);
+            for (int t = 0; t < TT; ++t) raw[t] = raw8_aligned(source(t), TYPE, 8 * (int64_t)c, true);
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-                raw8_floats(raw[t], d.x_type, VEC, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) m[t] = max_nan(m[t], fabsf(v[j]));
+                raw8_floats(raw[t], TYPE, true, v);
+                m[t] = max8_nan(v, m[t]);
             }
         }
+        for (int i = last; i < a.k; i += kDotThreads)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) m[t] = max_nan(m[t], fabsf(ops_load(source(t), TYPE, i)));
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             m[t] = warp_max_nan(m[t]);
@@ -255,10 +308,12 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
         for (int t = 0; t < TT && t < a.tokens; ++t) {
             float stored;
             const RowScale r = row_scale(warp_max_nan(part[t][lane & (kDotThreads / 32 - 1)]), &stored);
-            for (int c = tid; c < chunks; c += kDotThreads) {
-                raw8_floats(raw_x8<VEC>(row_at(d.x, d.x_type, t * d.ld_x), d.x_type, c, a.k), d.x_type, VEC, v);
-                *reinterpret_cast<uint2*>(qs + (size_t)t * d.kpad + 8 * c) = quant8(v, r);
+            int8_t* q = qs + (size_t)t * d.kpad;
+            for (int c = tid; c < whole; c += kDotThreads) {
+                raw8_floats(raw8_aligned(source(t), TYPE, 8 * (int64_t)c, true), TYPE, true, v);
+                *reinterpret_cast<uint2*>(q + 8 * c) = quant8(v, r);
             }
+            for (int i = last; i < d.kpad; i += kDotThreads) q[i] = i < a.k ? quant1(ops_load(source(t), TYPE, i), r) : 0;
             if (tid == 0) scale_s[t] = stored;
         }
     } else {
@@ -312,6 +367,17 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
         ops_store(a.out, a.out_type, t * a.ld_out + n,
                   int8_value(sums[r * TT + t], scale_s[t], a.w_scale[n], a.bias ? a.bias[n] : 0.0f, a.bias != nullptr));
     }
+}
+
+template <int TT, bool VEC>
+void (*dot_kernel(int type))(Int8Dot) {
+    return type == CLB_F32    ? k_int8_dot<TT, VEC, CLB_F32>
+           : type == CLB_BF16 ? k_int8_dot<TT, VEC, CLB_BF16>
+                              : k_int8_dot<TT, VEC, CLB_F16>;
+}
+void (*dot_kernel(int tt, bool vec, int type))(Int8Dot) {
+    return vec ? (tt == 1 ? dot_kernel<1, true>(type) : tt == 2 ? dot_kernel<2, true>(type) : dot_kernel<4, true>(type))
+               : (tt == 1 ? dot_kernel<1, false>(type) : tt == 2 ? dot_kernel<2, false>(type) : dot_kernel<4, false>(type));
 }
 
 // ------------------------------------------------------------------------------
@@ -832,10 +898,12 @@ cudaError_t gm_device(const GmDevice** out) {
                 if ((e = cudaFuncSetAttribute(gm_kernel(mode, type), cudaFuncAttributeMaxDynamicSharedMemorySize, kGmSmem)) !=
                     cudaSuccess)
                     return e;
-        for (auto kernel : {k_int8_dot<1, true>, k_int8_dot<2, true>, k_int8_dot<4, true>, k_int8_dot<1, false>,
-                            k_int8_dot<2, false>, k_int8_dot<4, false>})
-            if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDotSmemMax)) != cudaSuccess)
-                return e;
+        for (int tt : {1, 2, 4})
+            for (bool vec : {false, true})
+                for (int type : {CLB_F32, CLB_BF16, CLB_F16})
+                    if ((e = cudaFuncSetAttribute(dot_kernel(tt, vec, type), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  kDotSmemMax)) != cudaSuccess)
+                        return e;
         for (int size = 2; size <= kGmMaxSplit; ++size)
             if ((e = gm_launch(nullptr, size == 2 ? kPair : kSplit, CLB_F32, 1, size, false, nullptr, &d.clusters[size])) !=
                 cudaSuccess)
@@ -873,7 +941,7 @@ cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, const
 constexpr int kDotTokens = 4;
 
 cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_t ld_x, const GmDevice& dev, cudaStream_t s) {
-    Int8Dot d{a, x, ld_x, x_type, 0, 1, (a.k + 15) & ~15};
+    Int8Dot d{a, x, ld_x, 0, 1, (a.k + 15) & ~15};
     const bool vec = !x || ops_vec8(x, x_type, ld_x);
     const int tt = a.tokens <= 1 ? 1 : a.tokens <= 2 ? 2 : 4;
     d.rows = std::min((a.n + dev.sms - 1) / dev.sms, kDotMaxSums / tt);
@@ -884,8 +952,7 @@ cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_
         const double cost = (double)((d.rows * segs + warps - 1) / warps) / segs + 0.02 * segs;
         if (cost < least) least = cost, d.segs = segs;
     }
-    void (*kernel)(Int8Dot) = vec ? (tt == 1 ? k_int8_dot<1, true> : tt == 2 ? k_int8_dot<2, true> : k_int8_dot<4, true>)
-                                  : (tt == 1 ? k_int8_dot<1, false> : tt == 2 ? k_int8_dot<2, false> : k_int8_dot<4, false>);
+    void (*kernel)(Int8Dot) = dot_kernel(tt, vec, x ? x_type : CLB_F32);
     const size_t smem = (size_t)tt * d.kpad + (size_t)d.rows * tt * 4;
     return ops_launch(kernel, (unsigned)((a.n + d.rows - 1) / d.rows), kDotThreads, smem, s, d);
 }
