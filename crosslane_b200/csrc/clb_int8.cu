@@ -239,10 +239,10 @@ __device__ __forceinline__ float int8_value(int acc, float xs, float ws, float b
 // Few tokens (TT >= tokens): row dots. Bound by the weights' bytes, so there is one launch
 // and the first weights are in flight before the tokens are quantised: every CTA does that
 // by itself into shared memory (x comes from L2; floating x) or copies q (int8 x). A CTA has
-// `rows` weight rows, cut into `segs` pieces of K that its warps share out; a piece's sums
+// `rows` weight rows, cut into 2^log_segs pieces of K that its warps share out; a piece's sums
 // are integers, added in shared memory in any order.
-constexpr int kDotThreads = 512;
-constexpr int kDotAhead = 4;                 // 16-byte weight pieces a lane has in flight
+constexpr int kDotThreads = 1024;
+constexpr int kDotAhead = 4;                 // 16-byte weight pieces of a lane's group, two groups in flight
 constexpr int kDotSmem = 160 * 1024;         // largest tokens * pitch that is staged
 constexpr int kDotMaxSums = 8192;            // rows * tokens of a CTA
 constexpr int kDotSmemMax = kDotSmem + 4 * kDotMaxSums;
@@ -251,7 +251,7 @@ struct Int8Dot {
     Int8Args a;
     const void* x;      // floating x, or null: a.q and a.q_scale are given
     int64_t ld_x;
-    int rows, segs, kpad;
+    int rows, log_segs, kpad;
 };
 
 // TYPE: of a floating x.
@@ -264,20 +264,35 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     int* sums = reinterpret_cast<int*>(qs + (size_t)TT * d.kpad);   // [rows][TT]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r0 = blockIdx.x * d.rows, nr = min(d.rows, a.n - r0);
-    const int pieces = a.k >> 4, per = (pieces + d.segs - 1) / d.segs;
-    // the warp's first piece of weights
-    int item = warp;
-    int4 w[kDotAhead];
-    auto fetch = [&](int it, int at) {
-        const int8_t* row = a.w + (int64_t)(r0 + it / d.segs) * a.ld_w;
-        const int end = min(pieces, (it % d.segs + 1) * per);
+    const int pieces = a.k >> 4, per = (pieces + (1 << d.log_segs) - 1) >> d.log_segs;
+    // A warp's share: items (a row's piece of K) warp, warp + 32, ..., each in groups of 32 * kDotAhead
+    // weight pieces. The next group is asked for before one is multiplied, the first before the
+    // tokens are quantised.
+    struct Place {
+        int item, at, end;
+        const int4* row;
+    };
+    const int items = nr << d.log_segs;
+    auto start = [&](int item) {
+        const int seg = item & ((1 << d.log_segs) - 1);
+        return Place{item, seg * per, item < items ? min(pieces, (seg + 1) * per) : 0,
+                     reinterpret_cast<const int4*>(a.w + (int64_t)(r0 + (item >> d.log_segs)) * a.ld_w)};
+    };
+    auto advance = [&](Place p) {
+        p.at += 32 * kDotAhead;
+        return p.at < p.end ? p : start(p.item + kDotThreads / 32);
+    };
+    auto fetch = [&](int4 (&w)[kDotAhead], const Place& p) {
 #pragma unroll
         for (int u = 0; u < kDotAhead; ++u) {
-            const int p = at + lane + 32 * u;
-            w[u] = p < end ? __ldg(reinterpret_cast<const int4*>(row) + p) : make_int4(0, 0, 0, 0);
+            const int i = p.at + lane + 32 * u;
+            w[u] = make_int4(0, 0, 0, 0);
+            if (i < p.end) w[u] = __ldg(p.row + i);
         }
     };
-    if (item < nr * d.segs) fetch(item, item % d.segs * per);
+    Place here = start(warp);
+    int4 next[kDotAhead];
+    fetch(next, here);
     for (int i = tid; i < d.rows * TT; i += kDotThreads) sums[i] = 0;
     if (d.x) {
         // whole chunks, and the columns behind them as single values of the first threads (zeros behind k)
@@ -325,41 +340,47 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
         }
     }
     __syncthreads();
-    for (; item < nr * d.segs; item += kDotThreads / 32) {
-        const int seg = item % d.segs, end = min(pieces, (seg + 1) * per);
-        int acc[TT];
+    int acc[TT];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) acc[t] = 0;
-        for (int at = seg * per; at < end; at += 32 * kDotAhead) {
-            if (at > seg * per || item != warp) fetch(item, at);
+    for (int t = 0; t < TT; ++t) acc[t] = 0;
+    while (here.item < items) {
+        int4 w[kDotAhead];
 #pragma unroll
-            for (int u = 0; u < kDotAhead; ++u) {
-                const int p = min(at + lane + 32 * u, pieces - 1);  // weights behind the end are zero
+        for (int u = 0; u < kDotAhead; ++u) w[u] = next[u];
+        const Place then = advance(here);
+        fetch(next, then);
 #pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const int4 v = reinterpret_cast<const int4*>(qs + (size_t)t * d.kpad)[p];
-                    acc[t] = __dp4a(w[u].x, v.x, __dp4a(w[u].y, v.y, __dp4a(w[u].z, v.z, __dp4a(w[u].w, v.w, acc[t]))));
+        for (int u = 0; u < kDotAhead; ++u) {
+            if (here.at + 32 * u >= here.end) break;
+            const int p = min(here.at + lane + 32 * u, pieces - 1);  // weights behind the end are zero
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const int4 v = reinterpret_cast<const int4*>(qs + (size_t)t * d.kpad)[p];
+                acc[t] = __dp4a(w[u].x, v.x, __dp4a(w[u].y, v.y, __dp4a(w[u].z, v.z, __dp4a(w[u].w, v.w, acc[t]))));
+            }
+        }
+        if (then.item != here.item) {
+            const int row = here.item >> d.log_segs;
+            if ((~here.item & ((1 << d.log_segs) - 1)) == 0) {  // the columns behind the last whole piece
+                const int i = 16 * pieces + lane;
+                if (i < a.k) {
+                    const int wv = a.w[(int64_t)(r0 + row) * a.ld_w + i];
+#pragma unroll
+                    for (int t = 0; t < TT; ++t)
+                        if (t < a.tokens) acc[t] += wv * qs[(size_t)t * d.kpad + i];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+                acc[t] = 0;
+                if (lane == 0) {
+                    if (d.log_segs == 0) sums[row * TT + t] = sum;
+                    else atomicAdd(&sums[row * TT + t], sum);
                 }
             }
         }
-        const int row = item / d.segs;
-        if (seg == d.segs - 1) {  // the columns behind the last whole piece
-            const int i = 16 * pieces + lane;
-            if (i < a.k) {
-                const int wv = a.w[(int64_t)(r0 + row) * a.ld_w + i];
-#pragma unroll
-                for (int t = 0; t < TT; ++t)
-                    if (t < a.tokens) acc[t] += wv * qs[(size_t)t * d.kpad + i];
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
-            if (lane == 0) {
-                if (d.segs == 1) sums[row * TT + t] = sum;
-                else atomicAdd(&sums[row * TT + t], sum);
-            }
-        }
+        here = then;
     }
     __syncthreads();
     for (int i = tid; i < nr * a.tokens; i += kDotThreads) {
@@ -630,6 +651,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     // SPLIT: [source][token of this CTA's share][128 rows] behind the stages
     const int share = SPLIT ? (g.nt + g.split - 1) / g.split : 0;
     const uint32_t red = base + (uint32_t)g.stages * stage_bytes;
+    float split_ws = 0.0f, split_bias = -0.0f;  // for the sums that this CTA will add up
 
     if (warp == kGmLoadWarp) {
         if (lane == 0) {
@@ -687,7 +709,15 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
         const int half = (g.nt / 16 + 1) / 2 * 16, c0 = warp < 4 ? 0 : half, c1 = warp < 4 ? half : g.nt;
         const uint32_t lead_empty = PAIR ? cluster_addr(acc_empty(0), 0) : 0u;
         bool ok = true;
-        if (SPLIT) cluster_wait();
+        if (SPLIT) {
+            const int row = row_of(first) + (tid & 127), t = token_of(first) + rank * share + tid;
+            if (row < g.n) {
+                split_ws = g.w_scale[row];
+                if (g.bias) split_bias = g.bias[row];
+            }
+            if (tid < share) xs_s[0][tid] = t < g.tokens ? g.q_scale[t] : 0.0f;
+            cluster_wait();
+        }
         for (int i = 0; i < my_tiles; ++i) {  // to the end after a failed wait too: the warps meet at a barrier
             const int acc = i & 1, tile = first + i * step;
             const int row = row_of(tile) + (tid & 127), t0 = token_of(tile);
@@ -756,7 +786,6 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
         const int t0 = token_of(first) + rank * share, row = row_of(first) + (tid & 127);
         const int nc = min(share, min(g.nt - rank * share, g.tokens - t0));
         if (warp < kGmEpiWarps && row < g.n && !*abort_flag) {
-            const float ws = g.w_scale[row], bias = g.bias ? g.bias[row] : -0.0f;
             for (int c = tid >> 7; c < nc; c += 2) {
                 int v[kGmMaxSplit], sum = 0;
 #pragma unroll
@@ -769,7 +798,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
                 }
 #pragma unroll
                 for (int p = 0; p < kGmMaxSplit; ++p) sum += v[p];
-                ops_store(g.out, OUT, (int64_t)(t0 + c) * g.ld_out + row, int8_value(sum, g.q_scale[t0 + c], ws, bias, true));
+                ops_store(g.out, OUT, (int64_t)(t0 + c) * g.ld_out + row, int8_value(sum, xs_s[0][c], split_ws, split_bias, true));
             }
         }
     }
@@ -941,16 +970,17 @@ cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, const
 constexpr int kDotTokens = 4;
 
 cudaError_t launch_int8_dot(const Int8Args& a, const void* x, int x_type, int64_t ld_x, const GmDevice& dev, cudaStream_t s) {
-    Int8Dot d{a, x, ld_x, 0, 1, (a.k + 15) & ~15};
+    Int8Dot d{a, x, ld_x, 0, 0, (a.k + 15) & ~15};
     const bool vec = !x || ops_vec8(x, x_type, ld_x);
     const int tt = a.tokens <= 1 ? 1 : a.tokens <= 2 ? 2 : 4;
     d.rows = std::min((a.n + dev.sms - 1) / dev.sms, kDotMaxSums / tt);
-    // cut the rows so that the warps' shares are even: a round is kDotThreads / 32 items
-    constexpr int warps = kDotThreads / 32;
+    // cut the rows so that the warps' shares are even; an item costs its groups and as much as half a
+    // group for its sums
     double least = 1e300;
-    for (int segs = 1; segs <= 16 && a.k / segs >= 512; segs *= 2) {
-        const double cost = (double)((d.rows * segs + warps - 1) / warps) / segs + 0.02 * segs;
-        if (cost < least) least = cost, d.segs = segs;
+    for (int log = 0; log <= 5 && (d.kpad >> log) >= 512; ++log) {
+        const int per = ((a.k >> 4) + (1 << log) - 1) >> log, groups = (per + 32 * kDotAhead - 1) / (32 * kDotAhead);
+        const double cost = (double)(((d.rows << log) + kDotThreads / 32 - 1) / (kDotThreads / 32)) * (groups + 0.5);
+        if (cost < least) least = cost, d.log_segs = log;
     }
     void (*kernel)(Int8Dot) = dot_kernel(tt, vec, x ? x_type : CLB_F32);
     const size_t smem = (size_t)tt * d.kpad + (size_t)d.rows * tt * 4;
