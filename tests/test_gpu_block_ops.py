@@ -192,6 +192,79 @@ def test_route_flags_bad_rows_alone(cb, cuda, with_bias):
         assert int(status) == 1 and bool(torch.isnan(w).all()) and bool((ids == torch.arange(k, device="cuda")).all())
 
 
+def close_bias(kind, l, chosen, rng, target=0.9):
+    """A bias that puts the ranks of `chosen` within a few ulps of one another, above the others'."""
+    held = scores64(kind, l.astype(np.float64)).astype(np.float32)
+    bias = (rng.standard_normal(l.size) * 0.01 - 3.0).astype(np.float32)
+    top = np.float32(target + held.max())
+    bias[chosen] = top - held[chosen]
+    bias[chosen] += (rng.integers(-2, 3, len(chosen)) * np.spacing(top)).astype(np.float32)
+    return bias
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+@pytest.mark.parametrize("E,k,near", [(384, 6, 10), (384, 8, 31), (384, 8, 384), (64, 16, 64), (256, 8, 60), (1000, 1, 2)])
+def test_route_ranks_an_ulp_apart(cb, cuda, kind, E, k, near):
+    """Ranks closer than fp32 scores can tell: a few candidates, and more than a warp has lanes."""
+    torch = cuda
+    for seed in range(6):
+        rng = np.random.default_rng(seed * 1000 + E + near)
+        l = (rng.standard_normal((3, E)) * 2).astype(np.float32)
+        bias = close_bias(kind, l[0], rng.permutation(E)[:near], rng)
+        logits, b = torch.from_numpy(l).cuda(), torch.from_numpy(bias).cuda()
+        ids, w = torch.empty((3, k), dtype=torch.int32, device="cuda"), torch.empty((3, k), device="cuda")
+        op = cb.ExpertRoute(E, k, score=kind)
+        op.run(logits, ids, w, d_bias=b)
+        check_route(torch, op, logits, b, ids, w, kind)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("E,k,groups,top", [(384, 8, 8, 4), (96, 4, 32, 7), (352, 8, 11, 3)])
+def test_route_groups_an_ulp_apart(cb, cuda, kind, with_bias, E, k, groups, top):
+    torch = cuda
+    per = E // groups
+    for seed in range(6):
+        rng = np.random.default_rng(seed * 77 + E)
+        l = (rng.standard_normal((3, E)) * 2).astype(np.float32)
+        bias = None
+        first = np.concatenate([g * per + rng.permutation(per)[:2] for g in range(groups)])
+        if with_bias:
+            bias = close_bias(kind, l[0], first, rng)
+        else:  # the same two logits on top of every group, an ulp apart here and there
+            l[0] = np.minimum(l[0], 1.0)
+            l[0][first] = np.tile(np.array([2.5, 2.0], np.float32), groups)
+            l[0][first] += (rng.integers(-1, 2, 2 * groups) * np.spacing(np.float32(2.5))).astype(np.float32)
+        logits = torch.from_numpy(l).cuda()
+        b = None if bias is None else torch.from_numpy(bias).cuda()
+        ids, w = torch.empty((3, k), dtype=torch.int32, device="cuda"), torch.empty((3, k), device="cuda")
+        op = cb.ExpertRoute(E, k, score=kind, n_groups=groups, top_groups=top)
+        op.run(logits, ids, w, d_bias=b)
+        check_route(torch, op, logits, b, ids, w, kind, groups, top, True)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+def test_route_huge_and_tiny_logits(cb, cuda, kind):
+    torch = cuda
+    E, k = 64, 8
+    big = torch.finfo(torch.float32).max
+    l = torch.zeros((6, E), device="cuda")
+    l[0] = torch.linspace(-1, 1, E, device="cuda") * big   # differences that pass fp32
+    l[1] = -big
+    l[1, 7] = big
+    l[2] = 1e-42
+    l[2, 9] = -1e-42
+    l[3] = torch.linspace(-300, 300, E, device="cuda")
+    l[4] = -200.0
+    l[4, ::2] = -201.0
+    l[5] = big
+    for bias in (None, torch.linspace(0.1, -0.1, E, device="cuda")):
+        ids, w = torch.empty((6, k), dtype=torch.int32, device="cuda"), torch.empty((6, k), device="cuda")
+        op = cb.ExpertRoute(E, k, score=kind, renormalize=False)
+        op.run(l, ids, w, d_bias=bias)
+        check_route(torch, op, l, bias, ids, w, kind, renorm=False)
+
+
 def test_route_agrees_with_the_modes_there_were(cb, cuda):
     """Sigmoid without a bias is mode 0's choice; sqrt-softplus with a bias is mode 1's."""
     torch = cuda
@@ -310,6 +383,44 @@ def test_norm_parts(cb, cuda, gate, sig, post, pre, D):
 @pytest.mark.parametrize("h_t", ["float32", "bfloat16"])
 def test_norm_pitches(cb, cuda, pad, h_t):
     run_norm(cb, cuda, 33, 1024, h_t, "float16", "bfloat16", gate="full", pad=pad)
+
+
+@pytest.mark.parametrize("T,D", [(3, 1024), (400, 1024), (400, 1025)])
+@pytest.mark.parametrize("h_t,y_t", [("float32", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16")])
+def test_norm_rows_that_start_anywhere(cb, cuda, T, D, h_t, y_t):
+    """Tensors whose first element is one past an aligned address."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    dt = lambda n: getattr(torch, n)  # noqa: E731
+    at = lambda t, n: torch.randn((T, D + 9), generator=gen, device="cuda").to(dt(t))[:, n:n + D]  # noqa: E731
+    h, y, g, out, x = at(h_t, 1), at(y_t, 3), at(y_t, 0), at(h_t, 8), at(y_t, 5)
+    wide = torch.randn(D + 1, generator=gen, device="cuda")
+    w_post, w_pre = wide[1:], wide[:D]
+    cb.BlockNorm(D, eps=1e-5, gate="full").run(h, d_y=y, d_gate=g, d_w_post=w_post, d_w_pre=w_pre, d_h_out=out, d_x=x)
+    n64 = lambda t: t.double().cpu().numpy()  # noqa: E731
+    new, xw, rh, bz = norm64(n64(h), n64(y), n64(g), n64(w_post), n64(w_pre), True, "full", False, 1.0, 1.0, 1e-5)
+    check_norm(torch, n64(out), new, (rh, bz), D, h_t)
+    check_norm(torch, n64(x), xw, (rh, bz), D, y_t, (np.abs(xw) / np.maximum(np.abs(new), 1e-300), new))
+
+
+def test_norm_past_32_bits(cb, cuda):
+    """Rows whose offsets in elements and bytes pass 2^32 (bf16, 131073 rows, 32768 apart)."""
+    torch = cuda
+    T, D, pitch = 131073, 64, 32768
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of free memory")
+    h = torch.empty((T, pitch), dtype=torch.bfloat16, device="cuda")
+    x = torch.empty((T, pitch), dtype=torch.bfloat16, device="cuda")
+    h[:, :D] = torch.randn((T, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    cb.BlockNorm(D, post=False).run(h[:, :D], d_x=x[:, :D])
+    few = torch.empty((64, D), dtype=torch.bfloat16, device="cuda")
+    cb.BlockNorm(D, post=False).run(h[-64:, :D].contiguous(), d_x=few)
+    # another kernel for few rows: each within one rounding of the exact value
+    assert torch.allclose(x[-64:, :D].float(), few.float(), rtol=2.0 ** -7, atol=0)
+    logits = h[:, :D]
+    ids, w = torch.empty((T, 4), dtype=torch.int32, device="cuda"), torch.empty((T, 4), device="cuda")
+    cb.ExpertRoute(D, 4).run(logits, ids, w)
+    assert torch.equal(ids[-64:].long(), torch.sort(logits[-64:].float(), dim=1, descending=True, stable=True).indices[:, :4])
 
 
 def test_norm_without_weights_or_block(cb, cuda):
@@ -492,6 +603,76 @@ def test_linear_int8_input(cb, cuda, T, K, extra):
 @pytest.mark.parametrize("T", [1, 2, 30, 300])
 def test_linear_nan_row_stays_alone(cb, cuda, T):
     linear_case(cb, cuda, T, 256, 200, bad_row=T // 2)
+
+
+@pytest.mark.parametrize("T", [1, 3, 20, 300])
+def test_linear_outputs_that_start_anywhere(cb, cuda, T):
+    """16-bit outputs at odd elements and odd pitches, floating x one past an aligned address."""
+    torch = cuda
+    K, N = 264, 130
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    w = padded_int8(torch, N, K)
+    w.copy_(torch.randint(-127, 128, (N, K), generator=gen, device="cuda").to(torch.int8))
+    op = cb.Int8Linear(w, torch.rand(N, generator=gen, device="cuda"))
+    x = torch.randn((T, K + 3), generator=gen, device="cuda").to(torch.float16)
+    ws = torch.empty(op.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+    want = torch.empty((T, N), dtype=torch.bfloat16, device="cuda")
+    op.run(x[:, 1:1 + K].contiguous(), want, d_ws=ws)
+    for pad, off in ((1, 0), (1, 1), (6, 1), (6, 2), (2, 0)):
+        back = torch.full((T + 1, N + pad), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = back[:T, off:off + N]
+        op.run(x[:, 1:1 + K], out, d_ws=ws)
+        assert torch.equal(out, want), (pad, off)
+        mask = torch.ones_like(back, dtype=torch.bool)
+        mask[:T, off:off + N] = False
+        assert bool((back[mask] == 7).all()), (pad, off)
+
+
+def test_linear_past_32_bits(cb, cuda):
+    """Weights whose offsets pass 2^31 bytes, outputs whose offsets pass 2^31 elements."""
+    torch = cuda
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free memory")
+    K, N = 16384, 135000
+    w = torch.empty((N, K), dtype=torch.int8, device="cuda")
+    w.random_(-127, 128, generator=torch.Generator(device="cuda").manual_seed(1))
+    op = cb.Int8Linear(w, torch.full((N,), 0.5, device="cuda"))
+    for T in (1, 5, 40):
+        q = torch.randint(-127, 128, (T, K), device="cuda").to(torch.int8)
+        out = torch.empty((T, N), device="cuda")
+        op.run(q, out, d_x_scale=torch.ones(T, device="cuda"))
+        want = (q.double() @ w[-200:].double().t() * 0.5).float()
+        assert torch.equal(out[:, -200:], want), T  # exact: sums below 2^24 or rounded once
+    T, n = 16200, 135000
+    small = cb.Int8Linear(torch.ones((n, 16), dtype=torch.int8, device="cuda"), torch.ones(n, device="cuda"))
+    out = torch.empty((T, n), dtype=torch.bfloat16, device="cuda")
+    q = torch.ones((T, 16), dtype=torch.int8, device="cuda")
+    q[-1] = 2
+    small.run(q, out, d_x_scale=torch.ones(T, device="cuda"))
+    assert bool((out[-1] == 32).all()) and bool((out[-2] == 16).all()) and bool((out[:, -1][:-1] == 16).all())
+
+
+def test_calls_on_two_streams_at_once(cb, cuda):
+    """Calls that overlap, with a workspace each, give the bits of calls one after the other."""
+    torch = cuda
+    K, N = 4096, 1024
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randint(-127, 128, (N, K), generator=gen, device="cuda").to(torch.int8)
+    op = cb.Int8Linear(w, torch.rand(N, generator=gen, device="cuda"))
+    jobs = []
+    for i, T in enumerate((3, 40, 40, 700, 700, 64)):
+        x = torch.randn((T, K), generator=gen, device="cuda")
+        jobs.append((x, torch.empty((T, N), device="cuda"), torch.empty((T, N), device="cuda"),
+                     torch.empty(op.workspace_bytes(T), dtype=torch.uint8, device="cuda"), torch.cuda.Stream()))
+    for x, alone, _, ws, _ in jobs:
+        op.run(x, alone, d_ws=ws)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, _, out, ws, stream in jobs:
+            op.run(x, out, d_ws=ws, stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for _, alone, out, _, _ in jobs:
+        assert torch.equal(alone, out)
 
 
 def test_linear_extreme_sums(cb, cuda):
