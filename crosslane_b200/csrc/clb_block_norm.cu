@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
     const int x_type = SET ? norm_types(SET).other : a.x_type;
     __shared__ float part[2][32];
+    ops_begin();
     const int64_t row = blockIdx.x;
     const bool wide_gate = a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL;
     Raw8 yr[CH], hr[CH], gr[CH];
@@ -179,6 +180,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArg
     extern __shared__ __align__(16) uint8_t row_smem[];
     __shared__ float part[4][32];
     __shared__ uint64_t bars[kRowStages];
+    ops_begin();
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
     const int x_type = SET ? norm_types(SET).other : a.x_type, g_type = SET ? norm_types(SET).other : a.gate_type;
     const int tid = threadIdx.x, nt = blockDim.x, units = a.dim >> 3;

@@ -136,7 +136,7 @@ __device__ __forceinline__ float max8_nan(const float (&v)[8], float m) {
 template <int CH, int TYPE>
 __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
     __shared__ float part[32];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    ops_begin();
     const int tid = threadIdx.x, nt = blockDim.x, chunks = a.k >> 3, last = 8 * chunks + tid;
     const void* x = row_at(a.x, TYPE, (int64_t)blockIdx.x * a.ld_x);
     int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
 template <int TYPE>
 __global__ void __launch_bounds__(1024) k_int8_quantize_any(const QuantArgs a) {
     __shared__ float part[32];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    ops_begin();
     const int tid = threadIdx.x, nt = blockDim.x;
     const void* x = row_at(a.x, TYPE, (int64_t)blockIdx.x * a.ld_x);
     int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
@@ -259,6 +259,7 @@ template <int TT, bool VEC, int TYPE>
 __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     extern __shared__ uint4 dot_smem[];
     __shared__ float part[TT][kDotThreads / 32], scale_s[TT];
+    ops_begin();
     const Int8Args& a = d.a;
     int8_t* qs = reinterpret_cast<int8_t*>(dot_smem);               // [TT][kpad]
     int* sums = reinterpret_cast<int*>(qs + (size_t)TT * d.kpad);   // [rows][TT]
@@ -630,8 +631,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
         cluster_arrive();
         cluster_wait();
     }
-    // weights do not depend on the quantising kernel in front: their first loads go out before
-    // that kernel has finished, the tokens' after
+    // weights do not depend on the quantising kernel in front, and what is in front of that is
+    // complete (ops_begin): their first loads go out before that kernel has finished, the tokens' after
     const int ahead = (int)min((int64_t)g.stages, total);
     const uint32_t lead = PAIR ? cluster_addr(full(0), 0) : full(0);  // the stages' full barriers
     if (tid == 32 * kGmLoadWarp) {
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
 
     if (warp == kGmLoadWarp) {
         if (lane == 0) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");
+            ops_wait();
             // the place of a tile is found once a tile: the divisions in front of every copy would cost
             // more than the block's products
             int stage = 0, left = ahead;
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
             }
         }
     } else {
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // q_scale
+        ops_begin();  // q_scale
         const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const int half = (g.nt / 16 + 1) / 2 * 16, c0 = warp < 4 ? 0 : half, c1 = warp < 4 ? half : g.nt;
         const uint32_t lead_empty = PAIR ? cluster_addr(acc_empty(0), 0) : 0u;

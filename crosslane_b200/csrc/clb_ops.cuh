@@ -152,15 +152,31 @@ cudaError_t ops_device(int* sms, Setup setup) {
 }
 
 // Launch through cudaLaunchKernelEx, whose own status is the launch's (cudaGetLastError would
-// also hand over, and clear, an earlier error of the caller's).
+// also hand over, and clear, an earlier error of the caller's). The kernel's CTAs may be set
+// up while the kernel in front of it on the stream ends: it starts with ops_wait.
 template <class... P, class... A>
 cudaError_t ops_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t c{};
     c.gridDim = grid;
     c.blockDim = dim3((unsigned)threads);
     c.dynamicSmemBytes = smem;
     c.stream = s;
+    c.attrs = &attr;
+    c.numAttrs = 1;
     return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+
+// The first thing every thread of such a kernel does: waits until all work in front of it on the
+// stream has completed and is visible.
+__device__ __forceinline__ void ops_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The same, and lets the kernel behind it be set up under this one. In this order a kernel that runs
+// ahead of its own wait knows that all but the one in front is complete.
+__device__ __forceinline__ void ops_begin() {
+    ops_wait();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 }  // namespace clb

@@ -8,6 +8,7 @@
 // error; if the picks (and the groups) are further apart than that error they are the same
 // as with exact scores, else (about one row in a thousand with continuous logits) the experts
 // in question are ranked in double.
+#include <cfloat>
 #include <cmath>
 
 #include "clb_ops.cuh"
@@ -30,14 +31,14 @@ struct RouteArgs {
     int* status;
     int64_t ld;
     int tokens, type, E, k, groups, top_groups, pair, renorm;
-    int lanes_per_group;  // power of two, groups * lanes_per_group <= 32
+    int per, log_lanes;  // experts of a group; 2^log_lanes lanes work on one, groups << log_lanes <= 32
     float scale, per_inv;  // per_inv: groups / E
 };
 
-// Order-preserving map of a float to unsigned (-0 as +0); 0 is below every key.
+// Order-preserving map of a float to unsigned (-0 as +0).
 __device__ __forceinline__ uint32_t rank_key(float v) {
     const uint32_t u = __float_as_uint(__fadd_rn(v, 0.0f));
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
@@ -51,8 +52,10 @@ __device__ __forceinline__ float exp_diff(float l, float top) {
 }
 // A score in fp32. Error: expf and log1pf are within 2 ulp (4 half ulps each), __fdividef
 // within 2 ulp, the additions and the root half an ulp, so sigmoid and sqrt(softplus) are
-// within 9 half ulps; softmax divides by a sum of E terms whose chains are at most 37
-// additions long: within 6 + 6 + 37 + 4 half ulps.
+// within 9 half ulps. Softmax divides by a sum of E terms exp(l - top). A term's exponent d is
+// off by |d| half ulps, __expf by 4 + 2.4 |d|; weighted by the terms themselves the mean of |d|
+// is at most ln E <= 7, and the chains are at most 37 additions long: the sum is within 4 + 3.4 *
+// 7 + 37 = 65 half ulps, the score within 6 + 65 + 4 = 75.
 template <int KIND>
 __device__ __forceinline__ float score_f32(float l, float top, float sum) {
     if (KIND == CLB_SCORE_SIGMOID) return __fdividef(1.0f, 1.0f + expf(-l));
@@ -71,13 +74,20 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// One warp per token, expert e = 32 i + lane in the lane's i-th register. SCORED: the ranks or the
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// One warp per token, expert e = 32 i + lane in the lane's i-th register (-inf behind the last). SCORED: the ranks or the
 // groups' values need scores. Bound by latency and instructions (a token's 1.5 KB of logits
 // are read once).
 template <int NPL, int KIND, bool SCORED>
 __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 5 : 3) k_route_experts(const RouteArgs a) {
-    __shared__ uint4 cand_s[kRouteWarps][32];                                      // key, id, logit, bias
+    __shared__ unsigned long long cand_s[kRouteWarps][32];                         // key, ~id
     __shared__ float vals_s[SCORED ? kRouteWarps : 1][SCORED ? NPL * 32 : 1];  // scores, then with their bias
+    ops_wait();  // without letting the next kernel in early: its CTAs in this one's free slots made 2048 tokens 9.4 us, not 7.8
     const unsigned all = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * kRouteWarps + warp;
@@ -114,14 +124,10 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
             for (int i = 0; i < NPL; ++i) l[i] = __half2float(__ushort_as_half((uint16_t)raw[i]));
         }
     }
-    bool fine = true;
-    float top = -INFINITY;
+    float top = l[0], most = b[0];
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-        fine = fine && l[i] < INFINITY && b[i] < INFINITY;
-        top = fmaxf(top, l[i]);
-    }
-    if (!__all_sync(all, fine)) {
+    for (int i = 1; i < NPL; ++i) top = max_nan(top, l[i]), most = max_nan(most, b[i]);
+    if (!__all_sync(all, top < INFINITY && most < INFINITY)) {
         if (lane == 0 && a.status) atomicExch(a.status, 1);
         if (lane < a.k) {
             ids[lane] = lane;
@@ -129,18 +135,20 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         }
         return;
     }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+        if (32 * i + lane >= a.E) l[i] = -INFINITY;
     float sum = 1.0f;
-    if (KIND == CLB_SCORE_SOFTMAX || SCORED) top = warp_max(top);
+    if (KIND == CLB_SCORE_SOFTMAX || SCORED) top = fmaxf(warp_max(top), -FLT_MAX);
     if (KIND == CLB_SCORE_SOFTMAX) {
         sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NPL; ++i)
-            if (32 * i + lane < a.E && l[i] > -INFINITY) sum += exp_diff(l[i], top);
+        for (int i = 0; i < NPL; ++i) sum += __expf(l[i] - top);
         sum = ops_warp_sum(sum);
     }
     // the largest error of a score (s rises with l), and of the scores below the normal numbers
     const float off = !SCORED ? 0.0f
-                              : fmaf(KIND == CLB_SCORE_SOFTMAX ? 64.0f * kHalfUlp : 16.0f * kHalfUlp,
+                              : fmaf(KIND == CLB_SCORE_SOFTMAX ? 96.0f * kHalfUlp : 16.0f * kHalfUlp,
                                      KIND == CLB_SCORE_SQRT_SOFTPLUS ? score_f32<KIND>(top, 0.0f, 1.0f) : 1.0f, 1e-18f);
 
     uint32_t mine = 0;      // lane j: the key and id of the j-th largest rank
@@ -180,91 +188,96 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
                 v = !there ? -INFINITY : a.bias ? sc : l[i];
                 if (a.groups > 1) vals_s[warp][e] = there ? sc : -INFINITY;
             }
-            key[i] = e < a.E ? rank_key(v) : 0u;
+            key[i] = rank_key(v);
         }
         bool unsure = false;
         if (a.groups > 1) {
-            // lanes_per_group lanes find the two best of a group
-            const int per = a.E / a.groups, L = a.lanes_per_group, g = lane / L;
+            // 2^log_lanes lanes find the two best of a group
+            const int L = 1 << a.log_lanes, g = lane >> a.log_lanes;
+            const bool mine_too = g < a.groups;
             float v1 = -INFINITY, v2 = -INFINITY;
             __syncwarp();
-            if (g < a.groups)
-                for (int i = lane % L; i < per; i += L) {
-                    const float v = SCORED ? vals_s[warp][g * per + i] : ops_load(a.logits, a.type, row + g * per + i);
+            if (mine_too) {
+#pragma unroll 4
+                for (int i = lane & (L - 1); i < a.per; i += L) {
+                    const float v = SCORED ? vals_s[warp][g * a.per + i] : ops_load(a.logits, a.type, row + g * a.per + i);
                     v2 = fmaxf(v2, fminf(v1, v));
                     v1 = fmaxf(v1, v);
                 }
+            }
             __syncwarp();
             for (int o = 1; o < L; o <<= 1) {
                 const float o1 = __shfl_xor_sync(all, v1, o), o2 = __shfl_xor_sync(all, v2, o);
                 v2 = fmaxf(fmaxf(v2, o2), fminf(v1, o1));
                 v1 = fmaxf(v1, o1);
             }
-            const float value = a.pair && v2 > -INFINITY ? __fadd_rn(v1, v2) : v1;
-            uint32_t gkey = g < a.groups && lane % L == 0 ? rank_key(value) : 0u;
-            uint32_t kept = 0, last = 0;
-            for (int i = 0; i < a.top_groups; ++i) {
-                last = __reduce_max_sync(all, gkey);
-                const int at = __ffs(__ballot_sync(all, gkey == last)) - 1;
-                kept |= 1u << (at / L);
-                if (lane == at) gkey = 0;
+            // a group's place is the number of groups in front of it
+            const uint32_t gkey = rank_key(a.pair && v2 > -INFINITY ? __fadd_rn(v1, v2) : v1);
+            int place = 0;
+#pragma unroll 8
+            for (int j = 0; j < a.groups; ++j) {
+                const uint32_t other = __shfl_sync(all, gkey, j << a.log_lanes);
+                place += other > gkey || (other == gkey && j < g);
             }
+            const bool keep = mine_too && place < a.top_groups;
+            const unsigned kept = __ballot_sync(all, keep);
             if (SCORED && !exact && a.top_groups < a.groups) {
                 // a value's error: of two scores, of their ranks' roundings and of the sum's
-                const uint32_t next = __reduce_max_sync(all, gkey);
+                const uint32_t last = __reduce_min_sync(all, keep ? gkey : 0xffffffffu);
+                const uint32_t next = __reduce_max_sync(all, mine_too && !keep ? gkey : 0u);
                 const float lo = key_value(last), hi = key_value(next);
                 unsure = next != kKeyNegInf && !(lo - hi > 4.0f * (off + 2.0f * kHalfUlp * (fabsf(lo) + fabsf(hi))));
             }
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
-                const int e = 32 * i + lane, ge = (int)(((float)e + 0.5f) * a.per_inv);
-                if (e < a.E && !((kept >> ge) & 1u)) key[i] = kKeyNegInf;
+                const int e = 32 * i + lane, ge = min((int)(((float)e + 0.5f) * a.per_inv), a.groups - 1);
+                if (!((kept >> (ge << a.log_lanes)) & 1u)) key[i] = kKeyNegInf;
             }
         }
         // The k + 1 largest keys. The (k + 1)-th largest of the lanes' maxima is a lower bound of
         // them: the few keys from there on are collected, one to a lane, and ranked by counting.
         const int want = min(a.k + 1, a.E);
-        uint32_t cur = 0;
+        uint32_t cur = key[0];
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) cur = max(cur, key[i]);
+        for (int i = 1; i < NPL; ++i) cur = max(cur, key[i]);
         uint32_t bound = 0;
         for (int i = 0; i < want; ++i) {
             bound = __reduce_max_sync(all, cur);
             if (cur == bound) cur = 0;
         }
-        // the keys from `from` on into shared memory, in the order of the ids; their number
+        // the keys from `from` on (the ids of equal keys ascending) into shared memory; their number
         auto collect = [&](uint32_t from) {
-            int n = 0;
+            int at = 0;
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) {
-                const unsigned m = __ballot_sync(all, key[i] >= from);
-                if (m) {
-                    const int at = n + __popc(m & ((1u << lane) - 1u));
-                    if (key[i] >= from && at < 32)
-                        cand_s[warp][at] =
-                            make_uint4(key[i], (uint32_t)(32 * i + lane), __float_as_uint(l[i]), __float_as_uint(b[i]));
-                    n += __popc(m);
-                }
+            for (int i = 0; i < NPL; ++i) at += key[i] >= from;
+            const int own = at;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int before = __shfl_up_sync(all, at, o);
+                if (lane >= o) at += before;
             }
+            const int n = __shfl_sync(all, at, 31);
+            at -= own;
+            if (n <= 32)
+#pragma unroll
+                for (int i = 0; i < NPL; ++i)
+                    if (key[i] >= from) cand_s[warp][at++] = (unsigned long long)key[i] << 32 | (uint32_t)~(32 * i + lane);
             __syncwarp();
             return n;
         };
-        // lane j < n brings a candidate, collected as its j-th, and takes the j-th largest
+        // lane j < n brings candidate j and takes the j-th largest
         float bj = 0.0f;
-        auto order = [&](uint4 c, int n) {
+        auto order = [&](unsigned long long c, int n) {
             int place = 0;
-            for (int j = 0; j < n; ++j) {
-                const uint32_t ok = cand_s[warp][j].x;
-                place += ok > c.x || (ok == c.x && j < lane);
-            }
+            for (int j = 0; j < n; ++j) place += cand_s[warp][j] > c;
             __syncwarp();
             if (lane < n) cand_s[warp][place] = c;
             __syncwarp();
-            c = cand_s[warp][lane];
-            mine = c.x, id = (int)c.y, lj = __uint_as_float(c.z), bj = __uint_as_float(c.w);
+            c = lane < n ? cand_s[warp][lane] : 0ull;
+            mine = (uint32_t)(c >> 32), id = (int)~(uint32_t)c;
             __syncwarp();
         };
-        const int n = collect(max(bound, 1u));  // keys of 0 are no experts
+        const int n = collect(max(bound, 1u));
         if (n <= 32) {
             order(cand_s[warp][lane], n);
         } else {  // many equal keys: one pick at a time
@@ -283,11 +296,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
                     if ((uint32_t)(32 * i + lane) == e) left[i] = 0;
                 if (lane == j) mine = m, id = (int)e;
             }
-            if (lane < want) {
+        }
+        auto pick_inputs = [&] {  // of lane j's pick; without scores the key is the logit
+            if (!SCORED) {
+                lj = key_value(mine);
+            } else if (lane < want) {
                 lj = ops_load(a.logits, a.type, row + id);
                 if (a.bias) bj = a.bias[id];
             }
-        }
+        };
+        pick_inputs();
         if (!SCORED || exact) break;
         if (__any_sync(all, unsure)) {  // of the groups
             exact = 1;
@@ -308,12 +326,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
             exact = 1;
             continue;
         }
-        uint4 c = cand_s[warp][lane];
-        if (lane < close && c.x != kKeyNegInf)
-            c.x = rank_key(__fadd_rn(score_exact<KIND>(__uint_as_float(c.z), 0.0, 1.0), __uint_as_float(c.w)));
-        if (lane < close) cand_s[warp][lane].x = c.x;
+        unsigned long long c = lane < close ? cand_s[warp][lane] : 0ull;
+        if (lane < close && (uint32_t)(c >> 32) != kKeyNegInf) {
+            const int e = (int)~(uint32_t)c;
+            const float se = score_exact<KIND>(ops_load(a.logits, a.type, row + e), 0.0, 1.0);
+            c = (unsigned long long)rank_key(__fadd_rn(se, a.bias[e])) << 32 | (uint32_t)c;
+            cand_s[warp][lane] = c;
+        }
         __syncwarp();
         order(c, close);
+        pick_inputs();
         break;
     }
     s = lane < a.k && mine != kKeyNegInf ? score_f32<KIND>(lj, top, sum) : 0.0f;
@@ -377,9 +399,9 @@ extern "C" int32_t clb_route_experts_device(const clb_route_config_v1* cfg, cons
                     clb::ops_aligned(d_ids, 4) && clb::ops_aligned(d_w, 4) && clb::ops_aligned(d_status, 4),
                 CLB_E_INVALID, "misaligned pointer argument");
         clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, c.n_groups,
-                         c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, 1, c.scale,
+                         c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, c.n_experts / c.n_groups, 0, c.scale,
                          (float)c.n_groups / (float)c.n_experts};
-        while (2 * a.lanes_per_group * a.groups <= 32) a.lanes_per_group *= 2;
+        while ((2 * a.groups) << a.log_lanes <= 32) ++a.log_lanes;
         const bool scored = d_bias || (a.groups > 1 && a.pair);
         const int per_lane = (c.n_experts + 31) / 32;
         cuda_check(clb::ops_launch(scored ? clb::route_kernel<true>(c.score, per_lane) : clb::route_kernel<false>(c.score, per_lane),

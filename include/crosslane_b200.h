@@ -468,7 +468,9 @@ int32_t clb_expert_forward_noalloc(int32_t type, const void* w_gate, const void*
  * (NULL = legacy default stream), allocate nothing, do not synchronise, may be captured into
  * a graph, and check every argument before they touch the GPU. Zero tokens are no work and
  * no error. Rows are pitched: `ld_*` is the distance of two rows in elements (>= the row's
- * length). No counterpart in crosslane's lanes. */
+ * length). Their kernels are launched so that they are set up under the end of the kernel in
+ * front (programmatic dependent launch); they touch no memory before that kernel is
+ * complete. No counterpart in crosslane's lanes. */
 
 /* Element types. */
 #define CLB_F32 0
@@ -499,13 +501,15 @@ typedef struct clb_route_config_v1 {
 
 /* Picks of `tokens` rows of logits [tokens][n_experts]: d_ids [tokens][k] int32, d_w
  * [tokens][k] fp32, best first.
- *   s = sigmoid(l), softmax(l) or sqrt(softplus(l)), correctly rounded to fp32;
- *   rank = fl(s + d_bias[e]), or the logit itself without a bias (s rises with l);
+ *   s = sigmoid(l), softmax(l) or sqrt(softplus(l));
+ *   rank = fl(fl(s) + d_bias[e]) with fl(s) the correctly rounded float, or the logit itself
+ *   without a bias (s rises with l);
  *   with groups, those top_groups with the largest value stay (ties to the lower group):
  *   CLB_GROUP_MAX the largest rank, CLB_GROUP_PAIR the fp32 sum of the two largest
- *   s + bias (s without a bias);
+ *   fl(s) + bias (fl(s) without a bias);
  *   the k largest ranks are picked, ties to the lower id;
- *   w = s, divided by (sum of the picks' s + 1e-20) if renormalize, times scale.
+ *   w = s (fp32, within a few ulp), divided by (sum of the picks' s + 1e-20) if renormalize,
+ *   times scale.
  * An expert whose logit or bias is -inf is not available (it still counts in the softmax
  * if only its bias is -inf). Places left over take the remaining ids in ascending order
  * with weight 0, so the ids of a token are always distinct and in range: a row with no
@@ -542,8 +546,10 @@ typedef struct clb_block_norm_config_v1 {
  * (may be d_h itself) and d_x (NULL: none) the next block's input. d_y NULL: h' = h, only x
  * is written, and d_h_out, d_gate and d_w_post have to be NULL. d_w_post, d_w_pre [dim] fp32,
  * NULL = ones. Sums and h' are fp32 (x comes from h' before it is rounded to h_type); the
- * order of a row's sum depends on dim and the row count's class alone, so results repeat.
- * Apart from d_h_out = d_h with the same type and pitch, an output overlaps no input. */
+ * order of a row's sum depends on the layout and on whether there are more than 296 rows, so
+ * results repeat. Squares are summed as they are: values above about 1e18 overflow. Apart
+ * from d_h_out = d_h with the same pitch, an output overlaps no row of an input (else
+ * CLB_E_INVALID) nor a gate or weight vector. */
 int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, int32_t tokens, const void* d_h, const void* d_y,
                               const void* d_gate, const float* d_w_post, const float* d_w_pre, void* d_h_out,
                               void* d_x, void* stream, clb_error_v1* err);

@@ -93,11 +93,13 @@ def check_route(torch, op, logits, bias, ids, w, kind, groups=1, top_groups=1, p
             assert np.all(np.isnan(gw[t])), t
             continue
         # A score: expf and log1pf within 2 ulp (4 u each), a division within 2 ulp (4 u), additions
-        # and the root 1 u each: 9 u; softmax: exponentials of 6 u over a sum whose terms have 6 u and
-        # whose chains are at most 37 additions (32 of a lane, 5 of the tree), divided: 6 + 6 + 37 + 4 u.
+        # and the root 1 u each: 9 u. Softmax: an exponential of 6 u over a sum; a term exp(d) of
+        # the sum is off by |d| u in its argument and 4 + 2.4 |d| u in __expf, and the mean of |d|
+        # weighted by the terms is the entropy less the top's own, at most ln E <= 7; 37 additions
+        # in a chain (32 of a lane, 5 of the tree): 4 + 3.4 * 7 + 37 = 65 u; the division: 75 u.
         # Renormalised: the same again for the picks' sum, with its k additions, 1e-20 and the
         # division. Then the scale. Scores below 2^-126 may be flushed.
-        sc = 53 if kind == "softmax" else 9
+        sc = 75 if kind == "softmax" else 9
         tol = (2 * sc + k + 4 if renorm else sc + 2) * U * np.abs(ww) + 2.0 ** -149 * max(1.0, scale)
         s = np.where(ww > 0, scores64(kind, l32[t].astype(np.float64))[wi], 0.0)
         tol += 2.0 ** -125 * scale / ((s.sum() + 1e-20) if renorm else 1.0)
