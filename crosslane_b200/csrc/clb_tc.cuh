@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace clb {
 
 constexpr uint32_t kTcSuspendNs = 20000;      // try_wait suspend hint
@@ -87,16 +89,16 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 
 // The driver's cuTensorMapEncodeTiled, resolved once.
 inline cudaError_t tc_encoder(EncodeTiledFn* out) {
-    static EncodeTiledFn encode = nullptr;
-    if (!encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-        if (e != cudaSuccess) return e;
-        if (!fn || q != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
-        encode = reinterpret_cast<EncodeTiledFn>(fn);
-    }
-    *out = encode;
+    static std::atomic<EncodeTiledFn> known{nullptr};
+    *out = known.load(std::memory_order_acquire);
+    if (*out) return cudaSuccess;
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess) return e;
+    if (!fn || q != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    *out = reinterpret_cast<EncodeTiledFn>(fn);
+    known.store(*out, std::memory_order_release);
     return cudaSuccess;
 }
 

@@ -580,8 +580,10 @@ uint64_t clb_int8_linear_workspace_bytes(int32_t tokens, int32_t k);
  * both), d_bias [n] fp32 or NULL. x of a floating type is quantised per token as
  * clb_int8_quantize_device does (d_x_scale NULL); CLB_I8 x brings its scales in d_x_scale.
  * d_w, d_ws and CLB_I8 x are 16-byte aligned. d_ws (ws_bytes >= the size above; may be NULL
- * for CLB_I8) is the caller's: calls that overlap on the GPU need one each. A token whose
- * scale is NaN gives a row of NaN. The result does not depend on the other tokens of the
+ * for CLB_I8) is the caller's: calls that overlap on the GPU need one each. d_out overlaps
+ * none of the others. The integer sums stay below 2^31 for |q|, |w| <= 127, which is what the
+ * quantiser makes, and for any int8 values up to k = 131071. A token whose scale is NaN gives
+ * a row of NaN. The result does not depend on the other tokens of the
  * call. *d_status (int32, may be NULL) becomes 3 if a bounded wait in the kernel ran out
  * (the output is then incomplete). */
 int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, const int8_t* d_w, const float* d_w_scale,

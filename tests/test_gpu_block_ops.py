@@ -405,6 +405,37 @@ def test_norm_rows_that_start_anywhere(cb, cuda, T, D, h_t, y_t):
     check_norm(torch, n64(x), xw, (rh, bz), D, y_t, (np.abs(xw) / np.maximum(np.abs(new), 1e-300), new))
 
 
+@pytest.mark.parametrize("T", [1, 7, 500])
+@pytest.mark.parametrize("D", [64, 100, 1024])
+def test_norm_parts_of_one_buffer(cb, cuda, T, D):
+    """h, y, h_out and x as columns of one buffer, whose rows interleave."""
+    torch = cuda
+    buf = torch.randn((T, 4 * D), generator=torch.Generator(device="cuda").manual_seed(T + D), device="cuda")
+    h, y, out, x = (buf[:, i * D:(i + 1) * D] for i in range(4))
+    keep = buf.clone()
+    apart = [torch.empty((T, D), device="cuda") for _ in range(2)]
+    op = cb.BlockNorm(D)
+    op.run(h.contiguous(), d_y=y.contiguous(), d_h_out=apart[0], d_x=apart[1])
+    op.run(h, d_y=y, d_h_out=out, d_x=x)
+    for got, want in ((out, apart[0]), (x, apart[1])):  # the scalar and the aligned kernel add in another order
+        assert torch.allclose(got, want, rtol=2.0 ** -18, atol=1e-6)
+    assert torch.equal(buf[:, :2 * D], keep[:, :2 * D])
+    if T > 1:
+        with pytest.raises(cb.ClbError):
+            op.run(h, d_y=y, d_h_out=buf[:, D // 2:D // 2 + D], d_x=x)
+
+
+def test_no_tokens(cb, cuda):
+    torch = cuda
+    z = lambda n, t=torch.float32: torch.empty((0, n), dtype=t, device="cuda")  # noqa: E731
+    cb.BlockNorm(64).run(z(64), d_y=z(64), d_h_out=z(64), d_x=z(64))
+    w = torch.zeros((8, 64), dtype=torch.int8, device="cuda")
+    lin = cb.Int8Linear(w, torch.zeros(8, device="cuda"))
+    lin.run(z(64), z(8), d_ws=torch.empty(lin.workspace_bytes(0), dtype=torch.uint8, device="cuda"))
+    lin.run(z(64, torch.int8), z(8), d_x_scale=torch.empty(0, device="cuda"))
+    cb.int8_quantize(z(64), z(64, torch.int8), torch.empty(0, device="cuda"))
+
+
 def test_norm_past_32_bits(cb, cuda):
     """Rows whose offsets in elements and bytes pass 2^32 (bf16, 131073 rows, 32768 apart)."""
     torch = cuda
@@ -628,6 +659,98 @@ def test_linear_outputs_that_start_anywhere(cb, cuda, T):
         mask = torch.ones_like(back, dtype=torch.bool)
         mask[:T, off:off + N] = False
         assert bool((back[mask] == 7).all()), (pad, off)
+
+
+@pytest.mark.parametrize("T", [1, 4, 9, 200])
+def test_linear_lowest_int8(cb, cuda, T):
+    """-128 on both sides, at the deepest K for which the sums cannot overflow."""
+    torch = cuda
+    K, N = 131071, 24
+    back = torch.full((N, 131072), -128, dtype=torch.int8, device="cuda")
+    q = torch.full((T, 131072), -128, dtype=torch.int8, device="cuda")
+    out = torch.empty((T, N), device="cuda")
+    cb.Int8Linear(back[:, :K], torch.ones(N, device="cuda")).run(q[:, :K], out, d_x_scale=torch.ones(T, device="cuda"))
+    assert bool((out == float(np.float32(128 * 128 * K))).all())
+
+
+@pytest.mark.parametrize("T", [1, 3, 20, 300])
+@pytest.mark.parametrize("ready", [False, True])
+def test_linear_sees_what_was_written_just_before(cb, cuda, T, ready):
+    """Weights and tokens made by the calls in front, without a pause: a kernel that starts under
+    the end of another must not read early."""
+    torch = cuda
+    K, N = 2048, 1536
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    w, ws = torch.empty((N, K), dtype=torch.int8, device="cuda"), torch.empty(N, device="cuda")
+    x, h = torch.empty((T, K), device="cuda"), torch.empty((T, K), device="cuda")
+    q, qs = torch.empty((T, K), dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+    lin, norm = cb.Int8Linear(w, ws), cb.BlockNorm(K, post=False)
+    wsp = torch.empty(lin.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+    floats = [torch.randn((N, K), generator=gen, device="cuda") for _ in range(8)]
+    inputs = [torch.randn((T, K), generator=gen, device="cuda") for _ in range(8)]
+    outs = [[torch.empty((T, N), device="cuda") for _ in range(8)] for _ in range(2)]
+    for wait, into in ((True, outs[0]), (False, outs[1])):
+        pause = torch.cuda.synchronize if wait else lambda: None
+        for i in range(8):
+            h.copy_(inputs[i])
+            pause()
+            norm.run(h, d_x=x)
+            pause()
+            cb.int8_quantize(floats[i], w, ws)
+            pause()
+            if ready:
+                cb.int8_quantize(x, q, qs)
+                pause()
+                lin.run(q, into[i], d_x_scale=qs)
+            else:
+                lin.run(x, into[i], d_ws=wsp)
+            pause()
+    torch.cuda.synchronize()
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import crosslane_b200 as cb
+T, K, N = int(sys.argv[2]), 1024, 512
+x, w = torch.randn((T, K), device="cuda"), torch.randint(-127, 128, (N, K), device="cuda").to(torch.int8)
+lin = cb.Int8Linear(w, torch.ones(N, device="cuda"))
+h, y = torch.randn((T, K), device="cuda"), torch.randn((T, K), device="cuda")
+out, h2, x2 = torch.empty((T, N), device="cuda"), torch.empty_like(h), torch.empty_like(h)
+ids, wts = torch.empty((T, 4), dtype=torch.int32, device="cuda"), torch.empty((T, 4), device="cuda")
+ws = torch.empty(lin.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+norm, route = cb.BlockNorm(K), cb.ExpertRoute(64, 4)
+def step():
+    norm.run(h, d_y=y, d_h_out=h2, d_x=x2)
+    route.run(h2[:, :64], ids, wts)
+    lin.run(x2, out, d_ws=ws)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    step()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (h2, x2, ids, wts, out)]
+for t in (h2, x2, wts, out):
+    t.zero_()
+step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (h2, x2, ids, wts, out)))
+print("captured first")
+"""
+
+
+@pytest.mark.parametrize("T", [1, 40, 400])
+def test_first_call_inside_a_capture(cuda, T):
+    """A process whose first calls are captured into a graph: the one-time set-up needs no eager call."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL, root, str(T)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
 
 
 def test_linear_past_32_bits(cb, cuda):
