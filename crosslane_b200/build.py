@@ -7,7 +7,8 @@
 (Run as a file, not `-m`: importing the package loads the library being rebuilt.)
 
 Plain nvcc, one object per .cu, linked into an in-tree shared library with the
-static CUDA runtime; the library's interface is include/crosslane_b200.h.
+static CUDA runtime; the library's interface is include/crosslane_b200.h. Where torch is
+installed, g++ also builds _torch_call.so, through which block_ops.py calls it.
 """
 import argparse
 import concurrent.futures as cf
@@ -31,6 +32,35 @@ FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-cont
                 "--expt-relaxed-constexpr"]
 
 
+CXX = os.environ.get("CXX", "g++")
+TORCH_CALL = os.path.join(HERE, "_torch_call.so")
+
+
+def _torch_call(force):
+    """The Python module over torch tensors; None where torch is not installed."""
+    import importlib.util
+    import sysconfig
+    torch = importlib.util.find_spec("torch")
+    if torch is None:
+        return None
+    home = os.path.dirname(torch.origin)
+    src = os.path.join(CSRC, "torch_call.cpp")
+    header = os.path.join(HERE, "..", "include", "crosslane_b200.h")
+    newest = max(os.path.getmtime(f) for f in (src, header, os.path.join(home, "version.py")))
+    if not force and os.path.exists(TORCH_CALL) and os.path.getmtime(TORCH_CALL) >= newest:
+        return TORCH_CALL
+    lib = os.path.join(home, "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    cmd = [CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I" + sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(home, "include"), "-isystem",
+           os.path.join(home, "include", "torch", "csrc", "api", "include"), "-isystem", cuda, src, "-o", TORCH_CALL,
+           "-L" + lib, "-Wl,-rpath," + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for torch_call.cpp:\n{r.stdout}\n{r.stderr}")
+    return TORCH_CALL
+
+
 def _deps():
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
     headers.append(os.path.join(HERE, "..", "include", "crosslane_b200.h"))
@@ -52,8 +82,10 @@ def _compile(src, force, build_dir=BUILD, extra=()):
 def build(force: bool = False, verbose: bool = False, trace: bool = False) -> str:
     build_dir, lib, extra = (BUILD_TRACE, LIB_TRACE, ["-DCLB_FLOW_TRACE"]) if trace else (BUILD, LIB, [])
     os.makedirs(build_dir, exist_ok=True)
-    with cf.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        call = ex.submit(_torch_call, force)
         results = list(ex.map(lambda s: _compile(s, force, build_dir, extra), SOURCES))
+        call.result()
     objs = [o for o, _ in results]
     rebuilt = any(r for _, r in results)
     if rebuilt or force or not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs):

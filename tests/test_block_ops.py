@@ -154,3 +154,41 @@ def test_wrappers_refuse():
         lin.run(torch.zeros(4, 64), torch.zeros(4, 8), d_ws=torch.zeros(lin.workspace_bytes(4), dtype=torch.uint8))
     with pytest.raises(cb.ClbError):
         lin.run(torch.zeros(4, 32), torch.zeros(4, 8))
+
+
+def test_wrappers_refuse_what_is_no_tensor():
+    torch = pytest.importorskip("torch")
+    r, n = cb.ExpertRoute(64, 6), cb.BlockNorm(64)
+    t, ids, w = torch.zeros(4, 64), torch.zeros(4, 6, dtype=torch.int32), torch.zeros(4, 6)
+    with pytest.raises(TypeError):
+        r.run([[0.0] * 64], ids, w)
+    with pytest.raises(TypeError):
+        r.run(t, None, w)
+    with pytest.raises(TypeError):
+        n.run(t, d_y=3, d_h_out=t.clone(), d_x=t.clone())
+    with pytest.raises(TypeError):
+        cb.Int8Linear(None, w)
+    with pytest.raises(cb.ClbError):
+        cb.Int8Linear(torch.zeros(8, 64, dtype=torch.int8), None)
+    with pytest.raises(cb.ClbError):
+        cb.int8_quantize(t, torch.zeros(4, 64, dtype=torch.int8), None)
+    with pytest.raises(cb.ClbError):  # no rows of elements
+        r.run(t.to_sparse(), ids, w)
+    for meta in (t.to("meta"),):  # no storage
+        with pytest.raises((cb.ClbError, RuntimeError)):
+            r.run(meta, ids, w)
+    with pytest.raises(cb.ClbError):  # values of one element: every row the same address
+        n.run(torch.zeros(4, 1).expand(4, 64), d_x=t.clone())
+    with pytest.raises(cb.ClbError):  # overlapping rows
+        n.run(torch.zeros(128).as_strided((4, 64), (16, 1)), d_x=t.clone())
+
+
+def test_messages_name_the_argument():
+    torch = pytest.importorskip("torch")
+    r = cb.ExpertRoute(64, 6)
+    t, ids, w = torch.zeros(4, 64), torch.zeros(4, 6, dtype=torch.int32), torch.zeros(4, 6)
+    for args, word in (((t.double(), ids, w), "logits"), ((t, ids.long(), w), "ids"), ((t, ids, w.half()), "weights"),
+                       ((t, ids, w, torch.zeros(63)), "bias"), ((t, ids, w), "CUDA")):
+        with pytest.raises(cb.ClbError) as e:
+            r.run(*args)
+        assert word in str(e.value) and e.value.code == CLB_E_INVALID
