@@ -1,8 +1,8 @@
 // The residual step between two blocks: RMSNorm after the block, gate, scaled residual sum,
 // RMSNorm before the next block, in one pass over the rows: y and h are read once, h' and x
 // written once, so the kernels are bound by those bytes. A CTA holds a row in registers. The
-// two sums of squares are fp32: per thread in element order, then over the warp and the CTA
-// in a fixed tree.
+// two sums of squares are fp32: per thread in element order (one chain, or one for the even
+// and one for the odd elements), then over the warp and the CTA in a fixed tree.
 #include <algorithm>
 #include <cmath>
 
@@ -14,7 +14,8 @@ namespace {
 
 constexpr int kNormMaxDim = 32768;
 constexpr int kNormFewRows = 296;  // two an SM
-constexpr int kRowSmem = 216 * 1024;  // shared memory for rows on an SM
+constexpr int kRowFlight = 104 * 1024, kRowFlightTwo = 132 * 1024;  // bytes of rows asked for ahead on an SM
+constexpr int kRowSmem = 216 * 1024;    // the most a single CTA's rows take
 
 struct NormArgs {
     const void *h, *y, *gate;
@@ -163,11 +164,31 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 // chunks where the rows have them, and several CTAs an SM hide the sums' latency. Measured on
 // a B200 (device time): 2048 x 7168 fp32 42.4 us (5.5 TB/s), 8192 x 5120 bf16 with a sigmoid
 // gate 66.5 us (6.3 TB/s, 96 % of a copy's rate); a CTA per row took 65 and 138 us.
-constexpr int kRowStages = 4;
+constexpr int kRowStages = 2;
 constexpr uint32_t kRowPolls = 1u << 20;  // waits for a copy, each with a suspend hint of 20 us
 
-// Eight values, number i of a row in shared memory.
-__device__ __forceinline__ void row8(uint32_t p, int type, int i, float (&v)[8]) {
+// The gates of two values. FAST: exp2 of the scaled argument and a reciprocal, the instructions
+// alone: off by at most (|g| + 8) half ulps of fp32, far below a half step of the 16-bit types
+// that the call's results are rounded to (8192 x 5120 in a stream: 75 us with expf).
+template <bool FAST>
+__device__ __forceinline__ F2 gate2(F2 g, int sigmoid) {
+    if (!sigmoid) return g;
+    if (!FAST) {
+        const float2 v = f2_floats(g);
+        return f2(gate_value(v.x, 1), gate_value(v.y, 1));
+    }
+    const float2 t = f2_floats(f2_mul(g, f2(-1.44269504f, -1.44269504f)));
+    float a, b;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(t.y));
+    const float2 d = f2_floats(f2_add(f2(a, b), f2(1.0f, 1.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(d.y));
+    return f2(a, b);
+}
+
+// Eight values, number i of a row in shared memory, as pairs.
+__device__ __forceinline__ void row8(uint32_t p, int type, int i, F2 (&v)[4]) {
     Raw8 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     const uint32_t at = p + (uint32_t)i * (type == CLB_F32 ? 32u : 16u);
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w) : "r"(at));
@@ -175,12 +196,34 @@ __device__ __forceinline__ void row8(uint32_t p, int type, int i, float (&v)[8])
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
                      : "r"(at + 16u));
-    raw8_floats(r, type, true, v);
+    float w[8];
+    raw8_floats(r, type, true, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = f2(w[2 * j], w[2 * j + 1]);
+}
+__device__ __forceinline__ void store8_pairs(void* p, int type, int64_t i, const F2 (&v)[4]) {
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = f2_floats(v[j]);
+        w[2 * j] = f.x, w[2 * j + 1] = f.y;
+    }
+    store8_aligned(p, type, i, w);
+}
+// The sum of squares of eight values, in two chains (even and odd ones).
+__device__ __forceinline__ void square_sum(F2& s, const F2 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = f2_fma(v[j], v[j], s);
+}
+__device__ __forceinline__ float both(F2 s) {
+    const float2 f = f2_floats(s);
+    return f.x + f.y;
 }
 
 template <int CH, int THREADS, int CTAS, int SET>
 __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArgs a, int rows, int stages, uint32_t y_bytes,
                                                                    uint32_t h_bytes, uint32_t g_bytes) {
+    constexpr bool FAST = SET == kTypesBF16 || SET == kTypesF16;  // the results have 16 bits
     extern __shared__ __align__(16) uint8_t row_smem[];
     __shared__ float part[4][32];
     __shared__ uint64_t bars[kRowStages];
@@ -204,20 +247,23 @@ __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArg
         for (int s = 0; s < stages; ++s)
             if (blockIdx.x + (int64_t)s * gridDim.x < rows) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
     }
-    float wp[CH][8], wq[CH][8];
+    F2 wp[CH][4], wq[CH][4];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
+        float p[8], q[8], g[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) wp[c][j] = 1.0f, wq[c][j] = 1.0f;
-        if (a.w_post) raw8_floats(load8<true>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, true, wp[c]);
-        if (a.w_pre) raw8_floats(load8<true>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, true, wq[c]);
+        for (int j = 0; j < 8; ++j) p[j] = q[j] = 1.0f;
+        if (a.w_post) raw8_floats(load8<true>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, true, p);
+        if (a.w_pre) raw8_floats(load8<true>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, true, q);
         if (a.gate_kind == CLB_GATE_CHANNEL) {
-            float g[8];
             raw8_floats(load8<true>(a.gate, a.gate_type, 0, c, a.dim), a.gate_type, true, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) wp[c][j] *= gate_value(g[j], a.gate_sigmoid);
+            for (int j = 0; j < 8; ++j) p[j] *= gate_value(g[j], a.gate_sigmoid);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wp[c][j] = f2(p[2 * j], p[2 * j + 1]), wq[c][j] = f2(q[2 * j], q[2 * j + 1]);
     }
+    const F2 keep = f2(a.residual_scale, a.residual_scale);
     __syncthreads();
     int stage = 0, turn = 0;
     uint32_t phase = 0;
@@ -229,36 +275,36 @@ __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArg
         const uint32_t sy = base + (uint32_t)stage * stage_bytes, sh = sy + y_bytes, sg = sh + h_bytes;
         // a copy that never came (the wait ran out) shows as a row of NaN
         const float ok = here ? 1.0f : __int_as_float(0x7fffffff);
-        float v[CH][8];
+        F2 v[CH][4];
         if (y_bytes) {
             float f = gt * ok;
             if (a.post) {
-                float ss = 0.0f, y[8];
+                F2 ss = 0, y[4];  // two zeros
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
                     if (tid + c * nt < units) {
                         row8(sy, y_type, tid + c * nt, y);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+                        square_sum(ss, y);
                     }
-                f *= rsqrtf(cta_sum(ss, part[2 * turn]) * a.inv_dim + a.post_eps);
+                f *= rsqrtf(cta_sum(both(ss), part[2 * turn]) * a.inv_dim + a.post_eps);
             }
+            const F2 ff = f2(f, f);
             char* out = const_cast<char*>(at(a.h_out, h_type, row * a.ld_h_out));
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int u = tid + c * nt;
                 if (u < units) {
-                    float y[8], g[8];
+                    F2 y[4], g[4];
                     row8(sy, y_type, u, y);
                     row8(sh, h_type, u, v[c]);
                     if (g_bytes) {
                         row8(sg, g_type, u, g);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) y[j] *= gate_value(g[j], a.gate_sigmoid);
+                        for (int j = 0; j < 4; ++j) y[j] = f2_mul(y[j], gate2<FAST>(g[j], a.gate_sigmoid));
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[c][j] = fmaf(f, y[j] * wp[c][j], a.residual_scale * v[c][j]);
-                    store8_aligned(out, h_type, 8 * u, v[c]);
+                    for (int j = 0; j < 4; ++j) v[c][j] = f2_fma(ff, f2_mul(y[j], wp[c][j]), f2_mul(keep, v[c][j]));
+                    store8_pairs(out, h_type, 8 * u, v[c]);
                 }
             }
         } else {
@@ -268,28 +314,27 @@ __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArg
         }
         float inv = ok;
         if (a.x) {
-            float ss = 0.0f;
+            F2 ss = 0;
 #pragma unroll
             for (int c = 0; c < CH; ++c)
-                if (tid + c * nt < units)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) ss = fmaf(v[c][j], v[c][j], ss);
-            inv *= rsqrtf(cta_sum(ss, part[2 * turn + 1]) * a.inv_dim + a.pre_eps);
+                if (tid + c * nt < units) square_sum(ss, v[c]);
+            inv *= rsqrtf(cta_sum(both(ss), part[2 * turn + 1]) * a.inv_dim + a.pre_eps);
         } else {
             __syncthreads();
         }
         // the CTA has read the stage
         if (tid == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, stage);
         if (a.x) {
+            const F2 ii = f2(inv, inv);
             char* out = const_cast<char*>(at(a.x, x_type, row * a.ld_x));
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int u = tid + c * nt;
                 if (u < units) {
-                    float w[8];
+                    F2 w[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = wq[c][j] * (v[c][j] * inv);
-                    store8_aligned(out, x_type, 8 * u, w);
+                    for (int j = 0; j < 4; ++j) w[j] = f2_mul(wq[c][j], f2_mul(v[c][j], ii));
+                    store8_pairs(out, x_type, 8 * u, w);
                 }
             }
         }
@@ -300,10 +345,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArg
 
 template <int SET>
 void (*rows_kernel(int ch, int threads))(NormArgs, int, int, uint32_t, uint32_t, uint32_t) {
-    return ch == 1          ? k_block_norm_rows<1, 32, 16, SET>
-           : ch == 2        ? (threads <= 32 ? k_block_norm_rows<2, 32, 16, SET> : k_block_norm_rows<2, 512, 1, SET>)
-           : threads <= 256 ? k_block_norm_rows<4, 256, 2, SET>
-                            : k_block_norm_rows<4, 512, 1, SET>;
+    return ch == 1   ? (threads <= 32 ? k_block_norm_rows<1, 32, 16, SET> : k_block_norm_rows<1, 1024, 1, SET>)
+           : ch == 2 ? (threads <= 32    ? k_block_norm_rows<2, 32, 16, SET>
+                        : threads <= 352 ? k_block_norm_rows<2, 352, 2, SET>
+                                         : k_block_norm_rows<2, 448, 2, SET>)
+                     : (threads <= 256 ? k_block_norm_rows<4, 256, 2, SET> : k_block_norm_rows<4, 512, 1, SET>);
 }
 
 decltype(rows_kernel<kTypesAny>(0, 0)) rows_kernel(int set, int ch, int threads) {
@@ -344,19 +390,25 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStrea
             set = i;
     }
     if (vec && tokens > kNormFewRows && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
-        int ch = units <= 32 ? 1 : units <= 64 ? 2 : 4;
-        auto threads_of = [&](int chunks) { return std::max(32, ((units + chunks - 1) / chunks + 31) / 32 * 32); };
-        // CTAs on an SM: by the registers (128 a thread), with two rows of shared memory each or more
-        int ctas = std::min(16, 512 / threads_of(ch));
-        while (ctas > 1 && kRowSmem / ctas / (int)stage < 2) --ctas;
-        if (ctas == 1 && units > 512 && units <= 1024) ch = 2;  // one CTA: more warps
-        const int threads = threads_of(ch), stages = std::min(kRowStages, kRowSmem / ctas / (int)stage);
+        // Two rows in flight for each CTA, and as many CTAs as bring that to 104 KB an SM, or two up to 132 KB:
+        // with more, reads and writes get into each other's way in HBM (8192 x 5120 bf16, gate: 66.6 us
+        // with 123 KB, 76 us with 184 KB; 8192 x 2048 fp32 / bf16: 35.0 us with 98 KB, 38.9 us with 123
+        // KB). Chunks a thread: 4 where rows are short; 2 for two CTAs with wide rows (the gated case with
+        // 4: 84 us); 1 for a single CTA, which has to hide its sums by itself (2048 x 7168 fp32: 39.5 us,
+        // with 2 41.0, with 4 42.0 us).
+        int ctas = std::min(16, kRowFlight / 2 / (int)stage);
+        if (ctas < 2) ctas = 4 * (int)stage <= kRowFlightTwo ? 2 : 1;
+        const int ch = units <= 32 ? 1 : units <= 64 ? 2 : ctas == 1 ? (units <= 1024 ? 1 : 4) : units > 512 && units <= 896 ? 2 : 4;
+        const int threads = std::max(32, ((units + ch - 1) / ch + 31) / 32 * 32);
+        if (ch == 4) ctas = std::min(ctas, 512 / threads);  // 128 registers a thread
+        else if (threads > 32) ctas = std::min(ctas, 2);
+        const int stages = 2;
         int sms = 0;
         const cudaError_t e = ops_device(&sms, [] {
             cudaError_t e = cudaSuccess;
             for (int set = kTypesAny; set <= kTypesF32F16; ++set)
                 for (int ch : {1, 2, 4})
-                    for (int threads : {32, 512})
+                    for (int threads : {32, 352, 448, 512})
                         if (e == cudaSuccess)
                             e = cudaFuncSetAttribute(rows_kernel(set, ch, threads),
                                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);

@@ -101,6 +101,35 @@ __device__ __forceinline__ void raw8_floats(const Raw8& r, int type, bool packed
     }
 }
 
+// Two floats in a register pair: sm_100a multiplies and adds both in one instruction, each rounded
+// as the scalar operation is.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 f2_floats(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
 // Eight elements from i on, aligned as for raw8_aligned.
 __device__ __forceinline__ void store8_aligned(void* p, int type, int64_t i, const float (&v)[8]) {
     if (type == CLB_F32) {
