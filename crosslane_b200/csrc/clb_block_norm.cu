@@ -13,7 +13,7 @@ namespace clb {
 namespace {
 
 constexpr int kNormMaxDim = 32768;
-constexpr int kNormFewRows = 296;  // two an SM
+constexpr int64_t kNormManyChunks = 200000;  // rows * chunks of 8 from which k_block_norm_rows is faster
 constexpr int kRowFlight = 104 * 1024, kRowFlightTwo = 132 * 1024;  // bytes of rows asked for ahead on an SM
 constexpr int kRowSmem = 216 * 1024;    // the most a single CTA's rows take
 
@@ -79,7 +79,9 @@ __host__ __device__ constexpr NormTypes norm_types(int set) {
                                   : NormTypes{CLB_F32, CLB_F16};
 }
 
-// One CTA per row, CH chunks of 8 values per thread: few rows, where the latency of one counts,
+// One CTA per row, CH chunks of 8 values per thread: few rows, where the latency of one counts (up
+// to 1.6 million values: 200 x 7168 fp32 6.4 us, with k_block_norm_rows 7.0; 400 x 7168 12.7 and
+// 11.5 us; 1200 x 1024 fp32 / bf16 3.9 and 5.5 us; 2000 x 1024 5.7 and 5.9 us),
 // rows that are not aligned, and rows too wide for k_block_norm_rows. Bound by the latency of the
 // loads and the two sums. Measured on a B200 (device time): 1 x 7168 fp32 3.2 us, 64 x 7168
 // 3.6 us, 777 x 2311 in rows of 2316 elements 6.9 us (3.1 TB/s).
@@ -389,7 +391,7 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStrea
             (!g_bytes || a.gate_type == t.other))
             set = i;
     }
-    if (vec && tokens > kNormFewRows && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
+    if (vec && (int64_t)tokens * units > kNormManyChunks && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
         // Two rows in flight for each CTA, and as many CTAs as bring that to 104 KB an SM, or two up to 132 KB:
         // with more, reads and writes get into each other's way in HBM (8192 x 5120 bf16, gate: 66.6 us
         // with 123 KB, 76 us with 184 KB; 8192 x 2048 fp32 / bf16: 35.0 us with 98 KB, 38.9 us with 123

@@ -546,8 +546,8 @@ typedef struct clb_block_norm_config_v1 {
  * (may be d_h itself) and d_x (NULL: none) the next block's input. d_y NULL: h' = h, only x
  * is written, and d_h_out, d_gate and d_w_post have to be NULL. d_w_post, d_w_pre [dim] fp32,
  * NULL = ones. Sums and h' are fp32 (x comes from h' before it is rounded to h_type); the
- * order of a row's sum depends on the layout and on whether there are more than 296 rows, so
- * results repeat. Squares are summed as they are: values above about 1e18 overflow. Apart
+ * order of a row's sum depends on the layout and on whether the call has more than 1.6 million
+ * values, so results repeat. Squares are summed as they are: values above about 1e18 overflow. Apart
  * from d_h_out = d_h with the same pitch, an output overlaps no row of an input (else
  * CLB_E_INVALID) nor a gate or weight vector. */
 int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, int32_t tokens, const void* d_h, const void* d_y,

@@ -456,6 +456,77 @@ def test_norm_past_32_bits(cb, cuda):
     assert torch.equal(ids[-64:].long(), torch.sort(logits[-64:].float(), dim=1, descending=True, stable=True).indices[:, :4])
 
 
+# calls of more than 1.6 million values, aligned rows: the kernel whose CTAs stay
+LONG = [(210000, 8), (26000, 64), (13001, 128), (6600, 256), (6601, 264), (3301, 512), (3200, 520), (1701, 1024), (850, 2048),
+        (790, 2056), (420, 4096), (331, 5120), (301, 5640), (235, 7168), (225, 7176), (203, 8192), (199, 8200), (101, 16384)]
+
+
+@pytest.mark.parametrize("T,D", LONG)
+def test_norm_many_rows(cb, cuda, T, D):
+    run_norm(cb, cuda, T, D, gate="channel", sig=True, seed=8)
+    run_norm(cb, cuda, T, D, "bfloat16", "bfloat16", "bfloat16", gate="full", seed=9)
+
+
+@pytest.mark.parametrize("h_t,y_t,x_t", [("float32", "float32", "float32"), ("bfloat16", "bfloat16", "bfloat16"),
+                                         ("float16", "float16", "float16"), ("float32", "bfloat16", "bfloat16"),
+                                         ("float32", "float16", "float16"), ("bfloat16", "float16", "float32"),
+                                         ("float16", "float32", "bfloat16"), ("bfloat16", "float32", "float32")])
+@pytest.mark.parametrize("T,D", [(3300, 512), (420, 4096), (330, 5120), (235, 7168), (205, 8192)])
+def test_norm_many_rows_types(cb, cuda, T, D, h_t, y_t, x_t):
+    run_norm(cb, cuda, T, D, h_t, y_t, x_t, gate="full", sig=True, seed=10)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True), (False, False)])
+def test_norm_many_rows_parts(cb, cuda, gate, post, pre):
+    run_norm(cb, cuda, 1700, 1024, y_t="bfloat16", gate=gate, sig=gate != "channel", post=post, pre=pre, pad=8, seed=11)
+    run_norm(cb, cuda, 240, 7168, gate=gate, sig=True, post=post, pre=pre, seed=12)
+
+
+def test_norm_many_rows_alone_and_in_place(cb, cuda):
+    torch = cuda
+    run_norm(cb, cuda, 3400, 512, with_y=False, x_t="bfloat16", seed=13)
+    run_norm(cb, cuda, 3400, 512, weights=False, seed=14)
+    a = run_norm(cb, cuda, 260, 7168, in_place=True, seed=15)
+    b = run_norm(cb, cuda, 260, 7168, in_place=False, seed=15)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    T, D = 2000, 1024
+    h = torch.randn((T, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    y = torch.randn((T, D), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    outs = [torch.empty((T, D), device="cuda") for _ in range(4)]
+    op = cb.BlockNorm(D)
+    op.run(h, d_y=y, d_h_out=outs[0], d_x=outs[1])
+    y[7, 3], h[1999, 5], y[1000] = math.nan, math.inf, 0.0
+    op.run(h, d_y=y, d_h_out=outs[2], d_x=outs[3])
+    good = torch.ones(T, dtype=torch.bool, device="cuda")
+    good[[7, 1000, 1999]] = False
+    assert torch.equal(outs[0][good], outs[2][good]) and torch.equal(outs[1][good], outs[3][good])
+    assert bool(torch.isnan(outs[3][7]).all()) and torch.equal(outs[2][1000], h[1000])
+    assert bool(torch.isnan(outs[3][1999, 5])) and float(outs[2][1999, 5]) == math.inf
+
+
+@pytest.mark.parametrize("gate_scale", [1.0, 20.0, 90.0])
+@pytest.mark.parametrize("T", [40, 2000])
+def test_norm_far_gates(cb, cuda, T, gate_scale):
+    """Sigmoids of far arguments, in 16 bits (the fast form) and fp32. The fast form is off by at most
+    (|g| + 8) u: 2^-17 for |g| <= 120, against half a step of 2^-9 (bf16) for the results; below
+    -87.3 both forms may give 0 for a sigmoid under 2^-126, which is off by 2^-126 |y| after the
+    product."""
+    torch = cuda
+    D = 1024
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    for t in ("bfloat16", "float32"):
+        dt = getattr(torch, t)
+        h = torch.zeros((T, D), dtype=dt, device="cuda")
+        y = torch.randn((T, D), generator=gen, device="cuda").to(dt)
+        g = (torch.randn((T, D), generator=gen, device="cuda") * gate_scale).clamp_(-120, 120).to(dt)
+        out = torch.empty_like(h)
+        cb.BlockNorm(D, post=False, pre=False, gate="full", gate_sigmoid=True).run(h, d_y=y, d_gate=g, d_h_out=out)
+        want = y.double() / (1 + torch.exp(-g.double()))
+        tol = want.abs() * ((2.0 ** -17 + 2.0 ** -8) if t == "bfloat16" else 16 * U) + 2.0 ** -126 * y.double().abs() + TINY[t]
+        assert bool(((out.double() - want).abs() <= tol).all())
+
+
 def test_norm_without_weights_or_block(cb, cuda):
     run_norm(cb, cuda, 9, 1024, weights=False)
     run_norm(cb, cuda, 9, 7168, with_y=False)
