@@ -409,7 +409,7 @@ void (*dot_kernel(int tt, bool vec, int type))(Int8Dot) {
 // quantised tokens by TMA (128-byte rows of K, 128-byte swizzle), four tcgen05.mma kind::i8 of
 // K = 32 per 128-byte block. Warps 0-7 are the epilogue (a lane is a weight row, so a warp's
 // store of one token is contiguous; warps 0-3 take the first half of the tile's tokens, 4-7
-// the second), warp 8 loads, warp 9 issues. Three forms:
+// the second; 16 warps were no faster), warp 8 loads, warp 9 issues. Three forms:
 //  * kSingle: a CTA walks over tiles of 128 rows, the epilogue of one under the products of
 //    the next (two accumulators);
 //  * kPair: the same with the two SMs of a cluster on one tile of 256 rows (cta_group::2): each
@@ -423,8 +423,8 @@ void (*dot_kernel(int tt, bool vec, int type))(Int8Dot) {
 // and SM) and the stores for shallow ones (2047 x 1536 x 7168 into fp32: 27 us, 49 % active), and
 // by the chain launch - quantise - load - join for small ones (64 x 5120 x 2304: 8.3 us).
 enum : int { kSingle = 0, kPair = 1, kSplit = 2 };
-constexpr int kGmEpiWarps = 8, kGmLoadWarp = 8, kGmMmaWarp = 9;
-constexpr int kGmThreads = 320;
+constexpr int kGmEpiWarps = 8, kGmLoadWarp = kGmEpiWarps, kGmMmaWarp = kGmEpiWarps + 1;
+constexpr int kGmThreads = 32 * (kGmEpiWarps + 2);
 constexpr int kGmMaxStages = 12, kGmMaxSplit = 8;
 constexpr int kGmABytes = 128 * 128;
 constexpr int kGmSmem = 220 * 1024;           // dynamic shared memory, alignment included
@@ -438,7 +438,7 @@ struct Int8Gemm {
     void* out;
     int* status;
     int64_t ld_out;
-    int tokens, n, kblocks, nt, stages, mtiles, tiles, split;
+    int tokens, n, kblocks, nt, stages, ntiles, tiles, split;
     bool pairs;  // 16-bit outputs: two rows of a token in one aligned 4-byte store
 };
 
@@ -611,8 +611,9 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     const int64_t total = (int64_t)my_tiles * nkb;
     const int tile_rows = PAIR ? 256 : 128, brows = PAIR ? g.nt / 2 : g.nt;
     const uint32_t stage_bytes = (uint32_t)kGmABytes + (uint32_t)brows * 128u;
-    auto row_of = [&](int tile) { return (tile % g.mtiles) * tile_rows + (PAIR ? 128 * rank : 0); };
-    auto token_of = [&](int tile) { return (tile / g.mtiles) * g.nt; };
+    // neighbours share the weights' rows (the other order: 143 us for 139 at 4096 x 7168 x 7168)
+    auto row_of = [&](int tile) { return (tile / g.ntiles) * tile_rows + (PAIR ? 128 * rank : 0); };
+    auto token_of = [&](int tile) { return (tile % g.ntiles) * g.nt; };
 
     if (tid == 32 * kGmLoadWarp) {
         for (int i = 0; i < g.stages; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1);
@@ -713,7 +714,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     } else {
         ops_begin();  // q_scale
         const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const int half = (g.nt / 16 + 1) / 2 * 16, c0 = warp < 4 ? 0 : half, c1 = warp < 4 ? half : g.nt;
+        constexpr int kParts = kGmEpiWarps / 4;  // of the tile's tokens
+        const int part = (g.nt / 16 + kParts - 1) / kParts * 16, c0 = min(g.nt, part * (warp >> 2)), c1 = min(g.nt, c0 + part);
         const uint32_t lead_empty = PAIR ? cluster_addr(acc_empty(0), 0) : 0u;
         bool ok = true;
         if (SPLIT) {
@@ -793,7 +795,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
         const int t0 = token_of(first) + rank * share, row = row_of(first) + (tid & 127);
         const int nc = min(share, min(g.nt - rank * share, g.tokens - t0));
         if (warp < kGmEpiWarps && row < g.n && !*abort_flag) {
-            for (int c = tid >> 7; c < nc; c += 2) {
+            for (int c = tid >> 7; c < nc; c += kGmEpiWarps / 4) {
                 int v[kGmMaxSplit], sum = 0;
 #pragma unroll
                 for (int p = 0; p < kGmMaxSplit; ++p) {
@@ -965,8 +967,8 @@ cudaError_t launch_int8_gemm(const Int8Args& a, int* status, bool overlap, const
     g.pairs = a.n % 2 == 0 && a.ld_out % 2 == 0 && ops_aligned(a.out, 4);
     const int joined = plan.mode == kSplit ? plan.split * share * 512 : 0;  // the peers' sums
     g.stages = std::min(kGmMaxStages, (kGmSmem - 1024 - joined) / (kGmABytes + brows * 128));
-    g.mtiles = (a.n + (pair ? 255 : 127)) / (pair ? 256 : 128);
-    g.tiles = g.mtiles * ((a.tokens + g.nt - 1) / g.nt);
+    g.ntiles = (a.tokens + g.nt - 1) / g.nt;
+    g.tiles = (a.n + (pair ? 255 : 127)) / (pair ? 256 : 128) * g.ntiles;
     const int at_once = pair ? d.clusters[2] : d.sms;
     return gm_launch(&g, plan.mode, a.out_type, plan.mode == kSplit ? g.tiles : std::min(g.tiles, at_once),
                      pair ? 2 : plan.split, overlap, s, nullptr);
