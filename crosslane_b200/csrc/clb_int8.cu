@@ -69,14 +69,18 @@ constexpr float kQuantSure = 0.49997f;  // a rounding to a distance below this s
 // Eight quotients as bytes. Values of 16 bits hit the borders exactly every few hundred times, so
 // that path is short too; tiny rows take the general form.
 __device__ __forceinline__ uint2 quant8(const float (&v)[8], const RowScale& r) {
+    constexpr float kRound = 12582912.0f;
+    const F2 inv = f2(r.inv, r.inv), round = f2(kRound, kRound), minus = f2(-1.0f, -1.0f);
     float f[8], off = 0.0f;
     uint32_t q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float t = v[j] * r.inv;
-        f[j] = t + 12582912.0f;
-        q[j] = __float_as_uint(f[j]);
-        off = fmaxf(off, fabsf(t - (f[j] - 12582912.0f)));
+    for (int j = 0; j < 8; j += 2) {
+        const F2 t = f2_mul(f2(v[j], v[j + 1]), inv), u = f2_add(t, round);
+        const float2 d = f2_floats(f2_add(t, f2_fma(u, minus, round)));  // from the rounded quotient
+        const float2 uf = f2_floats(u);
+        f[j] = uf.x, f[j + 1] = uf.y;
+        q[j] = __float_as_uint(uf.x), q[j + 1] = __float_as_uint(uf.y);
+        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
     }
     if (off > kQuantSure)
 #pragma unroll
@@ -123,10 +127,24 @@ __device__ __forceinline__ float cta_max_nan(float m, float* part) {
     __syncthreads();
     return warp_max_nan(lane < (int)(blockDim.x >> 5) ? part[lane] : 0.0f);
 }
-__device__ __forceinline__ float max8_nan(const float (&v)[8], float m) {
+// The largest magnitude of eight aligned values and m (NaN if there is one); two at a time in 16 bits.
+template <int TYPE>
+__device__ __forceinline__ float max8_nan(const Raw8& r, float m) {
+    if (TYPE == CLB_F32) {
+        float v[8];
+        raw8_floats(r, TYPE, true, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
-    return m;
+        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+        return m;
+    }
+    if (TYPE == CLB_BF16) {
+        auto part = [](const uint32_t& w) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)); };
+        const __nv_bfloat162 x = __hmax2_nan(__hmax2_nan(part(r.a.x), part(r.a.y)), __hmax2_nan(part(r.a.z), part(r.a.w)));
+        return max_nan(m, max_nan(__low2float(x), __high2float(x)));
+    }
+    auto part = [](const uint32_t& w) { return __habs2(*reinterpret_cast<const __half2*>(&w)); };
+    const __half2 x = __hmax2_nan(__hmax2_nan(part(r.a.x), part(r.a.y)), __hmax2_nan(part(r.a.z), part(r.a.w)));
+    return max_nan(m, max_nan(__low2float(x), __high2float(x)));
 }
 
 // A CTA per aligned row, CH chunks of 8 values a thread in registers; or (CH = 0) rows too long for
@@ -148,16 +166,10 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
     const float tail = last < a.k ? ops_load(x, TYPE, last) : 0.0f;
     if (CH) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            raw8_floats(raw[i], TYPE, true, v);
-            m = max8_nan(v, m);
-        }
+        for (int i = 0; i < CH; ++i) m = max8_nan<TYPE>(raw[i], m);
     } else {
 #pragma unroll 4
-        for (int c = tid; c < chunks; c += nt) {
-            raw8_floats(raw8_aligned(x, TYPE, 8 * (int64_t)c, true), TYPE, true, v);
-            m = max8_nan(v, m);
-        }
+        for (int c = tid; c < chunks; c += nt) m = max8_nan<TYPE>(raw8_aligned(x, TYPE, 8 * (int64_t)c, true), m);
     }
     float stored;
     const RowScale r = row_scale(cta_max_nan(max_nan(m, fabsf(tail)), part), &stored);
@@ -309,10 +321,7 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
 #pragma unroll
             for (int t = 0; t < TT; ++t) raw[t] = raw8_aligned(source(t), TYPE, 8 * (int64_t)c, true);
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                raw8_floats(raw[t], TYPE, true, v);
-                m[t] = max8_nan(v, m[t]);
-            }
+            for (int t = 0; t < TT; ++t) m[t] = max8_nan<TYPE>(raw[t], m[t]);
         }
         for (int i = last; i < a.k; i += kDotThreads)
 #pragma unroll
