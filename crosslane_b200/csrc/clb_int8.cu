@@ -147,22 +147,32 @@ __device__ __forceinline__ float max8_nan(const Raw8& r, float m) {
     return max_nan(m, max_nan(__low2float(x), __high2float(x)));
 }
 
-// A CTA per aligned row, CH chunks of 8 values a thread in registers; or (CH = 0) rows too long for
-// that, read twice. The columns behind the last whole chunk are single values of the first
-// threads. Bound by the rows' bytes: 4096 x 7168 fp32 24 us (6.0 TB/s), bf16 22 us (3.9 TB/s:
+// A CTA per row, CH chunks of 8 values a thread in registers; or (CH = 0) rows too long for that,
+// read twice. Rows that start anywhere (not ALIGNED) come through shared memory. The columns behind
+// the last whole chunk are single values of the first threads. Bound by the rows' bytes: 4096 x 7168 fp32 24 us (6.0 TB/s), bf16 22 us (3.9 TB/s:
 // eleven instructions a value); 64 x 5120 bf16 1.9 us.
-template <int CH, int TYPE>
+template <int CH, int TYPE, bool ALIGNED>
 __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
     __shared__ float part[32];
     ops_begin();
     const int tid = threadIdx.x, nt = blockDim.x, chunks = a.k >> 3, last = 8 * chunks + tid;
     const void* x = row_at(a.x, TYPE, (int64_t)blockIdx.x * a.ld_x);
     int8_t* q = a.q + (int64_t)blockIdx.x * a.ld_q;
+    extern __shared__ uint4 row_smem[];
+    const uint32_t smem = (uint32_t)__cvta_generic_to_shared(row_smem), off = (uint32_t)reinterpret_cast<uintptr_t>(x) & 15u;
     Raw8 raw[CH ? CH : 1];
     float v[8], m = 0.0f;
+    if (!ALIGNED) {
+        row_to_smem(smem, x, (uint32_t)a.k * (TYPE == CLB_F32 ? 4u : 2u), TYPE);
+        __syncthreads();
+    }
     if (CH)
 #pragma unroll
-        for (int i = 0; i < CH; ++i) raw[i] = raw8_aligned(x, TYPE, 8 * (int64_t)(tid + i * nt), tid + i * nt < chunks);
+        for (int i = 0; i < CH; ++i) {
+            const int c = tid + i * nt;
+            if (ALIGNED) raw[i] = raw8_aligned(x, TYPE, 8 * (int64_t)c, c < chunks);
+            else raw[i] = c < chunks ? raw8_smem(smem, off, TYPE, c) : Raw8{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        }
     const float tail = last < a.k ? ops_load(x, TYPE, last) : 0.0f;
     if (CH) {
 #pragma unroll
@@ -191,7 +201,8 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
     if (tid == 0) a.scale[blockIdx.x] = stored;
 }
 
-// Rows of any alignment, value by value, read twice (the second time from L1 or L2).
+// Rows of any alignment too long for shared memory, value by value, read twice (the second time
+// from L1 or L2).
 template <int TYPE>
 __global__ void __launch_bounds__(1024) k_int8_quantize_any(const QuantArgs a) {
     __shared__ float part[32];
@@ -211,10 +222,12 @@ __global__ void __launch_bounds__(1024) k_int8_quantize_any(const QuantArgs a) {
 
 template <int TYPE>
 void (*quantize_kernel(int ch, bool vec))(QuantArgs) {
-    return !vec      ? k_int8_quantize_any<TYPE>
-           : ch == 0 ? k_int8_quantize<0, TYPE>
-           : ch == 1 ? k_int8_quantize<1, TYPE>
-                     : k_int8_quantize<4, TYPE>;
+    return !vec ? (ch == 0   ? k_int8_quantize_any<TYPE>
+                   : ch == 1 ? k_int8_quantize<1, TYPE, false>
+                             : k_int8_quantize<4, TYPE, false>)
+                : (ch == 0   ? k_int8_quantize<0, TYPE, true>
+                   : ch == 1 ? k_int8_quantize<1, TYPE, true>
+                             : k_int8_quantize<4, TYPE, true>);
 }
 
 // `limit`: columns written (k, or a pitch of a multiple of 16 whose rest is zeros).
@@ -225,13 +238,15 @@ cudaError_t launch_int8_quantize(const void* x, int type, int64_t ld_x, int rows
     const int units = (limit + 7) / 8;
     // few rows: as many threads as the row has chunks, for the latency; many: 4 chunks a thread, so that
     // several rows of an SM overlap their loads and stores
-    const int ch = units > 4096 ? 0 : units > 1024 || (rows > 296 && units > 128) ? 4 : 1;
-    const int per = vec ? (ch ? ch : 128) : 8;
-    const int threads = std::min(1024, std::max(32, ((units * (vec ? 1 : 8) + per - 1) / per + 31) / 32 * 32));
+    const size_t staged = vec ? 0 : (size_t)k * ops_type_bytes(type) + 48;
+    const bool whole = units <= 4096 && staged <= 47 * 1024;  // with the static shared memory, below 48 KB
+    const int ch = !whole ? 0 : units > 1024 || (rows > 296 && units > 128) ? 4 : 1;
+    const int per = ch ? ch : vec ? 128 : 8;
+    const int threads = std::min(1024, std::max(32, ((units * (vec || ch ? 1 : 8) + per - 1) / per + 31) / 32 * 32));
     void (*kernel)(QuantArgs) = type == CLB_F32    ? quantize_kernel<CLB_F32>(ch, vec)
                                 : type == CLB_BF16 ? quantize_kernel<CLB_BF16>(ch, vec)
                                                    : quantize_kernel<CLB_F16>(ch, vec);
-    return ops_launch(kernel, (unsigned)rows, threads, 0, s, a);
+    return ops_launch(kernel, (unsigned)rows, threads, ch ? staged : 0, s, a);
 }
 
 struct Int8Args {
@@ -272,7 +287,7 @@ struct Int8Dot {
 template <int TT, bool VEC, int TYPE>
 __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     extern __shared__ uint4 dot_smem[];
-    __shared__ float part[TT][kDotThreads / 32], scale_s[TT];
+    __shared__ float part[kDotThreads / 32], scale_s[TT];
     ops_begin();
     const Int8Args& a = d.a;
     int8_t* qs = reinterpret_cast<int8_t*>(dot_smem);               // [TT][kpad]
@@ -309,47 +324,38 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
     int4 next[kDotAhead];
     fetch(next, here);
     for (int i = tid; i < d.rows * TT; i += kDotThreads) sums[i] = 0;
+    // a token's threads, one after the other in it
+    constexpr int kGroup = kDotThreads / TT, kWarps = kGroup / 32;
+    const int own = tid / kGroup, at = tid % kGroup;
+    int8_t* q = qs + (size_t)own * d.kpad;
     if (d.x) {
-        // whole chunks, and the columns behind them as single values of the first threads (zeros behind k)
-        const int whole = VEC ? a.k >> 3 : 0, last = 8 * whole + tid;
-        float m[TT], v[8];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) m[t] = 0.0f;
-        auto source = [&](int t) { return row_at(d.x, TYPE, min(t, a.tokens - 1) * d.ld_x); };
-        for (int c = tid; c < whole; c += kDotThreads) {
-            Raw8 raw[TT];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) raw[t] = raw8_aligned(source(t), TYPE, 8 * (int64_t)c, true);
-#pragma unroll
-            for (int t = 0; t < TT; ++t) m[t] = max8_nan<TYPE>(raw[t], m[t]);
-        }
-        for (int i = last; i < a.k; i += kDotThreads)
-#pragma unroll
-            for (int t = 0; t < TT; ++t) m[t] = max_nan(m[t], fabsf(ops_load(source(t), TYPE, i)));
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            m[t] = warp_max_nan(m[t]);
-            if (lane == 0) part[t][warp] = m[t];
-        }
+        // whole chunks, and the columns behind them as single values (zeros behind k)
+        const int whole = VEC ? a.k >> 3 : 0, last = 8 * whole + at;
+        const void* x = row_at(d.x, TYPE, min(own, a.tokens - 1) * d.ld_x);
+        float m = 0.0f, v[8];
+#pragma unroll 4
+        for (int c = at; c < whole; c += kGroup) m = max8_nan<TYPE>(raw8_aligned(x, TYPE, 8 * (int64_t)c, true), m);
+#pragma unroll 4
+        for (int i = last; i < a.k; i += kGroup) m = max_nan(m, fabsf(ops_load(x, TYPE, i)));
+        m = warp_max_nan(m);
+        if (lane == 0) part[warp] = m;
         __syncthreads();
-        for (int t = 0; t < TT && t < a.tokens; ++t) {
-            float stored;
-            const RowScale r = row_scale(warp_max_nan(part[t][lane & (kDotThreads / 32 - 1)]), &stored);
-            int8_t* q = qs + (size_t)t * d.kpad;
-            for (int c = tid; c < whole; c += kDotThreads) {
-                raw8_floats(raw8_aligned(source(t), TYPE, 8 * (int64_t)c, true), TYPE, true, v);
+        float stored;
+        const RowScale r = row_scale(warp_max_nan(part[own * kWarps + (lane & (kWarps - 1))]), &stored);
+        if (own < a.tokens) {
+#pragma unroll 2
+            for (int c = at; c < whole; c += kGroup) {
+                raw8_floats(raw8_aligned(x, TYPE, 8 * (int64_t)c, true), TYPE, true, v);
                 *reinterpret_cast<uint2*>(q + 8 * c) = quant8(v, r);
             }
-            for (int i = last; i < d.kpad; i += kDotThreads) q[i] = i < a.k ? quant1(ops_load(source(t), TYPE, i), r) : 0;
-            if (tid == 0) scale_s[t] = stored;
+#pragma unroll 2
+            for (int i = last; i < d.kpad; i += kGroup) q[i] = i < a.k ? quant1(ops_load(x, TYPE, i), r) : 0;
+            if (at == 0) scale_s[own] = stored;
         }
-    } else {
-        for (int t = 0; t < a.tokens; ++t) {
-            for (int p = tid; p < pieces; p += kDotThreads)
-                reinterpret_cast<int4*>(qs + (size_t)t * d.kpad)[p] = reinterpret_cast<const int4*>(a.q + t * a.ld_q)[p];
-            for (int i = 16 * pieces + tid; i < a.k; i += kDotThreads) qs[(size_t)t * d.kpad + i] = a.q[t * a.ld_q + i];
-            if (tid == 0) scale_s[t] = a.q_scale[t];
-        }
+    } else if (own < a.tokens) {
+        for (int p = at; p < pieces; p += kGroup) reinterpret_cast<int4*>(q)[p] = reinterpret_cast<const int4*>(a.q + own * a.ld_q)[p];
+        for (int i = 16 * pieces + at; i < a.k; i += kGroup) q[i] = a.q[own * a.ld_q + i];
+        if (at == 0) scale_s[own] = a.q_scale[own];
     }
     __syncthreads();
     int acc[TT];

@@ -153,8 +153,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
     }
     // the largest error of a score (s rises with l), and of the scores below the normal numbers
     const float off = !SCORED ? 0.0f
-                              : fmaf(KIND == CLB_SCORE_SOFTMAX ? 96.0f * kHalfUlp : 16.0f * kHalfUlp,
-                                     KIND == CLB_SCORE_SQRT_SOFTPLUS ? score_f32<KIND>(top, 0.0f, 1.0f) : 1.0f, 1e-18f);
+                              : fmaf((KIND == CLB_SCORE_SOFTMAX ? 96.0f : 16.0f) * kHalfUlp,
+                                     KIND == CLB_SCORE_SOFTMAX ? __fdividef(1.0f, fmaxf(sum, 1.0f)) : score_f32<KIND>(top, 0.0f, 1.0f),
+                                     1e-18f);
 
     uint32_t mine = 0;      // lane j: the key and id of the j-th largest rank
     int id = 0;
