@@ -851,12 +851,14 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
 }
 
 // The form of a product, by an estimate of its time (us) whose constants fit measurements
-// from 16 x 7168 x 1536 to 4096 x 7168 x 7168 on a B200 to about 10 %: a 128-byte block of K
-// costs its loads and, from about 100 token columns on, its multiply-adds; a tile a fixed
-// part, a launch or a split another. CTAs run in waves over the SMs, clusters in the number that fits at
-// once. Measured at 4096 x 7168 x 7168, 256 tokens a tile: single 198 us, pair 172 us; at
+// from 16 x 512 x 512 to 4096 x 7168 x 7168 on a B200 to about 10 % (520 choices of form and tile for
+// 16 to 128 tokens: the estimate's choice is 0.2 % slower than the best on average, 2.5 % at most):
+// a 128-byte block of K costs its loads and, from about 100 token columns on, its multiply-adds; a
+// tile a fixed part, a launch or a split another. CTAs run in waves over the SMs, clusters in the
+// number that fits at once. Measured at 4096 x 7168 x 7168, 256 tokens a tile: single 198 us, pair 172 us; at
 // 500 x 1536 x 7168: 10.9 and 11.2 us; at 64 x 5120 x 2304, 64 tokens: single 15.4 us, split in
-// two 13.0, in four 9.3, in six 8.6 us, in seven (more clusters than fit at once) 15.0 us.
+// two 13.0, in four 9.3, in six 8.6 us, in seven (more clusters than fit at once) 15.0 us;
+// at 64 x 512 x 2304: single 5.4 us, split in four 7.0 us.
 struct GmPlan {
     int mode, nt, split;
 };
@@ -876,7 +878,9 @@ GmPlan gm_plan(int tokens, int n, int kblocks, const GmDevice& d) {
         if (mode == kSplit && waves > 1) return;
         const double block = mode == kPair ? std::max(0.30, 0.241 + 0.00077 * nt) : std::max(0.29, 0.15 + 0.00139 * nt);
         const double blocks = (kblocks + split - 1) / split * block;
-        const double cost = mode == kSplit ? blocks + 5.2 + 0.02 * nt : waves * (blocks + 0.8) + 4.2;
+        const double full = std::min(1.0, (double)tiles / at_once);
+        const double cost = mode == kSplit ? blocks + 5.4 + 0.02 * nt + 0.3 * full
+                                           : waves * (blocks + 0.8) + 3.2 + 0.006 * nt + 0.6 * full;
         if (cost < least) least = cost, best = GmPlan{mode, nt, split};
     };
     for (int nt = 16; nt <= 256; nt += 16) {
