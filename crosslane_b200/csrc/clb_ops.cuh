@@ -156,57 +156,54 @@ __device__ __forceinline__ void store8_aligned(void* p, int type, int64_t i, con
 }
 
 // Rows that start anywhere, through shared memory: byte j of the row lies at `smem` + (address mod 16)
-// + j, so its whole 16-byte pieces are copied as such, and the up to 15 bytes on either side by
-// elements. bytes + 48 of shared memory; a __syncthreads in front of the first use of a copy.
+// + j, so its whole 16-byte pieces are copied as such (asynchronously: row_landed comes before the
+// first use), and the up to 15 bytes on either side by elements. bytes + 48 of shared memory.
 __device__ __forceinline__ void row_to_smem(uint32_t smem, const void* row, uint32_t bytes, int type) {
     const char* p = static_cast<const char*>(row);
     const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u, es = type == CLB_F32 ? 4u : 2u;
     const uint32_t head = min((16u - off) & 15u, bytes), pieces = (bytes - head) >> 4, done = head + 16u * pieces;
-    for (uint32_t i = threadIdx.x; i < pieces; i += blockDim.x) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p + head + 16u * i);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(smem + off + head + 16u * i), "r"(v.x), "r"(v.y), "r"(v.z),
-                     "r"(v.w)
+    for (uint32_t i = threadIdx.x; i < pieces; i += blockDim.x)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem + off + head + 16u * i), "l"(p + head + 16u * i)
                      : "memory");
-    }
     const uint32_t edge = (head + bytes - done) / es;  // elements in front of and behind the pieces
     if (threadIdx.x < edge) {
         const uint32_t at = threadIdx.x * es < head ? threadIdx.x * es : done + threadIdx.x * es - head;
         if (type == CLB_F32)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(smem + off + at), "r"(*reinterpret_cast<const uint32_t*>(p + at))
-                         : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem + off + at), "l"(p + at) : "memory");
         else
             asm volatile("st.shared.u16 [%0], %1;" ::"r"(smem + off + at), "h"(*reinterpret_cast<const uint16_t*>(p + at))
                          : "memory");
     }
 }
-// Eight elements of such a row from its chunk c on, as raw8_aligned gives them; off: address mod 16.
-template <int S, bool HALF, int WORDS>
-__device__ __forceinline__ Raw8 shifted(const uint32_t (&w)[12]) {
-    uint32_t o[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        o[j] = j >= WORDS ? 0u : HALF ? __funnelshift_r(w[j + S], w[j + S + 1], 16) : w[j + S];
-    return Raw8{make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7])};
+__device__ __forceinline__ void row_landed() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 }
+// Eight elements of such a row from its chunk c on, as raw8_aligned gives them; off: address mod 16.
+// The words are moved by selects: a branch for each shift is 8 times the code, and what a launch of
+// few rows waits for is its code.
 __device__ __forceinline__ Raw8 raw8_smem(uint32_t smem, uint32_t off, int type, int c) {
     uint32_t w[12];
     const uint32_t p = smem + (uint32_t)c * (type == CLB_F32 ? 32u : 16u);
+    const int n = type == CLB_F32 ? 8 : 4;
 #pragma unroll
     for (int i = 0; i < 3; ++i)
         if (i < 2 || type == CLB_F32)
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
                          : "r"(p + 16u * i));
-    if (type == CLB_F32)
-        return off < 4u ? shifted<0, false, 8>(w) : off < 8u ? shifted<1, false, 8>(w) : off < 12u ? shifted<2, false, 8>(w)
-                                                                                                    : shifted<3, false, 8>(w);
-    if (off & 2u)
-        return off < 4u ? shifted<0, true, 4>(w) : off < 8u ? shifted<1, true, 4>(w) : off < 12u ? shifted<2, true, 4>(w)
-                                                                                                  : shifted<3, true, 4>(w);
-    return off < 4u ? shifted<0, false, 4>(w) : off < 8u ? shifted<1, false, 4>(w) : off < 12u ? shifted<2, false, 4>(w)
-                                                                                                : shifted<3, false, 4>(w);
+        else
+            w[8] = w[9] = w[10] = w[11] = 0u;
+    const bool two = off & 8u, one = off & 4u;
+#pragma unroll
+    for (int j = 0; j < 10; ++j) w[j] = two ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 9; ++j) w[j] = one ? w[j + 1] : w[j];
+    if (n == 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 2u) << 3);
+    return Raw8{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
 }
-
 __device__ __forceinline__ float ops_warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

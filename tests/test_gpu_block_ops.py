@@ -246,6 +246,26 @@ def test_route_groups_an_ulp_apart(cb, cuda, kind, with_bias, E, k, groups, top)
 
 
 @pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+@pytest.mark.parametrize("mean", [-60.0, -14.0, -3.0, 9.0])
+def test_route_small_and_close_scores(cb, cuda, kind, mean):
+    """Scores all tiny or all close to 1, and biases of the size of their last bits."""
+    torch = cuda
+    E, k = 320, 8
+    for seed in range(6):
+        rng = np.random.default_rng(seed * 31 + 5)
+        l = (rng.standard_normal((9, E)) * 0.01 + mean).astype(np.float32)
+        held = scores64(kind, l[0].astype(np.float64)).astype(np.float32)
+        bias = (rng.integers(-3, 4, E) * np.spacing(held.max())).astype(np.float32)
+        bias[rng.random(E) < 0.3] *= np.float32(0.37)
+        logits, b = torch.from_numpy(l).cuda(), torch.from_numpy(bias).cuda()
+        for groups, top in ((1, 1), (8, 3)):
+            ids, w = torch.empty((9, k), dtype=torch.int32, device="cuda"), torch.empty((9, k), device="cuda")
+            op = cb.ExpertRoute(E, k, score=kind, n_groups=groups, top_groups=top)
+            op.run(logits, ids, w, d_bias=b)
+            check_route(torch, op, logits, b, ids, w, kind, groups, top, True)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
 def test_route_huge_and_tiny_logits(cb, cuda, kind):
     torch = cuda
     E, k = 64, 8
@@ -599,6 +619,28 @@ def test_quantize_exact(cb, cuda, dtype, rows, k, pad, extra):
     assert np.array_equal(s[:rows].double().cpu().numpy(), ws) and float(s[rows]) == -7
     assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8))
     assert bool((q._base[:, k:] == 99).all())  # columns behind the row stay
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(3, 1), (3, 2), (3, 5), (3, 8), (3, 9), (3, 23), (3, 24), (5, 255), (5, 1001), (300, 1100),
+                                    (2, 8195), (2, 12000), (2, 12019), (2, 12020), (2, 12050), (2, 24039), (2, 24041)])
+def test_quantize_rows_that_start_anywhere(cb, cuda, dtype, rows, k):
+    """Every first element within 32 bytes, and pitches that move the start from row to row; a NaN on both
+    sides of each row shows any value that does not belong to it."""
+    torch = cuda
+    t = getattr(torch, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    values = torch.randn((rows, k), generator=gen, device="cuda").to(t)
+    wq, ws = quant64(values.double().cpu().numpy())
+    for first in range(1, 10 if k > 100 else 18):
+        pitch = k + 2 + first % 3
+        back = torch.full((first + rows * pitch + 8,), math.nan, dtype=t, device="cuda")
+        x = back[first:first + rows * pitch].view(rows, pitch)[:, :k]
+        x.copy_(values)
+        q, s = padded_int8(torch, rows, k), torch.empty(rows, device="cuda")
+        cb.int8_quantize(x, q, s)
+        assert np.array_equal(s.double().cpu().numpy(), ws), first
+        assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8)), first
 
 
 def test_quantize_borders_and_small_scales(cb, cuda):
