@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         auto pick_inputs = [&] {  // of lane j's pick; without scores the key is the logit
             if (!SCORED) {
                 lj = key_value(mine);
-            } else if (lane < want) {
+            } else if (lane < want && mine) {  // after the second order there may be no (k + 1)-th
                 lj = ops_load(a.logits, a.type, row + id);
                 if (a.bias) bj = a.bias[id];
             }

@@ -246,6 +246,25 @@ def test_route_groups_an_ulp_apart(cb, cuda, kind, with_bias, E, k, groups, top)
 
 
 @pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+@pytest.mark.parametrize("E,k", [(40, 4), (33, 16), (384, 8), (1024, 2)])
+def test_route_close_picks_and_a_far_rest(cb, cuda, kind, E, k):
+    """Two picks that fp32 cannot tell apart and everyone else far below: exactly k candidates."""
+    torch = cuda
+    rng = np.random.default_rng(E)
+    l = np.full((2, E), -3.0, np.float32) + rng.standard_normal((2, E)).astype(np.float32) * 0.1
+    first = rng.permutation(E)[:k]
+    l[:, first] = 1.0 + 0.25 * np.arange(k, dtype=np.float32)
+    bias = np.zeros(E, np.float32)
+    held = scores64(kind, l[0].astype(np.float64)).astype(np.float32)
+    bias[first[0]] = held[first[1]] - held[first[0]]
+    logits, b = torch.from_numpy(l).cuda(), torch.from_numpy(bias).cuda()
+    ids, w = torch.empty((2, k), dtype=torch.int32, device="cuda"), torch.empty((2, k), device="cuda")
+    op = cb.ExpertRoute(E, k, score=kind)
+    op.run(logits, ids, w, d_bias=b)
+    check_route(torch, op, logits, b, ids, w, kind)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
 @pytest.mark.parametrize("mean", [-60.0, -14.0, -3.0, 9.0])
 def test_route_small_and_close_scores(cb, cuda, kind, mean):
     """Scores all tiny or all close to 1, and biases of the size of their last bits."""
