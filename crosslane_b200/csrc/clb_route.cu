@@ -62,6 +62,31 @@ __device__ __forceinline__ float score_f32(float l, float top, float sum) {
     if (KIND == CLB_SCORE_SOFTMAX) return __fdividef(exp_diff(l, top), sum);
     return sqrtf(fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))));
 }
+// The same for the ranks' comparison alone, where what counts is the error in units of the row's
+// largest score s(top) (u: half ulps), and a third of the instructions:
+// - sigmoid: e = __expf(-l) is within 4 + 2.4 |l| u, s = 1 / (1 + e) within (1 - s) (4 + 2.4 |l|) + 5;
+//   s |l| is at most 0.28 for l >= top >= -1.3, where s(top) >= 0.21, and else at most s(top) |top|:
+//   within (13 + 2.4 max(0, -top)) u s(top).
+// - sqrt(log(1 + e^l)), from log1p(e) = 2 atanh(z), z = e / (2 + e) <= 1/3, whose series to z^13 leaves
+//   (1/9)^7 / 15: for l < 0 the logarithm is within 4 + 2.4 |l| + 9 u, its root within half of that and
+//   2; s |l| is at most 0.72, s(-2) = 0.356: within (13 + 1.2 max(0, -top)) u s(top); l > 0 adds less.
+// - softmax: the sum's own terms, each within e^d (4 + 3.4 |d|) u <= 5.3 u, times 1 / sum (2 u) and
+//   rounded, over a sum within 65 u: within 74 u / sum.
+// A score that is flushed to 0 is below 2^-63.
+template <int KIND>
+__device__ __forceinline__ float score_rough(float l) {
+    if (KIND == CLB_SCORE_SIGMOID) return __fdividef(1.0f, 1.0f + __expf(-l));
+    const float e = __expf(-fabsf(l)), z = __fdividef(e, 2.0f + e), t = z * z;
+    float p = fmaf(t, 1.0f / 13.0f, 1.0f / 11.0f);
+    p = fmaf(p, t, 1.0f / 9.0f);
+    p = fmaf(p, t, 1.0f / 7.0f);
+    p = fmaf(p, t, 1.0f / 5.0f);
+    p = fmaf(p, t, 1.0f / 3.0f);
+    p = fmaf(p, t, 1.0f);
+    p = fmaf(z + z, p, fmaxf(l, 0.0f));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(p) : "f"(p));
+    return p;
+}
 template <int KIND>
 __device__ __noinline__ float score_exact(double l, double top, double sum) {
     if (KIND == CLB_SCORE_SIGMOID) return (float)(1.0 / (1.0 + exp(-l)));
@@ -85,9 +110,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // once; what bounds it is the latency of one warp's chain for few tokens and the issue slots
 // for many (about 400 instructions a token), so candidates for the picks are cut down by the
 // lanes' maxima and ranked by counting instead of k passes over the row. Measured on a B200
-// (device time): 1 x 384, sigmoid and bias, k 6: 3.4 us; 61 x 384 in 8 groups: 5.7 us; 2048 x
-// 384, sqrt-softplus and bias: 7.1 us; 16383 x 256 softmax, k 8: 11.6 us (1.6 TB/s). One pick
-// after the other with all scores in double took 9.9, 15, 19 and 45 us.
+// (device time): 1 x 384, sigmoid and bias, k 6: 3.0 us; 61 x 384 in 8 groups: 5.0 us; 2048 x
+// 384, sqrt-softplus and bias: 5.6 us (7.0 with expf, log1pf and a rounded root for the ranks);
+// 16383 x 256 softmax, k 8: 11.6 us (1.5 TB/s). One pick after the other with all scores in double
+// took 9.9, 15, 19 and 45 us.
 template <int NPL, int KIND, bool SCORED>
 __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 5 : 3) k_route_experts(const RouteArgs a) {
     __shared__ unsigned long long cand_s[kRouteWarps][32];                         // key, ~id
@@ -148,14 +174,17 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
     if (KIND == CLB_SCORE_SOFTMAX) {
         sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) sum += __expf(l[i] - top);
+        for (int i = 0; i < NPL; ++i) {
+            const float e = __expf(l[i] - top);
+            sum += e;
+            if (SCORED) vals_s[warp][32 * i + lane] = e;
+        }
         sum = ops_warp_sum(sum);
     }
-    // the largest error of a score (s rises with l), and of the scores below the normal numbers
-    const float off = !SCORED ? 0.0f
-                              : fmaf((KIND == CLB_SCORE_SOFTMAX ? 96.0f : 16.0f) * kHalfUlp,
-                                     KIND == CLB_SCORE_SOFTMAX ? __fdividef(1.0f, fmaxf(sum, 1.0f)) : score_f32<KIND>(top, 0.0f, 1.0f),
-                                     1e-18f);
+    // the largest error of a rough score, and of the scores below the normal numbers
+    float off = 0.0f;
+    if (SCORED && KIND == CLB_SCORE_SOFTMAX) off = fmaf(96.0f * kHalfUlp, __fdividef(1.0f, fmaxf(sum, 1.0f)), 1e-18f);
+    else if (SCORED) off = fmaf(fmaf(fmaxf(-top, 0.0f), 2.5f, 16.0f) * kHalfUlp, score_rough<KIND>(top), 1e-18f);
 
     uint32_t mine = 0;      // lane j: the key and id of the j-th largest rank
     int id = 0;
@@ -166,8 +195,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         uint32_t key[NPL];
         if (SCORED) {
             if (!exact) {
+                if (KIND != CLB_SCORE_SOFTMAX)
 #pragma unroll
-                for (int i = 0; i < NPL; ++i) vals_s[warp][32 * i + lane] = score_f32<KIND>(l[i], top, sum);
+                    for (int i = 0; i < NPL; ++i) vals_s[warp][32 * i + lane] = score_rough<KIND>(l[i]);
             } else {  // rare: nothing kept in registers for it
                 double dsum = 1.0;
                 if (KIND == CLB_SCORE_SOFTMAX) {
@@ -184,12 +214,14 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
                     vals_s[warp][e] = score_exact<KIND>(ops_load(a.logits, a.type, row + e), top, dsum);
             }
         }
+        const float by = KIND != CLB_SCORE_SOFTMAX || exact ? 1.0f : __fdividef(1.0f, sum);
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
             const int e = 32 * i + lane;
             float v = l[i];
             if (SCORED) {
-                const float sc = __fadd_rn(vals_s[warp][e], b[i]);  // without a bias b is 0
+                // without a bias b is 0
+                const float sc = __fadd_rn(KIND == CLB_SCORE_SOFTMAX ? __fmul_rn(vals_s[warp][e], by) : vals_s[warp][e], b[i]);
                 const bool there = l[i] > -INFINITY && b[i] > -INFINITY;
                 v = !there ? -INFINITY : a.bias ? sc : l[i];
                 if (a.groups > 1) vals_s[warp][e] = there ? sc : -INFINITY;
