@@ -84,7 +84,7 @@ __host__ __device__ constexpr NormTypes norm_types(int set) {
 // 11.5 us; 1200 x 1024 fp32 / bf16 3.9 and 5.5 us; 2000 x 1024 5.7 and 5.9 us),
 // rows that are not aligned, and rows too wide for k_block_norm_rows. Bound by the latency of the
 // loads and the two sums. Measured on a B200 (device time): 1 x 7168 fp32 3.2 us, 64 x 7168
-// 3.6 us, 777 x 2311 in rows of 2316 elements 6.9 us (3.1 TB/s).
+// 3.6 us, 777 x 2311 in rows of 2316 elements 6.8 us (3.2 TB/s).
 template <int CH, bool VEC, int SET>
 __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
@@ -162,16 +162,17 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 // a full gate into shared memory while one is worked on, so that HBM is busy all the time;
 // what all rows share (w_post times the channels' gate, w_pre) stays in registers (from L1 it
 // cost 72 us for 42). A row's shared memory is asked for again as soon as the CTA has read it.
-// The instructions a thread spends on the two sums are as many as on 20 values, so it takes 4
-// chunks where the rows have them, and several CTAs an SM hide the sums' latency. Measured on
-// a B200 (device time): 2048 x 7168 fp32 42.4 us (5.5 TB/s), 8192 x 5120 bf16 with a sigmoid
-// gate 66.5 us (6.3 TB/s, 96 % of a copy's rate); a CTA per row took 65 and 138 us.
+// The instructions a thread spends on the two sums are as many as on 20 values, so it takes
+// several chunks where the rows have them, several CTAs an SM hide the sums' latency, and the
+// arithmetic is done in pairs. Measured on a B200 (device time): 2048 x 7168 fp32 38.9 us (6.0
+// TB/s), 8192 x 5120 bf16 with a sigmoid gate 67 us (6.25 TB/s, 96 % of a copy's rate); a CTA per
+// row took 65 and 138 us.
 constexpr int kRowStages = 2;
 constexpr uint32_t kRowPolls = 1u << 20;  // waits for a copy, each with a suspend hint of 20 us
 
 // The gates of two values. FAST: exp2 of the scaled argument and a reciprocal, the instructions
 // alone: off by at most (|g| + 8) half ulps of fp32, far below a half step of the 16-bit types
-// that the call's results are rounded to (8192 x 5120 in a stream: 75 us with expf).
+// that the call's results are rounded to (8192 x 5120 in a stream: 75 us with expf, 70 us so).
 template <bool FAST>
 __device__ __forceinline__ F2 gate2(F2 g, int sigmoid) {
     if (!sigmoid) return g;

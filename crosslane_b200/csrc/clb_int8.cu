@@ -268,8 +268,10 @@ __device__ __forceinline__ float int8_value(int acc, float xs, float ws, float b
 // by itself into shared memory (x comes from L2; floating x) or copies q (int8 x). A CTA has
 // `rows` weight rows, cut into 2^log_segs pieces of K that its warps share out; a piece's sums
 // are integers, added in shared memory in any order. Measured on a B200 (device time, weights
-// in part from L2): 1 token, fp32: 7168 x 1536 4.4 us (2.5 TB/s), 7168 x 7168 13 us (3.9 TB/s);
-// from 5 tokens on the tensor-core tiles are as fast (7168 x 7168: 17 us either way).
+// in part from L2), fp32 x: 1 token, 7168 x 1536 4.4 us (2.5 TB/s), 7168 x 7168 7.8 us; 4 tokens,
+// 512 x 1024 3.8 us, 7168 x 7168 13.8 us (5.7 and 16.3 us with one token quantised after the
+// other). 8 tokens took 4.3 us for the tiles' 5.2 at 512 x 1024, but 8.9 for 7.5 at 4096 x 2304 and
+// 24 for 13 at 7168 x 7168.
 constexpr int kDotThreads = 1024;
 constexpr int kDotAhead = 4;                 // 16-byte weight pieces of a lane's group, two groups in flight
 constexpr int kDotSmem = 160 * 1024;         // largest tokens * pitch that is staged
@@ -433,10 +435,10 @@ void (*dot_kernel(int tt, bool vec, int type))(Int8Dot) {
 //  * kSplit: the CTAs of a cluster share one tile's K range, for products with few tiles; each
 //    sends its sums to the CTA that owns the tokens, which adds them up (integers: the order
 //    does not matter).
-// Bound by the tensor pipe for large products (90 % active at 4096 x 7168 x 7168; 139 us = 3.0
-// POP/s for a burst, 154 us at the power cap's clock), by the loads from L2 (about 100 bytes per ns
-// and SM) and the stores for shallow ones (2047 x 1536 x 7168 into fp32: 27 us, 49 % active), and
-// by the chain launch - quantise - load - join for small ones (64 x 5120 x 2304: 8.3 us).
+// Bound by the tensor pipe for large products (90 % active at 4096 x 7168 x 7168; 135 us = 3.1
+// POP/s for a burst, 150 us at the power cap's clock), by the loads from L2 (about 100 bytes per ns
+// and SM) and the stores for shallow ones (2047 x 1536 x 7168 into fp32: 26 us, 49 % active), and
+// by the chain launch - quantise - load - join for small ones (64 x 5120 x 2304: 8.2 us).
 enum : int { kSingle = 0, kPair = 1, kSplit = 2 };
 constexpr int kGmEpiWarps = 8, kGmLoadWarp = kGmEpiWarps, kGmMmaWarp = kGmEpiWarps + 1;
 constexpr int kGmThreads = 32 * (kGmEpiWarps + 2);
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     const int64_t total = (int64_t)my_tiles * nkb;
     const int tile_rows = PAIR ? 256 : 128, brows = PAIR ? g.nt / 2 : g.nt;
     const uint32_t stage_bytes = (uint32_t)kGmABytes + (uint32_t)brows * 128u;
-    // neighbours share the weights' rows (the other order: 143 us for 139 at 4096 x 7168 x 7168)
+    // neighbours share the weights' rows (the other order: 143 us for 135 at 4096 x 7168 x 7168)
     auto row_of = [&](int tile) { return (tile / g.ntiles) * tile_rows + (PAIR ? 128 * rank : 0); };
     auto token_of = [&](int tile) { return (tile % g.ntiles) * g.nt; };
 
