@@ -17,7 +17,8 @@
 namespace clb {
 namespace {
 
-constexpr int kInt8MaxK = 131072;  // 127 * 127 * k stays below 2^31
+constexpr int kInt8MaxK = 131072;  // 127 * 128 * k stays below 2^31
+constexpr int kInt8MaxRows = 1 << 30;  // weight rows, tokens: their tiles are counted in int
 constexpr int kErrInt8Wait = 3;
 
 // The exactly rounded quotient; `inv` the fp32 reciprocal of scale.
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
                 // SPLIT: where the sums of token c go
                 int owner = SPLIT ? c0 / share : 0, off = SPLIT ? c0 % share : 0;
                 auto send_to = [&] { return cluster_addr(red + (uint32_t)((rank * share + off) * 128 + (tid & 127)) * 4u, owner); };
-                uint32_t to = SPLIT ? send_to() : 0u;
+                uint32_t to = SPLIT && c0 < c1 ? send_to() : 0u;
                 auto take = [&](const int (&r)[16], int c) {
                     if (SPLIT) {
 #pragma unroll
@@ -1058,7 +1059,8 @@ extern "C" int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, 
         require(cfg != nullptr, CLB_E_INVALID, "null int8 linear config");
         const clb_int8_linear_config_v1 c = *cfg;
         const bool ready = c.x_type == CLB_I8;
-        require(c.n >= 1 && c.k >= 1 && c.k <= clb::kInt8MaxK, CLB_E_INVALID, "n >= 1 and k in 1..%d", clb::kInt8MaxK);
+        require(c.n >= 1 && c.n <= clb::kInt8MaxRows && c.k >= 1 && c.k <= clb::kInt8MaxK, CLB_E_INVALID,
+                "n in 1..%d and k in 1..%d", clb::kInt8MaxRows, clb::kInt8MaxK);
         require((ready || clb::ops_float_type(c.x_type)) && clb::ops_float_type(c.out_type), CLB_E_INVALID,
                 "x is fp32, bf16, fp16 or int8; out is fp32, bf16 or fp16");
         require(c.ld_w >= c.k && c.ld_w % 16 == 0, CLB_E_INVALID, "ld_w is a multiple of 16, at least k");
@@ -1066,7 +1068,7 @@ extern "C" int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, 
                 "ld_x is at least k (a multiple of 16 for int8)");
         require(c.ld_out >= c.n, CLB_E_INVALID, "ld_out below n");
         for (int i = 0; i < 4; ++i) require(!c.reserved[i], CLB_E_INVALID, "reserved fields must be 0");
-        require(tokens >= 0, CLB_E_INVALID, "negative token count");
+        require(tokens >= 0 && tokens <= clb::kInt8MaxRows, CLB_E_INVALID, "token count not in 0..%d", clb::kInt8MaxRows);
         if (tokens == 0) return;
         require(d_w && d_w_scale && d_x && d_out, CLB_E_INVALID, "null pointer argument");
         require(ready == (d_x_scale != nullptr), CLB_E_INVALID, "x_scale goes with int8 x");

@@ -564,7 +564,7 @@ int32_t clb_int8_quantize_device(int32_t type, const void* d_x, int64_t ld_x, in
                                  int64_t ld_q, float* d_scale, void* stream, clb_error_v1* err);
 
 typedef struct clb_int8_linear_config_v1 {
-    int32_t n, k;              /* weight matrix [n][k]; k <= 131072 */
+    int32_t n, k;              /* weight matrix [n][k]; n <= 2^30, k <= 131072 */
     int32_t x_type;            /* CLB_F32, CLB_BF16, CLB_F16 (quantised by the call) or CLB_I8 */
     int32_t out_type;          /* CLB_F32, CLB_BF16 or CLB_F16 */
     int64_t ld_w, ld_x, ld_out;/* row pitches; ld_w (and ld_x for CLB_I8) a multiple of 16 */

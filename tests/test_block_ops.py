@@ -103,6 +103,13 @@ def test_linear_refusals(kw):
             a["x_scale"], a["out"], a["ws"], a["ws_bytes"], a["status"])
 
 
+@pytest.mark.parametrize("kw", [dict(n=(1 << 30) + 1, ld_out=(1 << 30) + 1), dict(n=2 ** 31 - 1, ld_out=2 ** 31 - 1),
+                                dict(tokens=(1 << 30) + 1), dict(tokens=2 ** 31 - 1)])
+def test_linear_refuses_more_rows_than_it_counts(kw):
+    cfg = Int8LinearConfigV1(**{**dict(n=32, k=16, ld_w=16, ld_x=16, ld_out=32), **{k: v for k, v in kw.items() if k != "tokens"}})
+    refused(lib.clb_int8_linear_device, C.byref(cfg), A, A, None, kw.get("tokens", 4), A, None, A, A, 1 << 62, None)
+
+
 def test_zero_tokens_are_no_work():
     err = ErrorV1()
     for fn, *args in (route(tokens=0, logits=None, ids=None, w=None),
