@@ -36,20 +36,40 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
     return ops_warp_sum(lane < nw ? part[lane] : 0.0f);
 }
 
-// Eight values of a thread's chunk c. VEC: 8 contiguous elements, 16-byte accesses. Otherwise
-// the elements are blockDim apart, so that a warp's scalar accesses stay contiguous.
-template <bool VEC>
+// Eight values of a thread's chunk c. W 8: 8 contiguous elements, 16- and 32-byte accesses. W 4: two
+// fours, blockDim fours apart (the up to 3 elements behind the last whole four are single values of
+// the first threads). W 1: elements, blockDim apart. So a warp's accesses are contiguous in each.
+template <int W>
 __device__ __forceinline__ Raw8 load8(const void* p, int type, int64_t row, int c, int dim) {
-    const void* r = static_cast<const char*>(p) + row * (type == CLB_F32 ? 4 : 2);
+    const char* r = static_cast<const char*>(p) + row * (type == CLB_F32 ? 4 : 2);
     const int nt = blockDim.x, tid = threadIdx.x;
-    return VEC ? raw8_aligned(r, type, 8 * (int64_t)(tid + c * nt), tid + c * nt < dim >> 3)
-               : raw8_strided(r, type, 8 * (int64_t)c * nt + tid, nt, dim);
+    if (W == 8) return raw8_aligned(r, type, 8 * (int64_t)(tid + c * nt), tid + c * nt < dim >> 3);
+    if (W == 1) return raw8_strided(r, type, 8 * (int64_t)c * nt + tid, nt, dim);
+    Raw8 v{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    const int i = 2 * c * nt + tid, j = i + nt, n = dim >> 2;
+    ld16_if(v.a, r + 16 * (int64_t)i, i < n && type == CLB_F32);
+    ld16_if(v.b, r + 16 * (int64_t)j, j < n && type == CLB_F32);
+    ld8_if(v.a.x, v.a.y, r + 8 * (int64_t)i, i < n && type != CLB_F32);
+    ld8_if(v.a.z, v.a.w, r + 8 * (int64_t)j, j < n && type != CLB_F32);
+    return v;
 }
-template <bool VEC>
+template <int W>
 __device__ __forceinline__ void store8(void* p, int type, int64_t row, int c, int dim, const float (&v)[8]) {
     const int nt = blockDim.x, tid = threadIdx.x;
-    if (VEC) {
+    if (W == 8) {
         if (tid + c * nt < dim >> 3) store8_aligned(p, type, row + 8 * (int64_t)(tid + c * nt), v);
+    } else if (W == 4) {
+        const int i = 2 * c * nt + tid, j = i + nt, n = dim >> 2;
+        if (type == CLB_F32) {
+            float4* r = reinterpret_cast<float4*>(static_cast<float*>(p) + row);
+            if (i < n) r[i] = make_float4(v[0], v[1], v[2], v[3]);
+            if (j < n) r[j] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint2* r = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + row);
+            const uint4 w = pack8(type, v);
+            if (i < n) r[i] = make_uint2(w.x, w.y);
+            if (j < n) r[j] = make_uint2(w.z, w.w);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -84,8 +104,9 @@ __host__ __device__ constexpr NormTypes norm_types(int set) {
 // 11.5 us; 1200 x 1024 fp32 / bf16 3.9 and 5.5 us; 2000 x 1024 5.7 and 5.9 us),
 // rows that are not aligned, and rows too wide for k_block_norm_rows. Bound by the latency of the
 // loads and the two sums. Measured on a B200 (device time): 1 x 7168 fp32 3.2 us, 64 x 7168
-// 3.6 us, 777 x 2311 in rows of 2316 elements 6.8 us (3.2 TB/s).
-template <int CH, bool VEC, int SET>
+// 3.6 us, 777 x 2311 fp32 / fp16 in rows of 2316 elements 5.0 us (4.3 TB/s; 6.8 element by element,
+// the way of rows of no such pitch), 2000 x 2311 bf16 12.5 and 20 us.
+template <int CH, int W, int SET>
 __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
     const int x_type = SET ? norm_types(SET).other : a.x_type;
@@ -94,22 +115,32 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     const int64_t row = blockIdx.x;
     const bool wide_gate = a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL;
     Raw8 yr[CH], hr[CH], gr[CH];
+    // W 4: the element behind the whole fours that is this thread's, as it lies in memory
+    const int last = (a.dim & ~3) + threadIdx.x;
+    const bool tail = W == 4 && last < a.dim;
+    uint32_t y1 = 0, h1 = 0, g1 = 0;
     float v[CH][8];
     if (a.y)
 #pragma unroll
-        for (int c = 0; c < CH; ++c) yr[c] = load8<VEC>(a.y, y_type, row * a.ld_y, c, a.dim);
+        for (int c = 0; c < CH; ++c) yr[c] = load8<W>(a.y, y_type, row * a.ld_y, c, a.dim);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) hr[c] = load8<VEC>(a.h, h_type, row * a.ld_h, c, a.dim);
-    if (CH == 1 && wide_gate) gr[0] = load8<VEC>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, 0, a.dim);
+    for (int c = 0; c < CH; ++c) hr[c] = load8<W>(a.h, h_type, row * a.ld_h, c, a.dim);
+    if (W == 4) {
+        ld_elem_if(y1, a.y, y_type, row * a.ld_y + last, tail && a.y);
+        ld_elem_if(h1, a.h, h_type, row * a.ld_h + last, tail);
+        ld_elem_if(g1, a.gate, a.gate_type, (a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0) + last, tail && wide_gate);
+    }
+    float v1 = elem_float(h1, h_type);
+    if (CH == 1 && wide_gate) gr[0] = load8<W>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, 0, a.dim);
     if (a.y) {
         float gt = 1.0f;
         if (a.gate_kind == CLB_GATE_TOKEN) gt = gate_value(ops_load(a.gate, a.gate_type, row), a.gate_sigmoid);
         float inv = 1.0f;
         if (a.post) {
-            float ss = 0.0f, y[8];
+            float ss = elem_float(y1, y_type) * elem_float(y1, y_type), y[8];
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                raw8_floats(yr[c], y_type, VEC, y);
+                raw8_floats(yr[c], y_type, W > 1, y);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
             }
@@ -119,29 +150,36 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             float y[8], w[8];
-            raw8_floats(yr[c], y_type, VEC, y);
+            raw8_floats(yr[c], y_type, W > 1, y);
             if (a.w_post) {
-                raw8_floats(load8<VEC>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, VEC, w);
+                raw8_floats(load8<W>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, W > 1, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] *= w[j];
             }
             if (wide_gate) {
-                if (CH > 1) gr[c] = load8<VEC>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, c, a.dim);
-                raw8_floats(gr[c], a.gate_type, VEC, w);
+                if (CH > 1) gr[c] = load8<W>(a.gate, a.gate_type, a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0, c, a.dim);
+                raw8_floats(gr[c], a.gate_type, W > 1, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] *= gate_value(w[j], a.gate_sigmoid);
             }
-            raw8_floats(hr[c], h_type, VEC, v[c]);
+            raw8_floats(hr[c], h_type, W > 1, v[c]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[c][j] = fmaf(f, y[j], a.residual_scale * v[c][j]);
-            store8<VEC>(a.h_out, h_type, row * a.ld_h_out, c, a.dim, v[c]);
+            store8<W>(a.h_out, h_type, row * a.ld_h_out, c, a.dim, v[c]);
+        }
+        if (tail) {
+            float y = elem_float(y1, y_type);
+            if (a.w_post) y *= a.w_post[last];
+            if (wide_gate) y *= gate_value(elem_float(g1, a.gate_type), a.gate_sigmoid);
+            v1 = fmaf(f, y, a.residual_scale * v1);
+            ops_store(a.h_out, h_type, row * a.ld_h_out + last, v1);
         }
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) raw8_floats(hr[c], h_type, VEC, v[c]);
+        for (int c = 0; c < CH; ++c) raw8_floats(hr[c], h_type, W > 1, v[c]);
     }
     if (a.x) {
-        float ss = 0.0f;
+        float ss = tail ? v1 * v1 : 0.0f;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -150,11 +188,12 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             float w[8];
-            if (a.w_pre) raw8_floats(load8<VEC>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, VEC, w);
+            if (a.w_pre) raw8_floats(load8<W>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, W > 1, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = a.w_pre ? w[j] * (v[c][j] * inv) : v[c][j] * inv;
-            store8<VEC>(a.x, x_type, row * a.ld_x, c, a.dim, w);
+            store8<W>(a.x, x_type, row * a.ld_x, c, a.dim, w);
         }
+        if (tail) ops_store(a.x, x_type, row * a.ld_x + last, a.w_pre ? a.w_pre[last] * (v1 * inv) : v1 * inv);
     }
 }
 
@@ -256,10 +295,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) k_block_norm_rows(const NormArg
         float p[8], q[8], g[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[j] = q[j] = 1.0f;
-        if (a.w_post) raw8_floats(load8<true>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, true, p);
-        if (a.w_pre) raw8_floats(load8<true>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, true, q);
+        if (a.w_post) raw8_floats(load8<8>(a.w_post, CLB_F32, 0, c, a.dim), CLB_F32, true, p);
+        if (a.w_pre) raw8_floats(load8<8>(a.w_pre, CLB_F32, 0, c, a.dim), CLB_F32, true, q);
         if (a.gate_kind == CLB_GATE_CHANNEL) {
-            raw8_floats(load8<true>(a.gate, a.gate_type, 0, c, a.dim), a.gate_type, true, g);
+            raw8_floats(load8<8>(a.gate, a.gate_type, 0, c, a.dim), a.gate_type, true, g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[j] *= gate_value(g[j], a.gate_sigmoid);
         }
@@ -364,23 +403,25 @@ decltype(rows_kernel<kTypesAny>(0, 0)) rows_kernel(int set, int ch, int threads)
                                   : rows_kernel<kTypesAny>(ch, threads);
 }
 
-template <int SET>
-void (*row_kernel(int ch, bool vec))(NormArgs) {
-    return vec ? (ch == 1 ? k_block_norm<1, true, SET> : ch == 2 ? k_block_norm<2, true, SET> : k_block_norm<4, true, SET>)
-               : (ch == 1   ? k_block_norm<1, false, SET>
-                  : ch == 2 ? k_block_norm<2, false, SET>
-                            : k_block_norm<4, false, SET>);
+template <int W, int SET>
+void (*row_kernel(int ch))(NormArgs) {
+    return ch == 1 ? k_block_norm<1, W, SET> : ch == 2 ? k_block_norm<2, W, SET> : k_block_norm<4, W, SET>;
 }
-void (*row_kernel(int set, int ch, bool vec))(NormArgs) {
-    return set == kTypesF32       ? row_kernel<kTypesF32>(ch, vec)
-           : set == kTypesBF16    ? row_kernel<kTypesBF16>(ch, vec)
-           : set == kTypesF16     ? row_kernel<kTypesF16>(ch, vec)
-           : set == kTypesF32BF16 ? row_kernel<kTypesF32BF16>(ch, vec)
-           : set == kTypesF32F16  ? row_kernel<kTypesF32F16>(ch, vec)
-                                  : row_kernel<kTypesAny>(ch, vec);
+template <int SET>
+void (*row_kernel(int ch, int width))(NormArgs) {
+    return width == 8 ? row_kernel<8, SET>(ch) : width == 4 ? row_kernel<4, SET>(ch) : row_kernel<1, SET>(ch);
+}
+void (*row_kernel(int set, int ch, int width))(NormArgs) {
+    return set == kTypesF32       ? row_kernel<kTypesF32>(ch, width)
+           : set == kTypesBF16    ? row_kernel<kTypesBF16>(ch, width)
+           : set == kTypesF16     ? row_kernel<kTypesF16>(ch, width)
+           : set == kTypesF32BF16 ? row_kernel<kTypesF32BF16>(ch, width)
+           : set == kTypesF32F16  ? row_kernel<kTypesF32F16>(ch, width)
+                                  : row_kernel<kTypesAny>(ch, width);
 }
 
-cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStream_t s) {
+// width: elements that every row's accesses may take at a time (8 also divides dim then).
+cudaError_t launch_block_norm(const NormArgs& a, int tokens, int width, cudaStream_t s) {
     const int units = (a.dim + 7) / 8;
     const uint32_t y_bytes = a.y ? a.dim * ops_type_bytes(a.y_type) : 0, h_bytes = a.dim * ops_type_bytes(a.h_type);
     const uint32_t g_bytes = a.gate_kind == CLB_GATE_FULL ? a.dim * ops_type_bytes(a.gate_type) : 0;
@@ -392,7 +433,7 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStrea
             (!g_bytes || a.gate_type == t.other))
             set = i;
     }
-    if (vec && (int64_t)tokens * units > kNormManyChunks && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
+    if (width == 8 && (int64_t)tokens * units > kNormManyChunks && units <= 2048 && 2 * stage <= (uint32_t)kRowSmem) {
         // Two rows in flight for each CTA, and as many CTAs as bring that to 104 KB an SM, or two up to 132 KB:
         // with more, reads and writes get into each other's way in HBM (8192 x 5120 bf16, gate: 66.6 us
         // with 123 KB, 76 us with 184 KB; 8192 x 2048 fp32 / bf16: 35.0 us with 98 KB, 38.9 us with 123
@@ -423,7 +464,7 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, bool vec, cudaStrea
     }
     const int ch = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
     const int threads = std::max(32, ((units + ch - 1) / ch + 31) / 32 * 32);
-    void (*kernel)(NormArgs) = row_kernel(set, ch, vec);
+    void (*kernel)(NormArgs) = row_kernel(set, ch, width);
     return ops_launch(kernel, (unsigned)tokens, threads, 0, s, a);
 }
 
@@ -466,19 +507,23 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
                                {d_h_out, c.h_type, c.ld_h_out, "h_out"}, {d_x, c.x_type, c.ld_x, "x"}};
         const Tensor vecs[] = {{full ? nullptr : d_gate, c.gate_type, 0, "gate"}, {d_w_post, CLB_F32, 0, "w_post"},
                                {d_w_pre, CLB_F32, 0, "w_pre"}};
-        bool vec = c.dim % 8 == 0;
+        // the widest accesses that every tensor's alignment allows
+        int width = c.dim % 8 == 0 ? 8 : 4;
+        auto narrow = [&](const void* p, int type, int64_t ld) {
+            while (width > 1 && (!clb::ops_aligned(p, width * clb::ops_type_bytes(type)) || ld % width)) width = width == 8 ? 4 : 1;
+        };
         for (const Tensor& t : rows) {
             if (!t.p) continue;
             const size_t b = clb::ops_type_bytes(t.type);
             require(t.ld >= c.dim && t.ld <= (int64_t)1 << 40, CLB_E_INVALID, "row pitch of %s below dim", t.name);
             require(clb::ops_aligned(t.p, b), CLB_E_INVALID, "%s is misaligned", t.name);
-            vec = vec && clb::ops_vec8(t.p, t.type, t.ld);
+            narrow(t.p, t.type, t.ld);
         }
         for (const Tensor& t : vecs) {
             if (!t.p) continue;
             require(clb::ops_aligned(t.p, clb::ops_type_bytes(t.type)), CLB_E_INVALID, "%s is misaligned", t.name);
             // a gate for each token is read one number at a time
-            if (t.p != d_gate || c.gate == CLB_GATE_CHANNEL) vec = vec && clb::ops_vec8(t.p, t.type, 0);
+            if (t.p != d_gate || c.gate == CLB_GATE_CHANNEL) narrow(t.p, t.type, 0);
         }
         // an output over an input: only h_out in h's place, row by row
         const Tensor outs[] = {rows[3], rows[4]};
@@ -511,7 +556,7 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
         a.gate_kind = d_gate ? c.gate : CLB_GATE_NONE, a.gate_sigmoid = c.gate_sigmoid, a.post = c.post;
         a.post_eps = c.post_eps, a.pre_eps = c.pre_eps, a.residual_scale = c.residual_scale;
         a.block_scale = c.block_scale, a.inv_dim = 1.0f / (float)c.dim;
-        cuda_check(clb::launch_block_norm(a, tokens, vec, static_cast<cudaStream_t>(stream)),
+        cuda_check(clb::launch_block_norm(a, tokens, width, static_cast<cudaStream_t>(stream)),
                    "block norm");
     });
 }

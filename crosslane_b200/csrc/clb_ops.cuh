@@ -60,6 +60,16 @@ __device__ __forceinline__ void ld_elem_if(uint32_t& v, const void* row, int typ
         : "+r"(v)
         : "l"(p), "r"((uint32_t)(ok && type == CLB_F32)), "r"((uint32_t)(ok && type != CLB_F32)));
 }
+__device__ __forceinline__ void ld8_if(uint32_t& a, uint32_t& b, const void* p, bool ok) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
+                 : "+r"(a), "+r"(b)
+                 : "l"(p), "r"((uint32_t)ok));
+}
+__device__ __forceinline__ float elem_float(uint32_t v, int type) {
+    return type == CLB_F32    ? __uint_as_float(v)
+           : type == CLB_BF16 ? __uint_as_float(v << 16)
+                              : __half2float(__ushort_as_half((uint16_t)v));
+}
 // Aligned (ops_vec8): elements i .. i + 7 of `row`, where ok; zeros otherwise.
 __device__ __forceinline__ Raw8 raw8_aligned(const void* row, int type, int64_t i, bool ok) {
     Raw8 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -130,14 +140,8 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
     return v;
 }
 
-// Eight elements from i on, aligned as for raw8_aligned.
-__device__ __forceinline__ void store8_aligned(void* p, int type, int64_t i, const float (&v)[8]) {
-    if (type == CLB_F32) {
-        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<float*>(p) + i), "f"(v[0]),
-                     "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-                     : "memory");
-        return;
-    }
+// Eight values as four pairs of a 16-bit type.
+__device__ __forceinline__ uint4 pack8(int type, const float (&v)[8]) {
     uint32_t w[4];
     if (type == CLB_BF16) {
 #pragma unroll
@@ -152,7 +156,17 @@ __device__ __forceinline__ void store8_aligned(void* p, int type, int64_t i, con
             w[j] = *reinterpret_cast<const uint32_t*>(&b);
         }
     }
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Eight elements from i on, aligned as for raw8_aligned.
+__device__ __forceinline__ void store8_aligned(void* p, int type, int64_t i, const float (&v)[8]) {
+    if (type == CLB_F32) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<float*>(p) + i), "f"(v[0]),
+                     "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+        return;
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = pack8(type, v);
 }
 
 // Rows that start anywhere, through shared memory: byte j of the row lies at `smem` + (address mod 16)

@@ -444,6 +444,43 @@ def test_norm_rows_that_start_anywhere(cb, cuda, T, D, h_t, y_t):
     check_norm(torch, n64(x), xw, (rh, bz), D, y_t, (np.abs(xw) / np.maximum(np.abs(new), 1e-300), new))
 
 
+@pytest.mark.parametrize("D", [1, 2, 3, 4, 5, 7, 12, 30, 127, 1001, 1002, 1003, 2311, 8190, 8191, 9001, 16387, 20002, 32765])
+@pytest.mark.parametrize("h_t,y_t,x_t", [("float32", "float32", "float32"), ("bfloat16", "bfloat16", "bfloat16"),
+                                         ("float32", "float16", "float16"), ("float16", "float32", "bfloat16")])
+def test_norm_rows_of_whole_fours(cb, cuda, D, h_t, y_t, x_t):
+    """Rows that start at a multiple of four elements but not of eight; widths with 0 to 3 behind the last four."""
+    pad = -D % 8 + 4
+    run_norm(cb, cuda, 3, D, h_t, y_t, x_t, gate="full", sig=True, pad=pad, seed=4)
+    run_norm(cb, cuda, 2, D, h_t, y_t, x_t, gate="channel", pad=pad, seed=5, in_place=True)
+    run_norm(cb, cuda, 2, D, h_t, y_t, x_t, pad=pad, post=False, weights=False, seed=6)
+    run_norm(cb, cuda, 2, D, h_t, y_t, x_t, pad=pad, pre=False, gate="token", seed=7)
+    run_norm(cb, cuda, 2, D, h_t, y_t, x_t, pad=pad, post=False, with_y=False, seed=8)
+    if D <= 2311:
+        run_norm(cb, cuda, 700, D, h_t, y_t, x_t, gate="full", pad=pad, seed=9)
+
+
+@pytest.mark.parametrize("T,D", [(3, 1024), (400, 1026), (5, 4)])
+@pytest.mark.parametrize("h_t,y_t", [("float32", "bfloat16"), ("bfloat16", "bfloat16"), ("float16", "float32")])
+def test_norm_rows_that_start_at_fours(cb, cuda, T, D, h_t, y_t):
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    dt = lambda n: getattr(torch, n)  # noqa: E731
+    pitch = (D + 3) // 4 * 4 + 12
+    at = lambda t, n: torch.randn((T, pitch), generator=gen, device="cuda").to(dt(t))[:, n:n + D]  # noqa: E731
+    h, y, g, out, x = at(h_t, 4), at(y_t, 12), at(y_t, 0), at(h_t, 8), at(y_t, 4)
+    before = x._base.clone()
+    wide = torch.randn(D + 4, generator=gen, device="cuda")
+    w_post, w_pre = wide[4:], wide[:D]
+    cb.BlockNorm(D, eps=1e-5, gate="full").run(h, d_y=y, d_gate=g, d_w_post=w_post, d_w_pre=w_pre, d_h_out=out, d_x=x)
+    n64 = lambda t: t.double().cpu().numpy()  # noqa: E731
+    new, xw, rh, bz = norm64(n64(h), n64(y), n64(g), n64(w_post), n64(w_pre), True, "full", False, 1.0, 1.0, 1e-5)
+    check_norm(torch, n64(out), new, (rh, bz), D, h_t)
+    check_norm(torch, n64(x), xw, (rh, bz), D, y_t, (np.abs(xw) / np.maximum(np.abs(new), 1e-300), new))
+    keep = torch.ones(pitch, dtype=torch.bool, device="cuda")
+    keep[4:4 + D] = False
+    assert torch.equal(x._base[:, keep], before[:, keep])
+
+
 @pytest.mark.parametrize("T", [1, 7, 500])
 @pytest.mark.parametrize("D", [64, 100, 1024])
 def test_norm_parts_of_one_buffer(cb, cuda, T, D):
