@@ -36,9 +36,9 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
     return ops_warp_sum(lane < nw ? part[lane] : 0.0f);
 }
 
-// Eight values of a thread's chunk c. W 8: 8 contiguous elements, 16- and 32-byte accesses. W 4: two
-// fours, blockDim fours apart (the up to 3 elements behind the last whole four are single values of
-// the first threads). W 1: elements, blockDim apart. So a warp's accesses are contiguous in each.
+// Eight values of a thread's chunk c. W 8: 8 contiguous elements, 16- and 32-byte accesses. W 4, 2: two
+// fours or four pairs, blockDim of them apart (the elements behind the last whole one are single
+// values of the first threads). W 1: elements, blockDim apart. So a warp's accesses are contiguous.
 template <int W>
 __device__ __forceinline__ Raw8 load8(const void* p, int type, int64_t row, int c, int dim) {
     const char* r = static_cast<const char*>(p) + row * (type == CLB_F32 ? 4 : 2);
@@ -46,6 +46,19 @@ __device__ __forceinline__ Raw8 load8(const void* p, int type, int64_t row, int 
     if (W == 8) return raw8_aligned(r, type, 8 * (int64_t)(tid + c * nt), tid + c * nt < dim >> 3);
     if (W == 1) return raw8_strided(r, type, 8 * (int64_t)c * nt + tid, nt, dim);
     Raw8 v{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (W == 2) {
+        uint32_t w[8] = {};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = (4 * c + k) * nt + tid;
+            const bool ok = i < dim >> 1;
+            uint32_t pair = 0;
+            ld8_if(w[2 * k], w[2 * k + 1], r + 8 * (int64_t)i, ok && type == CLB_F32);
+            ld4_if(pair, r + 4 * (int64_t)i, ok && type != CLB_F32);
+            if (type != CLB_F32) (&v.a.x)[k] = pair;
+        }
+        return type == CLB_F32 ? Raw8{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])} : v;
+    }
     const int i = 2 * c * nt + tid, j = i + nt, n = dim >> 2;
     ld16_if(v.a, r + 16 * (int64_t)i, i < n && type == CLB_F32);
     ld16_if(v.b, r + 16 * (int64_t)j, j < n && type == CLB_F32);
@@ -69,6 +82,15 @@ __device__ __forceinline__ void store8(void* p, int type, int64_t row, int c, in
             const uint4 w = pack8(type, v);
             if (i < n) r[i] = make_uint2(w.x, w.y);
             if (j < n) r[j] = make_uint2(w.z, w.w);
+        }
+    } else if (W == 2) {
+        const uint4 packed = pack8(type, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = (4 * c + k) * nt + tid;
+            if (i >= dim >> 1) continue;
+            if (type == CLB_F32) reinterpret_cast<float2*>(static_cast<float*>(p) + row)[i] = make_float2(v[2 * k], v[2 * k + 1]);
+            else reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + row)[i] = (&packed.x)[k];
         }
     } else {
 #pragma unroll
@@ -104,8 +126,9 @@ __host__ __device__ constexpr NormTypes norm_types(int set) {
 // 11.5 us; 1200 x 1024 fp32 / bf16 3.9 and 5.5 us; 2000 x 1024 5.7 and 5.9 us),
 // rows that are not aligned, and rows too wide for k_block_norm_rows. Bound by the latency of the
 // loads and the two sums. Measured on a B200 (device time): 1 x 7168 fp32 3.2 us, 64 x 7168
-// 3.6 us, 777 x 2311 fp32 / fp16 in rows of 2316 elements 5.0 us (4.3 TB/s; 6.8 element by element,
-// the way of rows of no such pitch), 2000 x 2311 bf16 12.5 and 20 us.
+// 3.6 us, 777 x 2311 fp32 / fp16 in rows of 2316 elements 4.6 us (4.7 TB/s; 6.8 element by element,
+// the way of rows of odd pitches), 2000 x 2311 bf16 12.5 and 20 us; in pairs 6313 x 822 fp16 16.8
+// and 21.5 us.
 template <int CH, int W, int SET>
 __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
@@ -115,9 +138,10 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
     const int64_t row = blockIdx.x;
     const bool wide_gate = a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL;
     Raw8 yr[CH], hr[CH], gr[CH];
-    // W 4: the element behind the whole fours that is this thread's, as it lies in memory
-    const int last = (a.dim & ~3) + threadIdx.x;
-    const bool tail = W == 4 && last < a.dim;
+    // W 4, 2: the element behind the whole fours or pairs that is this thread's, as it lies in memory
+    constexpr bool PARTS = W == 4 || W == 2;
+    const int last = (a.dim & -W) + threadIdx.x;
+    const bool tail = PARTS && last < a.dim;
     uint32_t y1 = 0, h1 = 0, g1 = 0;
     float v[CH][8];
     if (a.y)
@@ -125,7 +149,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
         for (int c = 0; c < CH; ++c) yr[c] = load8<W>(a.y, y_type, row * a.ld_y, c, a.dim);
 #pragma unroll
     for (int c = 0; c < CH; ++c) hr[c] = load8<W>(a.h, h_type, row * a.ld_h, c, a.dim);
-    if (W == 4) {
+    if (PARTS) {
         ld_elem_if(y1, a.y, y_type, row * a.ld_y + last, tail && a.y);
         ld_elem_if(h1, a.h, h_type, row * a.ld_h + last, tail);
         ld_elem_if(g1, a.gate, a.gate_type, (a.gate_kind == CLB_GATE_FULL ? row * a.ld_gate : 0) + last, tail && wide_gate);
@@ -409,7 +433,10 @@ void (*row_kernel(int ch))(NormArgs) {
 }
 template <int SET>
 void (*row_kernel(int ch, int width))(NormArgs) {
-    return width == 8 ? row_kernel<8, SET>(ch) : width == 4 ? row_kernel<4, SET>(ch) : row_kernel<1, SET>(ch);
+    return width == 8   ? row_kernel<8, SET>(ch)
+           : width == 4 ? row_kernel<4, SET>(ch)
+           : width == 2 ? row_kernel<2, SET>(ch)
+                        : row_kernel<1, SET>(ch);
 }
 void (*row_kernel(int set, int ch, int width))(NormArgs) {
     return set == kTypesF32       ? row_kernel<kTypesF32>(ch, width)
@@ -510,7 +537,7 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
         // the widest accesses that every tensor's alignment allows
         int width = c.dim % 8 == 0 ? 8 : 4;
         auto narrow = [&](const void* p, int type, int64_t ld) {
-            while (width > 1 && (!clb::ops_aligned(p, width * clb::ops_type_bytes(type)) || ld % width)) width = width == 8 ? 4 : 1;
+            while (width > 1 && (!clb::ops_aligned(p, width * clb::ops_type_bytes(type)) || ld % width)) width /= 2;
         };
         for (const Tensor& t : rows) {
             if (!t.p) continue;

@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     if (SPLIT) cluster_arrive();  // waited for before the first access to a peer
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tslot);
     // SPLIT: [source][four tokens of this CTA's share][128 rows][token] behind the stages, so that a
-    // warp's rows send 512 bytes in a row (64 x 5120 x 2304: 8.6 us, 8.8 token by token, 9.7 with a
+    // warp's rows send 512 bytes in a row (64 x 5120 x 2304: 8.3 us, 8.4 token by token, 9.4 with a
     // row's tokens together)
     const int share = SPLIT ? gm_share(g.nt, g.split) : 0;
     const uint32_t red = base + (uint32_t)g.stages * stage_bytes;

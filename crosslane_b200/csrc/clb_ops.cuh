@@ -60,6 +60,9 @@ __device__ __forceinline__ void ld_elem_if(uint32_t& v, const void* row, int typ
         : "+r"(v)
         : "l"(p), "r"((uint32_t)(ok && type == CLB_F32)), "r"((uint32_t)(ok && type != CLB_F32)));
 }
+__device__ __forceinline__ void ld4_if(uint32_t& a, const void* p, bool ok) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}" : "+r"(a) : "l"(p), "r"((uint32_t)ok));
+}
 __device__ __forceinline__ void ld8_if(uint32_t& a, uint32_t& b, const void* p, bool ok) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
                  : "+r"(a), "+r"(b)

@@ -449,7 +449,17 @@ def test_norm_rows_that_start_anywhere(cb, cuda, T, D, h_t, y_t):
                                          ("float32", "float16", "float16"), ("float16", "float32", "bfloat16")])
 def test_norm_rows_of_whole_fours(cb, cuda, D, h_t, y_t, x_t):
     """Rows that start at a multiple of four elements but not of eight; widths with 0 to 3 behind the last four."""
-    pad = -D % 8 + 4
+    norm_of_parts(cb, cuda, D, h_t, y_t, x_t, -D % 8 + 4)
+
+
+@pytest.mark.parametrize("D", [1, 2, 3, 4, 6, 9, 30, 127, 822, 1001, 2310, 2311, 8190, 8191, 9002, 16387, 32766])
+@pytest.mark.parametrize("h_t,y_t,x_t", [("float32", "float32", "float32"), ("bfloat16", "bfloat16", "bfloat16"),
+                                         ("float32", "float16", "float16"), ("float16", "float32", "bfloat16")])
+def test_norm_rows_of_whole_pairs(cb, cuda, D, h_t, y_t, x_t):
+    norm_of_parts(cb, cuda, D, h_t, y_t, x_t, -D % 4 + 2)
+
+
+def norm_of_parts(cb, cuda, D, h_t, y_t, x_t, pad):
     run_norm(cb, cuda, 3, D, h_t, y_t, x_t, gate="full", sig=True, pad=pad, seed=4)
     run_norm(cb, cuda, 2, D, h_t, y_t, x_t, gate="channel", pad=pad, seed=5, in_place=True)
     run_norm(cb, cuda, 2, D, h_t, y_t, x_t, pad=pad, post=False, weights=False, seed=6)
