@@ -22,7 +22,7 @@ struct NormArgs {
     const float *w_post, *w_pre;
     void *h_out, *x;
     int64_t ld_h, ld_y, ld_gate, ld_h_out, ld_x;
-    int dim, h_type, y_type, gate_type, x_type, gate_kind, gate_sigmoid, post;
+    int tokens, dim, h_type, y_type, gate_type, x_type, gate_kind, gate_sigmoid, post;
     float post_eps, pre_eps, residual_scale, block_scale, inv_dim;
 };
 
@@ -129,13 +129,16 @@ __host__ __device__ constexpr NormTypes norm_types(int set) {
 // 3.6 us, 777 x 2311 fp32 / fp16 in rows of 2316 elements 4.6 us (4.7 TB/s; 6.8 element by element,
 // the way of rows of odd pitches), 2000 x 2311 bf16 12.5 and 20 us; in pairs 6313 x 822 fp16 16.8
 // and 21.5 us.
-template <int CH, int W, int SET>
-__global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
+template <int CH, int W, int SET, bool SHORT>
+__global__ void __launch_bounds__(SHORT ? 256 : 1024) k_block_norm(const NormArgs a) {
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;
     const int x_type = SET ? norm_types(SET).other : a.x_type;
     __shared__ float part[2][32];
     ops_begin();
-    const int64_t row = blockIdx.x;
+    // SHORT: eight rows a CTA have a warp each and do not meet
+    const int64_t row = SHORT ? (int64_t)blockIdx.x * 8 + threadIdx.y : blockIdx.x;
+    if (SHORT && row >= a.tokens) return;
+    auto row_sum = [&](float v, float* p) { return SHORT ? ops_warp_sum(v) : cta_sum(v, p); };
     const bool wide_gate = a.gate_kind == CLB_GATE_CHANNEL || a.gate_kind == CLB_GATE_FULL;
     Raw8 yr[CH], hr[CH], gr[CH];
     // W 4, 2: the element behind the whole fours or pairs that is this thread's, as it lies in memory
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
             }
-            inv = rsqrtf(cta_sum(ss, part[0]) * a.inv_dim + a.post_eps);
+            inv = rsqrtf(row_sum(ss, part[0]) * a.inv_dim + a.post_eps);
         }
         const float f = a.block_scale * gt * inv;
 #pragma unroll
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(1024) k_block_norm(const NormArgs a) {
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss = fmaf(v[c][j], v[c][j], ss);
-        const float inv = rsqrtf(cta_sum(ss, part[1]) * a.inv_dim + a.pre_eps);
+        const float inv = rsqrtf(row_sum(ss, part[1]) * a.inv_dim + a.pre_eps);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             float w[8];
@@ -428,8 +431,11 @@ decltype(rows_kernel<kTypesAny>(0, 0)) rows_kernel(int set, int ch, int threads)
 }
 
 template <int W, int SET>
-void (*row_kernel(int ch))(NormArgs) {
-    return ch == 1 ? k_block_norm<1, W, SET> : ch == 2 ? k_block_norm<2, W, SET> : k_block_norm<4, W, SET>;
+void (*row_kernel(int ch))(NormArgs) {  // ch 0: short rows
+    return ch == 0   ? k_block_norm<1, W, SET, true>
+           : ch == 1 ? k_block_norm<1, W, SET, false>
+           : ch == 2 ? k_block_norm<2, W, SET, false>
+                     : k_block_norm<4, W, SET, false>;
 }
 template <int SET>
 void (*row_kernel(int ch, int width))(NormArgs) {
@@ -489,10 +495,14 @@ cudaError_t launch_block_norm(const NormArgs& a, int tokens, int width, cudaStre
         return ops_launch(rows_kernel(set, ch, threads), (unsigned)std::min<int64_t>(tokens, (int64_t)sms * ctas), threads,
                           (size_t)stages * stage, s, a, tokens, stages, y_bytes, h_bytes, g_bytes);
     }
+    // Many short rows: a warp each, eight to a CTA (8192 CTAs take 9 us to start). 8192 x 64 bf16 with a
+    // channel gate 5.9 for 9.2 us, 8192 x 256 6.1 for 9.2, 2000 x 256 3.1 for 3.5, 600 x 256 2.7 either way;
+    // 2000 x 512 unaligned would take 6.4 for 5.1 us.
+    if (units <= 32 && tokens >= 1000)
+        return ops_launch(row_kernel(set, 0, width), (unsigned)(((int64_t)tokens + 7) / 8), dim3(32, 8), 0, s, a);
     const int ch = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
     const int threads = std::max(32, ((units + ch - 1) / ch + 31) / 32 * 32);
-    void (*kernel)(NormArgs) = row_kernel(set, ch, width);
-    return ops_launch(kernel, (unsigned)tokens, threads, 0, s, a);
+    return ops_launch(row_kernel(set, ch, width), (unsigned)tokens, threads, 0, s, a);
 }
 
 }  // namespace
@@ -579,7 +589,7 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
         clb::NormArgs a{};
         a.h = d_h, a.y = d_y, a.gate = d_gate, a.w_post = d_w_post, a.w_pre = d_w_pre, a.h_out = d_h_out, a.x = d_x;
         a.ld_h = c.ld_h, a.ld_y = c.ld_y, a.ld_gate = c.ld_gate, a.ld_h_out = c.ld_h_out, a.ld_x = c.ld_x;
-        a.dim = c.dim, a.h_type = c.h_type, a.y_type = c.y_type, a.gate_type = c.gate_type, a.x_type = c.x_type;
+        a.tokens = tokens, a.dim = c.dim, a.h_type = c.h_type, a.y_type = c.y_type, a.gate_type = c.gate_type, a.x_type = c.x_type;
         a.gate_kind = d_gate ? c.gate : CLB_GATE_NONE, a.gate_sigmoid = c.gate_sigmoid, a.post = c.post;
         a.post_eps = c.post_eps, a.pre_eps = c.pre_eps, a.residual_scale = c.residual_scale;
         a.block_scale = c.block_scale, a.inv_dim = 1.0f / (float)c.dim;

@@ -250,13 +250,13 @@ cudaError_t ops_device(int* sms, Setup setup) {
 // also hand over, and clear, an earlier error of the caller's). The kernel's CTAs may be set
 // up while the kernel in front of it on the stream ends: it starts with ops_wait.
 template <class... P, class... A>
-cudaError_t ops_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+cudaError_t ops_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t c{};
     c.gridDim = grid;
-    c.blockDim = dim3((unsigned)threads);
+    c.blockDim = block;
     c.dynamicSmemBytes = smem;
     c.stream = s;
     c.attrs = &attr;

@@ -121,11 +121,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
     ops_wait();  // without letting the next kernel in early: its CTAs in this one's free slots made 2048 tokens 9.4 us, not 7.8
     const unsigned all = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = blockIdx.x * kRouteWarps + warp;
+    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp;
     if (t >= a.tokens) return;
-    const int64_t row = (int64_t)t * a.ld;
-    int* ids = a.ids + (int64_t)t * a.k;
-    float* w = a.w + (int64_t)t * a.k;
+    const int64_t row = t * a.ld;
+    int* ids = a.ids + t * a.k;
+    float* w = a.w + t * a.k;
 
     float l[NPL], b[NPL];
     {
@@ -443,7 +443,7 @@ extern "C" int32_t clb_route_experts_device(const clb_route_config_v1* cfg, cons
         const bool scored = d_bias || (a.groups > 1 && a.pair);
         const int per_lane = (c.n_experts + 31) / 32;
         cuda_check(clb::ops_launch(scored ? clb::route_kernel<true>(c.score, per_lane) : clb::route_kernel<false>(c.score, per_lane),
-                                   (unsigned)((tokens + clb::kRouteWarps - 1) / clb::kRouteWarps), 32 * clb::kRouteWarps, 0,
+                                   (unsigned)(((int64_t)tokens + clb::kRouteWarps - 1) / clb::kRouteWarps), 32 * clb::kRouteWarps, 0,
                                    static_cast<cudaStream_t>(stream), a),
                    "routing");
     });

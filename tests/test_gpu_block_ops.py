@@ -491,6 +491,14 @@ def test_norm_rows_that_start_at_fours(cb, cuda, T, D, h_t, y_t):
     assert torch.equal(x._base[:, keep], before[:, keep])
 
 
+@pytest.mark.parametrize("T", [999, 1000, 1001, 1007, 5000])
+@pytest.mark.parametrize("D,pad", [(1, 0), (3, 1), (8, 0), (60, 4), (64, 2), (201, 0), (256, 0), (256, 1), (255, 5), (257, 0)])
+def test_norm_many_short_rows(cb, cuda, T, D, pad):
+    run_norm(cb, cuda, T, D, "float32", "bfloat16", "float16", gate="full", sig=True, pad=pad, seed=21)
+    run_norm(cb, cuda, T, D, "bfloat16", "bfloat16", "bfloat16", gate="token", pad=pad, seed=22, in_place=True)
+    run_norm(cb, cuda, T, D, "float16", "float16", "float16", gate="channel", pad=pad, seed=23, post=False)
+
+
 @pytest.mark.parametrize("T", [1, 7, 500])
 @pytest.mark.parametrize("D", [64, 100, 1024])
 def test_norm_parts_of_one_buffer(cb, cuda, T, D):
@@ -707,6 +715,29 @@ def test_quantize_rows_that_start_anywhere(cb, cuda, dtype, rows, k):
         cb.int8_quantize(x, q, s)
         assert np.array_equal(s.double().cpu().numpy(), ws), first
         assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8)), first
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 100), (9, 256), (1499, 300), (1500, 300), (1501, 512), (1503, 513), (1500, 1000), (2000, 1024),
+                                    (2001, 1025), (2000, 7), (1777, 1)])
+@pytest.mark.parametrize("pad", [0, 8, 3])
+def test_quantize_many_short_rows(cb, cuda, dtype, rows, k, pad):
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(rows + k)
+    x = torch.randn((rows, k), generator=gen, device="cuda")
+    x[rows // 2] = 0.0
+    x[rows // 3] *= 2.0 ** -120  # a subnormal scale; zeros in fp16
+    x[rows - 1] = torch.round(x[rows - 1] * 8) * 0.5
+    x[rows - 1, 0] = 127.0
+    if rows > 4:
+        x[1, k - 1] = math.inf
+    x = pitched(torch, x, getattr(torch, dtype), pad)
+    q, s = padded_int8(torch, rows, k, 16), torch.full((rows + 1,), -7.0, device="cuda")
+    cb.int8_quantize(x, q, s[:rows])
+    wq, ws = quant64(x.double().cpu().numpy())
+    assert np.array_equal(s[:rows].double().cpu().numpy(), ws, equal_nan=True) and float(s[rows]) == -7
+    assert np.array_equal(q.cpu().numpy(), wq.astype(np.int8))
+    assert bool((q._base[:, k:] == 99).all())
 
 
 def test_quantize_borders_and_small_scales(cb, cuda):
