@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
             }
             const bool keep = mine_too && place < a.top_groups;
             const unsigned kept = __ballot_sync(all, keep);
-            if (SCORED && !exact && a.top_groups < a.groups) {
+            if (SCORED && !exact) {
                 // a value's error: of two scores, of their ranks' roundings and of the sum's
                 const uint32_t last = __reduce_min_sync(all, keep ? gkey : 0xffffffffu);
                 const uint32_t next = __reduce_max_sync(all, mine_too && !keep ? gkey : 0u);
@@ -436,9 +436,11 @@ extern "C" int32_t clb_route_experts_device(const clb_route_config_v1* cfg, cons
         require(clb::ops_aligned(d_logits, clb::ops_type_bytes(c.logits_type)) && clb::ops_aligned(d_bias, 4) &&
                     clb::ops_aligned(d_ids, 4) && clb::ops_aligned(d_w, 4) && clb::ops_aligned(d_status, 4),
                 CLB_E_INVALID, "misaligned pointer argument");
-        clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, c.n_groups,
-                         c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, c.n_experts / c.n_groups, 0, c.scale,
-                         (float)c.n_groups / (float)c.n_experts};
+        // groups that all stay decide nothing (9972 x 88, 2 of 2 groups, sigmoid: 7.6 us, 12.1 with their values)
+        const int groups = c.top_groups < c.n_groups ? c.n_groups : 1;
+        clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, groups,
+                         c.top_groups, c.group_score == CLB_GROUP_PAIR, c.renormalize, c.n_experts / groups, 0, c.scale,
+                         (float)groups / (float)c.n_experts};
         while ((2 * a.groups) << a.log_lanes <= 32) ++a.log_lanes;
         const bool scored = d_bias || (a.groups > 1 && a.pair);
         const int per_lane = (c.n_experts + 31) / 32;

@@ -246,6 +246,25 @@ def test_route_groups_an_ulp_apart(cb, cuda, kind, with_bias, E, k, groups, top)
 
 
 @pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
+@pytest.mark.parametrize("pair", [True, False])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("E,k,groups", [(96, 16, 2), (64, 8, 32), (104, 15, 4), (384, 8, 8)])
+def test_route_all_groups_stay(cb, cuda, kind, pair, with_bias, E, k, groups):
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(E + k)
+    logits = torch.randn((70, E), generator=gen, device="cuda") * 2
+    logits[torch.rand((70, E), generator=gen, device="cuda") < 0.2] = -math.inf
+    logits[3] = -math.inf
+    logits[5, 9] = math.nan
+    b = torch.randn(E, generator=gen, device="cuda") * 0.1 if with_bias else None
+    ids, w = torch.empty((70, k), dtype=torch.int32, device="cuda"), torch.empty((70, k), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    op = cb.ExpertRoute(E, k, score=kind, n_groups=groups, top_groups=groups, group_score="pair" if pair else "max")
+    op.run(logits, ids, w, d_bias=b, d_status=status)
+    assert check_route(torch, op, logits, b, ids, w, kind, groups, groups, pair) == 1 and int(status) == 1
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax", "sqrt_softplus"])
 @pytest.mark.parametrize("E,k", [(40, 4), (33, 16), (384, 8), (1024, 2)])
 def test_route_close_picks_and_a_far_rest(cb, cuda, kind, E, k):
     """Two picks that fp32 cannot tell apart and everyone else far below: exactly k candidates."""
