@@ -93,6 +93,7 @@ __device__ __noinline__ float score_exact(double l, double top, double sum) {
     if (KIND == CLB_SCORE_SOFTMAX) return (float)(exp(l - top) / sum);
     return (float)sqrt(fmax(l, 0.0) + log1p(exp(-fabs(l))));
 }
+__device__ __noinline__ double exp_exact(float l, float top) { return exp((double)l - (double)top); }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -190,6 +191,17 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
     int id = 0;
     float lj = 0.0f, s;     // lane j < k: logit and score of its pick
     int exact = 0;
+    auto exact_sum = [&] {
+        double d = KIND == CLB_SCORE_SOFTMAX ? 0.0 : 1.0;
+        if (KIND == CLB_SCORE_SOFTMAX) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i)
+                if (l[i] > -INFINITY) d += exp_exact(l[i], top);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(all, d, o);
+        }
+        return d;
+    };
 #pragma unroll 1
     for (;;) {
         uint32_t key[NPL];
@@ -199,16 +211,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
 #pragma unroll
                     for (int i = 0; i < NPL; ++i) vals_s[warp][32 * i + lane] = score_rough<KIND>(l[i]);
             } else {  // rare: nothing kept in registers for it
-                double dsum = 1.0;
-                if (KIND == CLB_SCORE_SOFTMAX) {
-                    dsum = 0.0;
-#pragma unroll 1
-                    for (int e = lane; e < a.E; e += 32) {
-                        const float le = ops_load(a.logits, a.type, row + e);
-                        if (le > -INFINITY) dsum += exp((double)le - (double)top);
-                    }
-                    for (int o = 16; o > 0; o >>= 1) dsum += __shfl_xor_sync(all, dsum, o);
-                }
+                const double dsum = exact_sum();
 #pragma unroll 1
                 for (int e = lane; e < a.E; e += 32)
                     vals_s[warp][e] = score_exact<KIND>(ops_load(a.logits, a.type, row + e), top, dsum);
@@ -359,15 +362,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         if (!__any_sync(all, unsure)) break;
         // whoever can be among the picks: an exact rank for each, a lane apiece
         const float least = __shfl_sync(all, v, a.k - 1), margin = 4.0f * (off + 2.0f * kHalfUlp * fabsf(least));
-        const int close = KIND == CLB_SCORE_SOFTMAX || !(least > -INFINITY) ? 33 : collect(rank_key(least - margin));
+        const int close = !(least > -INFINITY) ? 33 : collect(rank_key(least - margin));
         if (close > 32) {
             exact = 1;
             continue;
         }
         unsigned long long c = lane < close ? cand_s[warp][lane] : 0ull;
+        const double dsum = exact_sum();
         if (lane < close && (uint32_t)(c >> 32) != kKeyNegInf) {
             const int e = (int)~(uint32_t)c;
-            const float se = score_exact<KIND>(ops_load(a.logits, a.type, row + e), 0.0, 1.0);
+            const float se = score_exact<KIND>(ops_load(a.logits, a.type, row + e), top, dsum);
             c = (unsigned long long)rank_key(__fadd_rn(se, a.bias[e])) << 32 | (uint32_t)c;
             cand_s[warp][lane] = c;
         }
