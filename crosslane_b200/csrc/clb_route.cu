@@ -112,7 +112,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // for many (about 400 instructions a token), so candidates for the picks are cut down by the
 // lanes' maxima and ranked by counting instead of k passes over the row. Measured on a B200
 // (device time): 1 x 384, sigmoid and bias, k 6: 3.0 us; 61 x 384 in 8 groups: 5.0 us; 2048 x
-// 384, sqrt-softplus and bias: 5.6 us (7.0 with expf, log1pf and a rounded root for the ranks);
+// 384, sqrt-softplus and bias: 5.7 us (7.0 with expf, log1pf and a rounded root for the ranks);
 // 16383 x 256 softmax, k 8: 11.6 us (1.5 TB/s). One pick after the other with all scores in double
 // took 9.9, 15, 19 and 45 us.
 template <int NPL, int KIND, bool SCORED>
