@@ -182,10 +182,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         }
         sum = ops_warp_sum(sum);
     }
-    // the largest error of a rough score, and of the scores below the normal numbers
+    // the largest error of a rough score, and of the scores below the normal numbers (from logits of -200 on
+    // all are, so that -top enters as 200 at most: 2.5 times the lowest fp32 would be infinite, and off not a number)
     float off = 0.0f;
     if (SCORED && KIND == CLB_SCORE_SOFTMAX) off = fmaf(96.0f * kHalfUlp, __fdividef(1.0f, fmaxf(sum, 1.0f)), 1e-18f);
-    else if (SCORED) off = fmaf(fmaf(fmaxf(-top, 0.0f), 2.5f, 16.0f) * kHalfUlp, score_rough<KIND>(top), 1e-18f);
+    else if (SCORED) off = fmaf(fmaf(fminf(fmaxf(-top, 0.0f), 200.0f), 2.5f, 16.0f) * kHalfUlp, score_rough<KIND>(top), 1e-18f);
 
     uint32_t mine = 0;      // lane j: the key and id of the j-th largest rank
     int id = 0;
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         // whoever can be among the picks: an exact rank for each, a lane apiece
         const float least = __shfl_sync(all, v, a.k - 1), margin = 4.0f * (off + 2.0f * kHalfUlp * fabsf(least));
         const int close = !(least > -INFINITY) ? 33 : collect(rank_key(least - margin));
-        if (close > 32) {
+        if (close > 32 || close < a.k) {  // the k picks are among them by construction
             exact = 1;
             continue;
         }
