@@ -360,6 +360,19 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         const float v = key_value(mine), nv = key_value(nkey);
         if (lane + 1 < want && nkey != kKeyNegInf && !(lj == nl && bj == nb))
             unsure = !(v - nv > 2.0f * (off + kHalfUlp * (fabsf(v) + fabsf(nv))));
+        // where the last pick and the place behind it are such a pair, the best of the others decides
+        const int cut = a.k - 1;
+        if (__any_sync(all, lane == cut && cut + 1 < want && nkey != kKeyNegInf && lj == nl && bj == nb)) {
+            const uint32_t own = __shfl_sync(all, mine, cut);
+            const float pl = __shfl_sync(all, lj, cut), pb = __shfl_sync(all, bj, cut);
+            uint32_t rest = 0;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i)
+                if (key[i] <= own && !(l[i] == pl && b[i] == pb)) rest = max(rest, key[i]);
+            rest = __reduce_max_sync(all, rest);
+            const float pv = key_value(own), rv = key_value(rest);
+            unsure |= rest > kKeyNegInf && !(pv - rv > 2.0f * (off + kHalfUlp * (fabsf(pv) + fabsf(rv))));
+        }
         if (!__any_sync(all, unsure)) break;
         // whoever can be among the picks: an exact rank for each, a lane apiece
         const float least = __shfl_sync(all, v, a.k - 1), margin = 4.0f * (off + 2.0f * kHalfUlp * fabsf(least));

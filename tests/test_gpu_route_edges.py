@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_block_ops import check_route
+from test_gpu_block_ops import check_route, scores64
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,50 @@ def test_route_rows_of_the_lowest_value(cb, cuda, kind, dtype, E, k, groups, top
         for renorm in (True, False):
             ids, _ = run_and_check(cb, torch, logits, bias, k, kind, groups, top, renorm=renorm)
             assert int(ids.min()) >= 0 and int(ids.max()) < E
+
+
+def test_route_identical_experts_at_the_last_place(cb, cuda):
+    """One pick of [16.4, 16.7, 16.7]: all three scores are 1 - 2^-24 in fp32, so the first expert is it."""
+    torch = cuda
+    logits = torch.full((2, 9), -4.0, device="cuda")
+    logits[0, :3] = torch.tensor([16.4, 16.7, 16.7])
+    logits[1, 5:8] = torch.tensor([16.7, 16.7, 16.4])
+    ids, _ = run_and_check(cb, torch, logits, torch.zeros(9, device="cuda"), 1, "sigmoid")
+    assert ids.flatten().tolist() == [0, 5]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("E,k,copies", [(40, 1, 2), (40, 3, 2), (384, 6, 2), (384, 8, 3), (384, 6, 50), (1000, 16, 2)])
+@pytest.mark.parametrize("third_first", [True, False])
+def test_route_twins_at_the_cut(cb, cuda, kind, E, k, copies, third_first):
+    """k - 1 sure picks, then experts of one logit and one bias around the last place, and another whose rank is
+    within an ulp of theirs, at a lower or a higher id."""
+    torch = cuda
+    for seed in range(40):
+        rng = np.random.default_rng(seed * 100 + E + k)
+        l = (rng.standard_normal(E) - 2.0).astype(np.float32)
+        at = np.sort(rng.permutation(E)[:k + copies])
+        sure, twins = at[:k - 1], at[k - 1:]
+        third = twins[0] if third_first else twins[-1]
+        twins = twins[1:] if third_first else twins[:-1]
+        l[sure] = 2.5
+        l[twins] = np.float32(rng.uniform(0.3, 1.5))
+        l[third] = np.float32(rng.uniform(0.3, 1.5))
+        held = scores64(kind, l.astype(np.float64)).astype(np.float32)
+        bias = np.full(E, -2.0, np.float32)
+        bias[sure] = 1.0
+        bias[twins] = np.float32(rng.uniform(0.0, 0.4))
+        rank = held[twins[0]] + bias[twins[0]]
+        bias[third] = rank - held[third] + np.float32(rng.integers(-1, 2)) * np.spacing(rank)
+        run_and_check(cb, torch, torch.from_numpy(l[None]).cuda(), torch.from_numpy(bias).cuda(), k, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("groups", [1, 4])
+def test_route_constant_rows(cb, cuda, kind, groups):
+    """Every expert the same: ascending ids."""
+    torch = cuda
+    logits = torch.zeros((5, 256), device="cuda")
+    logits[1], logits[2], logits[3, ::3], logits[4, 200:] = 3.7, -20.0, 1.0, -np.inf
+    for b in (0.0, 0.3, -1e9):
+        run_and_check(cb, torch, logits, torch.full((256,), b, device="cuda"), 8, kind, groups, max(1, groups // 2))
