@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
                 v1 = fmaxf(v1, o1);
             }
             // a group's place is the number of groups in front of it
-            const uint32_t gkey = rank_key(a.pair && v2 > -INFINITY ? __fadd_rn(v1, v2) : v1);
+            const float second = a.pair && v2 > -INFINITY ? v2 : 0.0f, value = __fadd_rn(v1, second);
+            const uint32_t gkey = rank_key(value);
             int place = 0;
 #pragma unroll 8
             for (int j = 0; j < a.groups; ++j) {
@@ -264,11 +265,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
             const bool keep = mine_too && place < a.top_groups;
             const unsigned kept = __ballot_sync(all, keep);
             if (SCORED && !exact) {
-                // a value's error: of two scores, of their ranks' roundings and of the sum's
-                const uint32_t last = __reduce_min_sync(all, keep ? gkey : 0xffffffffu);
-                const uint32_t next = __reduce_max_sync(all, mine_too && !keep ? gkey : 0u);
-                const float lo = key_value(last), hi = key_value(next);
-                unsure = next != kKeyNegInf && !(lo - hi > 4.0f * (off + 2.0f * kHalfUlp * (fabsf(lo) + fabsf(hi))));
+                // A value's error: 2 off of two scores, a rounding of each rank on both sides (of the rank's own size: the
+                // two may cancel), the sum's and the bound's own: 5 u (|v1| + |second|). Other experts may be the two best
+                // by exact ranks, but a rank and its error grow together, so the bound holds for whoever is.
+                const float err = fmaf(6.0f * kHalfUlp, fabsf(v1), fmaf(6.0f * kHalfUlp, fabsf(second), 2.0f * off));
+                const uint32_t last = __reduce_min_sync(all, keep ? rank_key(value - err) : 0xffffffffu);
+                const uint32_t next = __reduce_max_sync(all, mine_too && !keep && value > -INFINITY ? rank_key(value + err) : 0u);
+                unsure = next > kKeyNegInf && last <= next;
             }
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {

@@ -99,3 +99,62 @@ def test_route_constant_rows(cb, cuda, kind, groups):
     logits[1], logits[2], logits[3, ::3], logits[4, 200:] = 3.7, -20.0, 1.0, -np.inf
     for b in (0.0, 0.3, -1e9):
         run_and_check(cb, torch, logits, torch.full((256,), b, device="cuda"), 8, kind, groups, max(1, groups // 2))
+
+
+def at_borders(kind, base, step, firsts, low, rng):
+    """Logits whose scores at `firsts` lie a few ulps around the middle between two ranks of fp32, where ranks are
+    `step` apart (multiples of it from `base` on)."""
+    E = low.size
+    l = low.astype(np.float64)
+    want = np.empty(len(firsts))
+    for i in range(len(firsts)):
+        border = (np.floor(base / step) + 0.5) * step
+        want[i] = border + rng.integers(-5, 6) * np.spacing(np.float32(border)).astype(np.float64)
+    if kind == "sigmoid":
+        l[firsts] = np.log(want / (1 - want))
+    elif kind == "sqrt_softplus":
+        l[firsts] = np.log(np.expm1(want * want))
+    else:  # the firsts' share of the sum is known: the others keep theirs
+        rest = np.exp(l[np.setdiff1d(np.arange(E), firsts)]).sum()
+        l[firsts] = np.log(want * rest / (1 - want.sum()))
+    return l.astype(np.float32)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B", [1.0, 64.0, 1000.0, 1e6])
+@pytest.mark.parametrize("groups,per,top", [(8, 2, 3), (8, 12, 3), (6, 12, 2)])
+def test_route_group_values_that_cancel(cb, cuda, kind, B, groups, per, top):
+    """A group's two best ranks are near +B and -B, so its value is small while each rank's rounding is a step of B;
+    the first scores lie where that rounding turns."""
+    torch = cuda
+    rng = np.random.default_rng(int(B) + groups + per)
+    E, T = groups * per, 300
+    firsts, seconds = np.arange(groups) * per, np.arange(groups) * per + per - 1
+    bias = np.full(E, -3 * B, np.float32)
+    bias[firsts], bias[seconds] = B, -B
+    step = float(np.spacing(np.float32(B + 0.03)))
+    rows = []
+    for _ in range(T):
+        low = np.full(E, 0.5, np.float32)
+        # a score that the firsts can all have at once (softmax), more than half a step of the largest B
+        rows.append(at_borders(kind, 0.07 if kind == "softmax" else 0.3, step, firsts, low, rng))
+    run_and_check(cb, torch, torch.from_numpy(np.stack(rows)).cuda(), torch.from_numpy(bias).cuda(), min(4, top * per),
+                  kind, groups, top, True)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pair", [True, False])
+@pytest.mark.parametrize("mask", [-1e9, float(np.finfo(np.float32).min)])
+def test_route_biases_that_mask(cb, cuda, kind, pair, mask):
+    """Finite biases that put experts out of the running, one of a group, most of a group, whole groups."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    logits = torch.randn((50, 96), generator=gen, device="cuda")
+    bias = torch.randn(96, generator=gen, device="cuda") * 0.1
+    bias[3] = mask
+    bias[13:24] = mask
+    bias[24:48] = mask
+    with np.errstate(over="ignore"):  # the definition adds two lowest values
+        run_and_check(cb, torch, logits, bias, 6, kind, 8, 3, pair)
+        bias[:90] = mask
+        run_and_check(cb, torch, logits, bias, 6, kind, 8, 3, pair)
