@@ -60,7 +60,8 @@ template <int KIND>
 __device__ __forceinline__ float score_f32(float l, float top, float sum) {
     if (KIND == CLB_SCORE_SIGMOID) return __fdividef(1.0f, 1.0f + expf(-l));
     if (KIND == CLB_SCORE_SOFTMAX) return __fdividef(exp_diff(l, top), sum);
-    return sqrtf(fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))));
+    // far below, e^l and then the logarithm are no normal numbers long before their root e^(l/2) is (off by e^l / 4)
+    return l < -20.0f ? expf(0.5f * l) : sqrtf(fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))));
 }
 // The same for the ranks' comparison alone, where what counts is the error in units of the row's
 // largest score s(top) (u: half ulps), and a third of the instructions:

@@ -1,4 +1,4 @@
-"""Routing where its fast ranks are hardest to trust, against the definition of test_gpu_block_ops."""
+"""Routing where its fast arithmetic is hardest to trust, against the definition of test_gpu_block_ops."""
 import numpy as np
 import pytest
 
@@ -158,3 +158,16 @@ def test_route_biases_that_mask(cb, cuda, kind, pair, mask):
         run_and_check(cb, torch, logits, bias, 6, kind, 8, 3, pair)
         bias[:90] = mask
         run_and_check(cb, torch, logits, bias, 6, kind, 8, 3, pair)
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("with_bias", [True, False])
+def test_route_square_root_scores_far_below(cb, cuda, renorm, with_bias):
+    """sqrt(softplus(l)) is e^(l/2) for very negative logits: a normal number down to l = -174, long after e^l is
+    not."""
+    torch = cuda
+    E, k = 64, 8
+    logits = torch.stack([torch.linspace(hi, hi - 4.0, E, device="cuda")
+                          for hi in (-10.0, -18.0, -50.0, -80.0, -86.0, -88.0, -95.0, -100.0, -104.0, -120.0, -165.0, -400.0)])
+    bias = torch.linspace(-0.1, 0.1, E, device="cuda") if with_bias else None
+    run_and_check(cb, torch, logits, bias, k, "sqrt_softplus", renorm=renorm)
