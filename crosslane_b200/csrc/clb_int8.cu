@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kDotThreads, 1) k_int8_dot(const Int8Dot d) {
         for (int u = 0; u < kDotAhead; ++u) {
             const int i = p.at + lane + 32 * u;
             w[u] = make_int4(0, 0, 0, 0);
-            if (i < p.end) w[u] = __ldg(p.row + i);
+            if (i < p.end) w[u] = p.row[i];
         }
     };
     Place here = start(warp);

@@ -266,6 +266,9 @@ cudaError_t ops_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
 
 // The first thing every thread of such a kernel does: waits until all work in front of it on the
 // stream has completed and is visible.
+// Behind it memory is read by coherent loads alone: the read-only path (ld.global.nc) is for data that
+// nobody writes while the kernel runs, and the kernel in front may still be writing when this one's CTAs
+// start; such a load may also be moved in front of the wait.
 __device__ __forceinline__ void ops_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // The same, and lets the kernel behind it be set up under this one. In this order a kernel that runs
 // ahead of its own wait knows that all but the one in front is complete.

@@ -135,17 +135,17 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         if (a.type == CLB_F32) {
             const uint32_t* p = static_cast<const uint32_t*>(a.logits) + row;
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) raw[i] = __ldg(p + min(32 * i + lane, a.E - 1));
+            for (int i = 0; i < NPL; ++i) raw[i] = p[min(32 * i + lane, a.E - 1)];
         } else {
             const uint16_t* p = static_cast<const uint16_t*>(a.logits) + row;
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) raw[i] = __ldg(p + min(32 * i + lane, a.E - 1));
+            for (int i = 0; i < NPL; ++i) raw[i] = p[min(32 * i + lane, a.E - 1)];
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) b[i] = 0.0f;
         if (a.bias)
 #pragma unroll
-            for (int i = 0; i < NPL; ++i) b[i] = __ldg(a.bias + min(32 * i + lane, a.E - 1));
+            for (int i = 0; i < NPL; ++i) b[i] = a.bias[min(32 * i + lane, a.E - 1)];
         if (a.type == CLB_F32) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i) l[i] = __uint_as_float(raw[i]);

@@ -1,4 +1,7 @@
-"""Routing where its fast arithmetic is hardest to trust, against the definition of test_gpu_block_ops."""
+"""Routing where its fast ranks are hardest to trust: rows of the types' lowest values, identical
+experts on both sides of the last pick, group values that cancel, scores far below the smallest
+exponential, and logits written by the call in front. Against the definition of test_gpu_block_ops.
+"""
 import numpy as np
 import pytest
 
@@ -171,3 +174,29 @@ def test_route_square_root_scores_far_below(cb, cuda, renorm, with_bias):
                           for hi in (-10.0, -18.0, -50.0, -80.0, -86.0, -88.0, -95.0, -100.0, -104.0, -120.0, -165.0, -400.0)])
     bias = torch.linspace(-0.1, 0.1, E, device="cuda") if with_bias else None
     run_and_check(cb, torch, logits, bias, k, "sqrt_softplus", renorm=renorm)
+
+
+@pytest.mark.parametrize("T", [1, 33, 3000])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_route_sees_what_was_written_just_before(cb, cuda, T, dtype):
+    """Logits made by the call in front, without a pause, over those of the call before."""
+    torch = cuda
+    E, k = 256, 8
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    op, norm = cb.ExpertRoute(E, k, score="softmax"), cb.BlockNorm(E, post=False)
+    inputs = [torch.randn((T, E), generator=gen, device="cuda") for _ in range(8)]
+    logits = torch.zeros((T, E), dtype=getattr(torch, dtype), device="cuda")
+    runs = []
+    for wait in (True, False):
+        out = [(torch.empty((T, k), dtype=torch.int32, device="cuda"), torch.empty((T, k), device="cuda")) for _ in inputs]
+        for x, (ids, w) in zip(inputs, out):
+            norm.run(x, d_x=logits)
+            if wait:
+                torch.cuda.synchronize()
+            op.run(logits, ids, w)
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        runs.append(out)
+    for (a, aw), (b, bw) in zip(*runs):
+        assert torch.equal(a, b) and torch.equal(aw, bw)
