@@ -563,29 +563,20 @@ extern "C" int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, in
             if (t.p != d_gate || c.gate == CLB_GATE_CHANNEL) narrow(t.p, t.type, 0);
         }
         // an output over an input: only h_out in h's place, row by row
-        const Tensor outs[] = {rows[3], rows[4]};
-        for (int o = 0; o < 2; ++o) {
-            if (!outs[o].p) continue;
-            const char* lo = static_cast<const char*>(outs[o].p);
-            const char* hi = lo + ((tokens - 1) * outs[o].ld + c.dim) * clb::ops_type_bytes(outs[o].type);
-            for (int i = 0; i < 5; ++i) {
-                const Tensor& t = rows[i];
-                if (!t.p || i == 3 + o) continue;
-                if (i == 0 && o == 0 && t.p == outs[o].p && t.ld == outs[o].ld) continue;
-                const char* l = static_cast<const char*>(t.p);
-                const char* h = l + ((tokens - 1) * t.ld + c.dim) * clb::ops_type_bytes(t.type);
-                // rows of one wider buffer may interleave: same pitch in bytes, disjoint columns
-                const int64_t pitch = t.ld * clb::ops_type_bytes(t.type);
-                bool apart = hi <= l || h <= lo;
-                if (!apart && pitch == outs[o].ld * clb::ops_type_bytes(outs[o].type)) {
-                    const int64_t wo = (int64_t)c.dim * clb::ops_type_bytes(outs[o].type);
-                    const int64_t wt = (int64_t)c.dim * clb::ops_type_bytes(t.type);
-                    const int64_t d = (((lo - l) % pitch) + pitch) % pitch;  // column of the output after t's start
-                    apart = d >= wt && d + wo <= pitch;
-                }
-                require(apart, CLB_E_INVALID, "%s overlaps %s", outs[o].name, t.name);
-            }
-        }
+        const int64_t gate_count = c.gate == CLB_GATE_TOKEN ? tokens : c.dim;
+        const clb::OpsRows all[] = {clb::ops_rows("h", d_h, tokens, c.dim, c.ld_h, c.h_type),
+                                    clb::ops_rows("y", d_y, tokens, c.dim, c.ld_y, c.y_type),
+                                    full ? clb::ops_rows("gate", d_gate, tokens, c.dim, c.ld_gate, c.gate_type)
+                                         : clb::ops_rows("gate", d_gate, 1, gate_count, gate_count, c.gate_type),
+                                    clb::ops_rows("w_post", d_w_post, 1, c.dim, c.dim, CLB_F32),
+                                    clb::ops_rows("w_pre", d_w_pre, 1, c.dim, c.dim, CLB_F32)};
+        const clb::OpsRows h_out = clb::ops_rows("h_out", d_h_out, tokens, c.dim, c.ld_h_out, c.h_type);
+        const clb::OpsRows x = clb::ops_rows("x", d_x, tokens, c.dim, c.ld_x, c.x_type), to_x[] = {x};
+        const bool in_place = d_h_out == d_h && (c.ld_h_out == c.ld_h || tokens == 1);
+        for (const clb::OpsRows& t : all)
+            require((&t == all && in_place) || clb::ops_apart(h_out, t), CLB_E_INVALID, "h_out overlaps %s", t.name);
+        clb::ops_require_apart(x, all);
+        clb::ops_require_apart(h_out, to_x);
         clb::NormArgs a{};
         a.h = d_h, a.y = d_y, a.gate = d_gate, a.w_post = d_w_post, a.w_pre = d_w_pre, a.h_out = d_h_out, a.x = d_x;
         a.ld_h = c.ld_h, a.ld_y = c.ld_y, a.ld_gate = c.ld_gate, a.ld_h_out = c.ld_h_out, a.ld_x = c.ld_x;

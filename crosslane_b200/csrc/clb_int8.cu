@@ -1115,6 +1115,12 @@ extern "C" int32_t clb_int8_quantize_device(int32_t type, const void* d_x, int64
         require(clb::ops_aligned(d_x, clb::ops_type_bytes(type)) && clb::ops_aligned(d_q, 16) &&
                     clb::ops_aligned(d_scale, 4),
                 CLB_E_INVALID, "misaligned pointer argument (q is 16-byte aligned)");
+        const clb::OpsRows in[] = {clb::ops_rows("x", d_x, rows, k, ld_x, type)};
+        const clb::OpsRows q = clb::ops_rows("q", d_q, rows, k, ld_q, CLB_I8);
+        const clb::OpsRows scale = clb::ops_rows("scale", d_scale, 1, rows, rows, CLB_F32), to_scale[] = {scale};
+        clb::ops_require_apart(q, in);
+        clb::ops_require_apart(scale, in);
+        clb::ops_require_apart(q, to_scale);
         cuda_check(clb::launch_int8_quantize(d_x, type, ld_x, rows, k, d_q, ld_q, k, d_scale,
                                              static_cast<cudaStream_t>(stream)),
                    "int8 quantise");
@@ -1154,6 +1160,17 @@ extern "C" int32_t clb_int8_linear_device(const clb_int8_linear_config_v1* cfg, 
                 CLB_E_INVALID, "misaligned pointer argument");
         require(ready || (d_ws && ws_bytes >= clb_int8_linear_workspace_bytes(tokens, c.k)), CLB_E_INVALID,
                 "workspace below clb_int8_linear_workspace_bytes");
+        const int64_t ws_need = ready ? 0 : (int64_t)clb_int8_linear_workspace_bytes(tokens, c.k);
+        const clb::OpsRows ws = clb::ops_rows("the workspace", ready ? nullptr : d_ws, 1, ws_need, ws_need, CLB_I8), to_ws[] = {ws};
+        const clb::OpsRows in[] = {clb::ops_rows("x", d_x, tokens, c.k, c.ld_x, c.x_type),
+                                   clb::ops_rows("x_scale", d_x_scale, 1, tokens, tokens, CLB_F32),
+                                   clb::ops_rows("w", d_w, c.n, c.k, c.ld_w, CLB_I8),
+                                   clb::ops_rows("w_scale", d_w_scale, 1, c.n, c.n, CLB_F32),
+                                   clb::ops_rows("bias", d_bias, 1, c.n, c.n, CLB_F32)};
+        const clb::OpsRows out = clb::ops_rows("out", d_out, tokens, c.n, c.ld_out, c.out_type);
+        clb::ops_require_apart(out, in);
+        clb::ops_require_apart(out, to_ws);
+        clb::ops_require_apart(ws, in);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         clb::Int8Args a{d_w, nullptr, d_w_scale, nullptr, d_bias, d_out, c.ld_w, 0, c.ld_out, tokens, c.n, c.k,
                         c.out_type};

@@ -21,6 +21,33 @@ inline bool ops_aligned(const void* p, size_t n) { return reinterpret_cast<uintp
 // fp32, 16 of the others).
 inline bool ops_vec8(const void* p, int type, int64_t ld) { return ops_aligned(p, type == CLB_F32 ? 32 : 16) && ld % 8 == 0; }
 
+// A tensor's rows in bytes (a vector: one row); an absent tensor has no pointer.
+struct OpsRows {
+    const char* name;
+    const void* p;
+    __int128 rows, width, pitch;  // no pitch of 64 bits overflows
+};
+inline OpsRows ops_rows(const char* name, const void* p, int64_t rows, int64_t width, int64_t ld, int type) {
+    const int b = ops_type_bytes(type);
+    return {name, p, rows, (__int128)width * b, (__int128)ld * b};
+}
+// Whether no row of one shares a byte with a row of the other: apart as ranges, or of one pitch in
+// columns apart (rows of one wider buffer interleave).
+inline bool ops_apart(const OpsRows& a, const OpsRows& b) {
+    if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return true;
+    const __int128 la = reinterpret_cast<uintptr_t>(a.p), lb = reinterpret_cast<uintptr_t>(b.p);
+    const __int128 ha = la + (a.rows - 1) * a.pitch + a.width, hb = lb + (b.rows - 1) * b.pitch + b.width;
+    if (ha <= lb || hb <= la) return true;
+    if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch)) return false;
+    const __int128 pitch = a.rows > 1 ? a.pitch : b.pitch, d = ((la - lb) % pitch + pitch) % pitch;  // column of a in b's rows
+    return d >= b.width && d + a.width <= pitch;
+}
+// Refuses an output that lies over one of the others.
+template <size_t N>
+void ops_require_apart(const OpsRows& out, const OpsRows (&others)[N]) {
+    for (const OpsRows& t : others) require(ops_apart(out, t), CLB_E_INVALID, "%s overlaps %s", out.name, t.name);
+}
+
 // One element of a floating tensor; `type` is uniform over the grid.
 __device__ __forceinline__ float ops_load(const void* p, int type, int64_t i) {
     if (type == CLB_F32) return static_cast<const float*>(p)[i];

@@ -458,6 +458,13 @@ extern "C" int32_t clb_route_experts_device(const clb_route_config_v1* cfg, cons
         require(clb::ops_aligned(d_logits, clb::ops_type_bytes(c.logits_type)) && clb::ops_aligned(d_bias, 4) &&
                     clb::ops_aligned(d_ids, 4) && clb::ops_aligned(d_w, 4) && clb::ops_aligned(d_status, 4),
                 CLB_E_INVALID, "misaligned pointer argument");
+        const clb::OpsRows in[] = {clb::ops_rows("logits", d_logits, tokens, c.n_experts, ld, c.logits_type),
+                                   clb::ops_rows("bias", d_bias, 1, c.n_experts, c.n_experts, CLB_F32)};
+        const clb::OpsRows ids = clb::ops_rows("ids", d_ids, 1, (int64_t)tokens * c.k, 0, CLB_F32);
+        const clb::OpsRows w = clb::ops_rows("weights", d_w, 1, (int64_t)tokens * c.k, 0, CLB_F32), to_w[] = {w};
+        clb::ops_require_apart(ids, in);
+        clb::ops_require_apart(w, in);
+        clb::ops_require_apart(ids, to_w);
         // groups that all stay decide nothing (9972 x 88, 2 of 2 groups, sigmoid: 7.6 us, 12.1 with their values)
         const int groups = c.top_groups < c.n_groups ? c.n_groups : 1;
         clb::RouteArgs a{d_logits, d_bias, d_ids, d_w, d_status, ld, tokens, c.logits_type, c.n_experts, c.k, groups,

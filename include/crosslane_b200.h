@@ -468,7 +468,9 @@ int32_t clb_expert_forward_noalloc(int32_t type, const void* w_gate, const void*
  * (NULL = legacy default stream), allocate nothing, do not synchronise, may be captured into
  * a graph, and check every argument before they touch the GPU. Zero tokens are no work and
  * no error. Rows are pitched: `ld_*` is the distance of two rows in elements (>= the row's
- * length). Their kernels are launched so that they are set up under the end of the kernel in
+ * length); rows of one pitch may interleave in a wider buffer. An output that shares a byte with
+ * an input, the workspace or another output is refused with CLB_E_INVALID; where one may, its
+ * function says so. Their kernels are launched so that they are set up under the end of the kernel in
  * front (programmatic dependent launch); they touch no memory before that kernel is
  * complete. No counterpart in crosslane's lanes. */
 
@@ -547,9 +549,8 @@ typedef struct clb_block_norm_config_v1 {
  * is written, and d_h_out, d_gate and d_w_post have to be NULL. d_w_post, d_w_pre [dim] fp32,
  * NULL = ones. Sums and h' are fp32 (x comes from h' before it is rounded to h_type); the
  * order of a row's sum depends on the layout and on whether the call has more than 1.6 million
- * values, so results repeat. Squares are summed as they are: values above about 1e18 overflow. Apart
- * from d_h_out = d_h with the same pitch, an output overlaps no row of an input (else
- * CLB_E_INVALID) nor a gate or weight vector. */
+ * values, so results repeat. Squares are summed as they are: values above about 1e18 overflow.
+ * d_h_out may be d_h with the same pitch. */
 int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, int32_t tokens, const void* d_h, const void* d_y,
                               const void* d_gate, const float* d_w_post, const float* d_w_pre, void* d_h_out,
                               void* d_x, void* stream, clb_error_v1* err);
@@ -580,8 +581,8 @@ uint64_t clb_int8_linear_workspace_bytes(int32_t tokens, int32_t k);
  * both), d_bias [n] fp32 or NULL. x of a floating type is quantised per token as
  * clb_int8_quantize_device does (d_x_scale NULL); CLB_I8 x brings its scales in d_x_scale.
  * d_w, d_ws and CLB_I8 x are 16-byte aligned. d_ws (ws_bytes >= the size above; may be NULL
- * for CLB_I8) is the caller's: calls that overlap on the GPU need one each. d_out overlaps
- * none of the others. The integer sums stay below 2^31 for |q|, |w| <= 127, which is what the
+ * for CLB_I8) is the caller's: calls that overlap on the GPU need one each. The
+ * integer sums stay below 2^31 for |q|, |w| <= 127, which is what the
  * quantiser makes, and for any int8 values up to k = 131071. A token whose scale is NaN gives
  * a row of NaN. The result does not depend on the other tokens of the
  * call. *d_status (int32, may be NULL) becomes 3 if a bounded wait in the kernel ran out
