@@ -21,26 +21,28 @@ inline bool ops_aligned(const void* p, size_t n) { return reinterpret_cast<uintp
 // fp32, 16 of the others).
 inline bool ops_vec8(const void* p, int type, int64_t ld) { return ops_aligned(p, type == CLB_F32 ? 32 : 16) && ld % 8 == 0; }
 
-// A tensor's rows in bytes (a vector: one row); an absent tensor has no pointer.
+// A tensor's rows in bytes (a vector: one row); an absent tensor holds none.
 struct OpsRows {
     const char* name;
-    const void* p;
-    __int128 rows, width, pitch;  // no pitch of 64 bits overflows
+    uint64_t lo, hi;  // the first byte and the one behind the last
+    int64_t rows, width, pitch;
 };
 inline OpsRows ops_rows(const char* name, const void* p, int64_t rows, int64_t width, int64_t ld, int type) {
+    if (!p || rows < 1) return {name, 0, 0, 0, 0, 0};
+    const uint64_t lo = reinterpret_cast<uintptr_t>(p);
     const int b = ops_type_bytes(type);
-    return {name, p, rows, (__int128)width * b, (__int128)ld * b};
+    const unsigned __int128 hi = lo + ((unsigned __int128)(rows - 1) * (uint64_t)ld + (uint64_t)width) * b;
+    return {name, lo, hi >> 64 ? UINT64_MAX : (uint64_t)hi, rows, width * b, ld < ((int64_t)1 << 60) ? ld * b : INT64_MAX};
 }
 // Whether no row of one shares a byte with a row of the other: apart as ranges, or of one pitch in
 // columns apart (rows of one wider buffer interleave).
 inline bool ops_apart(const OpsRows& a, const OpsRows& b) {
-    if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return true;
-    const __int128 la = reinterpret_cast<uintptr_t>(a.p), lb = reinterpret_cast<uintptr_t>(b.p);
-    const __int128 ha = la + (a.rows - 1) * a.pitch + a.width, hb = lb + (b.rows - 1) * b.pitch + b.width;
-    if (ha <= lb || hb <= la) return true;
+    if (a.hi <= b.lo || b.hi <= a.lo) return true;
     if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch)) return false;
-    const __int128 pitch = a.rows > 1 ? a.pitch : b.pitch, d = ((la - lb) % pitch + pitch) % pitch;  // column of a in b's rows
-    return d >= b.width && d + a.width <= pitch;
+    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    const int64_t apart = (int64_t)(a.lo >= b.lo ? a.lo - b.lo : b.lo - a.lo) % pitch;
+    const int64_t d = a.lo >= b.lo || apart == 0 ? apart : pitch - apart;  // column of a in b's rows
+    return d >= b.width && a.width <= pitch - d;
 }
 // Refuses an output that lies over one of the others.
 template <size_t N>
