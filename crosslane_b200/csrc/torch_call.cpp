@@ -268,14 +268,19 @@ PyObject* py_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return Py_BuildValue("LLL", (long long)w.n, (long long)w.w, (long long)pitch16(w));
 }
 
-// linear(config, w, w_scale, bias, x, out, ws, x_scale, status, stream); w, w_scale and bias as checked by weights
+// linear(config, w, w_scale, bias, x, out, ws, x_scale, status, stream). The linear's own tensors are checked again: they
+// may have been replaced or changed in place (moved, resized) since weights.
 PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return python([&] {
         arguments(n, 10);
         clb_int8_linear_config_v1 c = config<clb_int8_linear_config_v1>(a[0]);
-        const at::Tensor& w = tensor(a[1], "w");
-        const int d = device_of(w);
+        const Rows w = rows(a[1], "w", bit(kI8), -2, c.n, c.k);
+        const int d = w.device;
+        if (a[2] == Py_None) refuse(CLB_E_INVALID, "w_scale: a vector is needed");
+        void* w_scale = vector(a[2], "w_scale", bit(kF32), d, c.n);
+        void* bias = vector(a[3], "bias", bit(kF32), d, c.n);
         on_cuda(d, "the weights");
+        c.ld_w = pitch16(w);
         const Rows x = rows(a[4], "x", kFloats | bit(kI8), d, -1, c.k), o = rows(a[5], "out", kFloats, d, x.n, c.n);
         c.x_type = x.kind, c.ld_x = x.kind == kI8 ? pitch16(x) : x.ld;
         c.out_type = o.kind, c.ld_out = o.ld;
@@ -283,10 +288,8 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         void* ws = vector(a[6], "workspace", bit(kU8), d, -1, nullptr, &ws_bytes);
         void* scale = vector(a[7], "x_scale", bit(kF32), d, x.n);
         void* status = vector(a[8], "status", bit(kI32), d, 1);
-        void* w_scale = tensor(a[2], "w_scale").data_ptr();
-        void* bias = a[3] == Py_None ? nullptr : tensor(a[3], "bias").data_ptr();
         call(d, [&](clb_error_v1* err) {
-            return g_linear(&c, static_cast<int8_t*>(w.data_ptr()), static_cast<float*>(w_scale), static_cast<float*>(bias),
+            return g_linear(&c, static_cast<int8_t*>(w.p), static_cast<float*>(w_scale), static_cast<float*>(bias),
                             (int32_t)x.n, x.p, static_cast<float*>(scale), o.p, ws, ws_bytes, static_cast<int32_t*>(status),
                             stream_of(a[9], d), err);
         });

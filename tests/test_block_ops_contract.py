@@ -4,6 +4,7 @@ import os
 
 import pytest
 
+import crosslane_b200 as cb
 from crosslane_b200._capi import (BlockNormConfigV1, CLB_E_INVALID, ErrorV1, Int8LinearConfigV1, RouteConfigV1, lib)
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "crosslane_b200", "csrc")
@@ -71,3 +72,32 @@ def test_linear_refuses_outputs_over_inputs(kw, word, tokens):
     cfg = Int8LinearConfigV1(n=32, k=64, x_type=a["x_type"], ld_w=a["ld_w"], ld_x=64, ld_out=a["ld_out"])
     over(word, lib.clb_int8_linear_device, C.byref(cfg), a["w"], a["w_scale"], a["bias"], tokens, a["x"], a["x_scale"],
          a["out"], a["ws"], 1 << 16, None)
+
+
+def test_linear_checks_its_own_tensors_at_every_call():
+    """Scales, bias and weights that were replaced or changed in place behind a linear's back."""
+    torch = pytest.importorskip("torch")
+
+    def linear():
+        return cb.Int8Linear(torch.zeros((8, 64), dtype=torch.int8), torch.zeros(8), torch.zeros(8))
+
+    x, out = torch.zeros(4, 64), torch.zeros(4, 8)
+    ws = torch.zeros(linear().workspace_bytes(4), dtype=torch.uint8)
+
+    def refused_with(lin, word):
+        with pytest.raises(cb.ClbError, match=word):
+            lin.run(x, out, d_ws=ws)
+
+    refused_with(linear(), "not on a CUDA device")  # nothing else is wrong with it
+    for name, bad, word in (("d_w", torch.zeros((4, 64), dtype=torch.int8), "w is"), ("d_w", torch.zeros(8, 64), "w: "),
+                            ("d_w_scale", torch.zeros(4), "w_scale"), ("d_w_scale", None, "w_scale"),
+                            ("d_w_scale", torch.zeros(8).half(), "w_scale"), ("d_bias", torch.zeros(7), "bias")):
+        lin = linear()
+        setattr(lin, name, bad)
+        refused_with(lin, word)
+    lin = linear()
+    lin.d_w_scale.resize_(3)
+    refused_with(lin, "w_scale")
+    lin = linear()
+    lin.d_w.resize_(2, 64)
+    refused_with(lin, "w is")
