@@ -67,7 +67,10 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
         PyErr_Format(PyExc_TypeError, "%s: a torch tensor is needed, not %s", name, Py_TYPE(o)->tp_name);
         throw Refused{};
     }
-    return THPVariable_Unpack(o);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    // torch negates such a view's values when it reads them (the imaginary part of a conjugated tensor is one)
+    if (t.is_neg()) refuse(CLB_E_INVALID, "%s: a lazily negated view (resolve_neg gives its values)", name);
+    return t;
 }
 int kind_of(const at::Tensor& t) {
     switch (t.scalar_type()) {

@@ -101,3 +101,17 @@ def test_linear_checks_its_own_tensors_at_every_call():
     lin = linear()
     lin.d_w.resize_(2, 64)
     refused_with(lin, "w is")
+
+
+def test_wrappers_refuse_negated_views():
+    """A view whose values torch negates as it reads them: its memory holds the opposite numbers."""
+    torch = pytest.importorskip("torch")
+    neg = torch.complex(torch.zeros(4, 1), torch.ones(4, 1)).conj().imag
+    assert neg.is_neg() and float(neg[0, 0]) == -1
+    with pytest.raises(cb.ClbError, match="negated"):
+        cb.BlockNorm(1, post=False).run(neg, d_x=torch.zeros(4, 1))
+    with pytest.raises(cb.ClbError, match="negated"):
+        cb.BlockNorm(1, gate="token").run(torch.zeros(4, 1), d_y=torch.zeros(4, 1), d_gate=torch.zeros(4),
+                                          d_h_out=torch.zeros(4, 1), d_x=neg)
+    with pytest.raises(cb.ClbError, match="not on a CUDA device"):
+        cb.BlockNorm(1, post=False).run(neg.resolve_neg(), d_x=torch.zeros(4, 1))
