@@ -18,7 +18,7 @@ from ._capi import (BlockNormConfigV1, CLB_E_INVALID, ClbError, ErrorV1, Int8Lin
 try:
     from . import _torch_call as _call
 except ImportError as e:
-    raise ImportError("crosslane_b200: _torch_call.so is not built for this torch (run "
+    raise ImportError("crosslane_b200: _torch_call is not built for this Python and torch (run "
                       "`python crosslane_b200/build.py`)") from e
 
 _call.bind(*(C.cast(f, C.c_void_p).value for f in (lib.clb_route_experts_device, lib.clb_block_norm_device,

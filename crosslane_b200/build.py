@@ -7,14 +7,17 @@
 (Run as a file, not `-m`: importing the package loads the library being rebuilt.)
 
 Plain nvcc, one object per .cu, linked into an in-tree shared library with the
-static CUDA runtime; the library's interface is include/crosslane_b200.h. Where torch is
-installed, g++ also builds _torch_call.so, through which block_ops.py calls it.
+static CUDA runtime; the library's interface is include/crosslane_b200.h. Where a torch with
+CUDA is installed, g++ also builds the Python module _torch_call, through which block_ops.py
+calls it; the library does not depend on it.
 """
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -33,31 +36,43 @@ FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-cont
 
 
 CXX = os.environ.get("CXX", "g++")
-TORCH_CALL = os.path.join(HERE, "_torch_call.so")
+# named for this Python's ABI: another Python does not take it for its own
+TORCH_CALL = os.path.join(HERE, "_torch_call" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def _torch_call(force):
-    """The Python module over torch tensors; None where torch is not installed."""
-    import importlib.util
-    import sysconfig
+    """The Python module over torch tensors; None where no torch with CUDA is installed."""
     torch = importlib.util.find_spec("torch")
-    if torch is None:
+    if torch is None or not torch.origin:
         return None
     home = os.path.dirname(torch.origin)
+    lib = os.path.join(home, "lib")
+    if not os.path.exists(os.path.join(lib, "libc10_cuda.so")):
+        return None
     src = os.path.join(CSRC, "torch_call.cpp")
     header = os.path.join(HERE, "..", "include", "crosslane_b200.h")
-    newest = max(os.path.getmtime(f) for f in (src, header, os.path.join(home, "version.py")))
-    if not force and os.path.exists(TORCH_CALL) and os.path.getmtime(TORCH_CALL) >= newest:
-        return TORCH_CALL
-    lib = os.path.join(home, "lib")
+    # the torch that it was built for, beside the object files: another one may have older files
+    stamp = os.path.join(BUILD, "torch_call.txt")
+    with open(os.path.join(home, "version.py")) as f:
+        built_for = f"{home}\n{os.path.basename(TORCH_CALL)}\n{f.read()}"
+    newest = max(os.path.getmtime(src), os.path.getmtime(header))
+    if not force and os.path.exists(TORCH_CALL) and os.path.getmtime(TORCH_CALL) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == built_for:
+                return TORCH_CALL
     cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
     cmd = [CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I" + sysconfig.get_paths()["include"],
            "-isystem", os.path.join(home, "include"), "-isystem",
            os.path.join(home, "include", "torch", "csrc", "api", "include"), "-isystem", cuda, src, "-o", TORCH_CALL,
            "-L" + lib, "-Wl,-rpath," + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"torch_call.cpp: {CXX} does not run: {e}") from e
     if r.returncode != 0:
         raise RuntimeError(f"{CXX} failed for torch_call.cpp:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(built_for)
     return TORCH_CALL
 
 
@@ -81,11 +96,11 @@ def _compile(src, force, build_dir=BUILD, extra=()):
 
 def build(force: bool = False, verbose: bool = False, trace: bool = False) -> str:
     build_dir, lib, extra = (BUILD_TRACE, LIB_TRACE, ["-DCLB_FLOW_TRACE"]) if trace else (BUILD, LIB, [])
-    os.makedirs(build_dir, exist_ok=True)
+    for d in (BUILD, build_dir):
+        os.makedirs(d, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         call = ex.submit(_torch_call, force)
         results = list(ex.map(lambda s: _compile(s, force, build_dir, extra), SOURCES))
-        call.result()
     objs = [o for o, _ in results]
     rebuilt = any(r for _, r in results)
     if rebuilt or force or not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs):
@@ -95,6 +110,7 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         if verbose:
             print("built", lib)
+    call.result()  # the library stands without the module
     return lib
 
 
