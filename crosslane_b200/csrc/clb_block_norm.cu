@@ -126,9 +126,11 @@ __host__ __device__ constexpr NormTypes norm_types(int set) {
 // 11.5 us; 1200 x 1024 fp32 / bf16 3.9 and 5.5 us; 2000 x 1024 5.7 and 5.9 us),
 // rows that are not aligned, and rows too wide for k_block_norm_rows. Bound by the latency of the
 // loads and the two sums. Measured on a B200 (device time): 1 x 7168 fp32 3.2 us, 64 x 7168
-// 3.6 us, 777 x 2311 fp32 / fp16 in rows of 2316 elements 4.6 us (4.7 TB/s; 6.8 element by element,
+// 3.6 us, 777 x 2311 fp32 / fp16 in rows of 2316 elements 4.4 us (4.9 TB/s; 6.8 element by element,
 // the way of rows of odd pitches), 2000 x 2311 bf16 12.5 and 20 us; in pairs 6313 x 822 fp16 16.8
-// and 21.5 us.
+// and 21.5 us. Rows wider than 16384 take four chunks a thread, whose registers spill (16 to 700 bytes a
+// thread by layout and types), and one CTA an SM: 512 x 16384 bf16 17.5 us (k_block_norm_rows), 512 x
+// 16392 31 us, 512 x 32768 43 us, fp32 72 us (3.7 TB/s).
 template <int CH, int W, int SET, bool SHORT>
 __global__ void __launch_bounds__(SHORT ? 256 : 1024) k_block_norm(const NormArgs a) {
     const int h_type = SET ? norm_types(SET).h : a.h_type, y_type = SET ? norm_types(SET).other : a.y_type;

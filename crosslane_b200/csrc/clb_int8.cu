@@ -150,8 +150,10 @@ __device__ __forceinline__ float max8_nan(const Raw8& r, float m) {
 
 // A CTA per row, CH chunks of 8 values a thread in registers; or (CH = 0) rows too long for that,
 // read twice. Rows that start anywhere (not ALIGNED) come through shared memory. The columns behind
-// the last whole chunk are single values of the first threads. Bound by the rows' bytes: 4096 x 7168 fp32 24 us (6.0 TB/s), bf16 22 us (3.9 TB/s:
-// eleven instructions a value), in rows that start anywhere 32 and 29 us; 64 x 5120 bf16 2.0 us.
+// the last whole chunk are single values of the first threads. fp32 rows are bound by their bytes: 4096 x 7168
+// 23.5 us (6.2 TB/s). 16-bit rows are not: bf16 21.7 us, fp16 18.3 us (4.1 and 4.8 TB/s); bf16 has 17
+// instructions a value, 13.8 us of issue slots, and what its warps wait for most are the loads. In rows
+// that start anywhere fp32 takes 32 and bf16 29 us; 64 x 5120 bf16 2.0 us.
 template <int CH, int TYPE, bool ALIGNED>
 __global__ void __launch_bounds__(1024) k_int8_quantize(const QuantArgs a) {
     __shared__ float part[32];
@@ -502,8 +504,9 @@ void (*dot_kernel(int tt, bool vec, int type))(Int8Dot) {
 //  * kSplit: the CTAs of a cluster share one tile's K range, for products with few tiles; each
 //    sends its sums to the CTA that owns the tokens, which adds them up (integers: the order
 //    does not matter).
-// Bound by the tensor pipe for large products (90 % active at 4096 x 7168 x 7168; 135 us = 3.1
-// POP/s for a burst, 150 us at the power cap's clock), by the loads from L2 (about 100 bytes per ns
+// Bound by the tensor pipe for large products (4096 x 7168 x 7168: 135 us = 3.1 POP/s for a burst; the
+// pipe is busy for 90 % of the SMs' active cycles and 75 % of all, since 448 tiles on 74 pairs are six
+// whole waves and one of 4 tiles), by the loads from L2 (about 100 bytes per ns
 // and SM) and the stores for shallow ones (2047 x 1536 x 7168 into fp32: 26 us, 49 % active), and
 // by the chain launch - quantise - load - join for small ones (64 x 5120 x 2304: 8.2 us).
 enum : int { kSingle = 0, kPair = 1, kSplit = 2 };
@@ -928,15 +931,17 @@ __global__ void __launch_bounds__(kGmThreads, 1) k_int8_gemm(const __grid_consta
     }
 }
 
-// The form of a product, by an estimate of its time (us) whose constants fit measurements
-// from 16 x 512 x 512 to 4096 x 7168 x 7168 on a B200 to about 10 % (520 choices of form and tile for
-// 16 to 128 tokens: the estimate's choice is 0.2 % slower than the best on average, 2.5 % at most):
-// a 128-byte block of K costs its loads and, from about 100 token columns on, its multiply-adds; a
-// tile a fixed part, a launch or a split another. CTAs run in waves over the SMs, clusters in the
-// number that fits at once. Measured at 4096 x 7168 x 7168, 256 tokens a tile: single 198 us, pair 172 us; at
-// 500 x 1536 x 7168: 10.9 and 11.2 us; at 64 x 5120 x 2304, 64 tokens: single 15.4 us, split in
-// two 13.0, in four 9.3, in six 8.6 us, in seven (more clusters than fit at once) 15.0 us;
-// at 64 x 512 x 2304: single 5.4 us, split in four 7.0 us.
+// The form of a product, by an estimate of its time (us): a 128-byte block of K costs its loads and, from
+// about 100 token columns on, its multiply-adds; a tile a fixed part, a launch or a split another. CTAs
+// run in waves over the SMs, clusters in the number that fits at once. The constants were fitted for 16
+// to 128 tokens, and for larger products before neighbouring tiles shared the weights' rows: those it
+// overstates (4096 x 7168 x 7168: 183 us for 135; 1024 x 7168 x 7168: 53 for 40; 2047 x 1536 x 7168: 28 for
+// 25). Measured on a B200 (product alone, tokens a tile in brackets):
+// 4096 x 7168 x 7168 single (256) 148 us, pair (256, chosen) 135, pair (224) 144; 1024 x 7168 x 7168 single
+// (256) 47, pair (224, chosen) 40.0, pair (256) 41.3; 500 x 1536 x 7168 single (256) 9.5, pair (256, chosen) 10.5,
+// single (128) 12.0; 64 x 5120 x 2304 (64) single 14.5, split in two 11.1, in four 8.8, in six (chosen) 8.2,
+// in seven (more clusters than fit at once) 14.0; 64 x 512 x 2304 single (32, chosen) 4.9, single (64) 5.3,
+// split in four 6.3.
 struct GmPlan {
     int mode, nt, split;
 };

@@ -110,12 +110,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // One warp per token, expert e = 32 i + lane in the lane's i-th register (-inf behind the last).
 // SCORED: the ranks or the groups' values need scores. A token's 1.5 KB of logits are read
 // once; what bounds it is the latency of one warp's chain for few tokens and the issue slots
-// for many (about 400 instructions a token), so candidates for the picks are cut down by the
-// lanes' maxima and ranked by counting instead of k passes over the row. Measured on a B200
-// (device time): 1 x 384, sigmoid and bias, k 6: 3.0 us; 61 x 384 in 8 groups: 5.0 us; 2048 x
-// 384, sqrt-softplus and bias: 5.7 us (7.0 with expf, log1pf and a rounded root for the ranks);
+// for many (590 warp instructions a token in the last of these cases), so candidates for the picks are
+// cut down by the lanes' maxima and ranked by counting instead of k passes over the row. Measured on a
+// B200 (device time): 1 x 384, sigmoid and bias, k 6: 3.1 us; 61 x 384 in 8 groups: 3.7 us; 2048 x
+// 384, sqrt-softplus and bias: 5.9 us (7.0 with expf, log1pf and a rounded root for the ranks);
 // 16383 x 256 softmax, k 8: 11.6 us (1.5 TB/s). One pick after the other with all scores in double
-// took 9.9, 15, 19 and 45 us.
+// took 9.9, 15, 19 and 45 us. The form for more than 512 experts spills up to 200 bytes a thread, that for
+// 384 up to 44: 2048 tokens, sigmoid and bias, 512 experts 7.1 us, 544 and 1024 10.4 us.
 template <int NPL, int KIND, bool SCORED>
 __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 5 : 3) k_route_experts(const RouteArgs a) {
     __shared__ unsigned long long cand_s[kRouteWarps][32];                         // key, ~id

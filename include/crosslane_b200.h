@@ -510,8 +510,9 @@ typedef struct clb_route_config_v1 {
  *   CLB_GROUP_MAX the largest rank, CLB_GROUP_PAIR the fp32 sum of the two largest
  *   fl(s) + bias (fl(s) without a bias);
  *   the k largest ranks are picked, ties to the lower id;
- *   w = s (fp32, within a few ulp), divided by (sum of the picks' s + 1e-20) if renormalize,
- *   times scale.
+ *   w = s, divided by (sum of the picks' s + 1e-20) if renormalize, times scale, in fp32: s
+ *   within 9 half ulps for sigmoid and sqrt(softplus) and 75 for softmax (its sum of up to 1024
+ *   exponentials; about one in practice); an s below 2^-126 may be 0.
  * An expert whose logit or bias is -inf is not available (it still counts in the softmax
  * if only its bias is -inf). Places left over take the remaining ids in ascending order
  * with weight 0, so the ids of a token are always distinct and in range: a row with no
@@ -547,9 +548,10 @@ typedef struct clb_block_norm_config_v1 {
  * d_h [tokens][dim] is the residual stream, d_y the block's output, d_h_out receives h'
  * (may be d_h itself) and d_x (NULL: none) the next block's input. d_y NULL: h' = h, only x
  * is written, and d_h_out, d_gate and d_w_post have to be NULL. d_w_post, d_w_pre [dim] fp32,
- * NULL = ones. Sums and h' are fp32 (x comes from h' before it is rounded to h_type); the
+ * NULL = ones. Sums and h' are fp32 (x comes from h' before it is rounded to h_type). The
  * order of a row's sum depends on the layout and on whether the call has more than 1.6 million
- * values, so results repeat. Squares are summed as they are: values above about 1e18 overflow.
+ * values, and so does a full sigmoid gate: within 9 half ulps of fp32, in larger calls whose
+ * tensors all have the same 16-bit type within |gate| + 8. Equal calls give equal bits. Squares are summed as they are: values above about 1e18 overflow.
  * d_h_out may be d_h with the same pitch. */
 int32_t clb_block_norm_device(const clb_block_norm_config_v1* cfg, int32_t tokens, const void* d_h, const void* d_y,
                               const void* d_gate, const float* d_w_post, const float* d_w_pre, void* d_h_out,
