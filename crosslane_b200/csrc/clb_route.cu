@@ -365,15 +365,21 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         const float v = key_value(mine), nv = key_value(nkey);
         if (lane + 1 < want && nkey != kKeyNegInf && !(lj == nl && bj == nb))
             unsure = !(v - nv > 2.0f * (off + kHalfUlp * (fabsf(v) + fabsf(nv))));
-        // where the last pick and the place behind it are such a pair, the best of the others decides
+        // Where the last pick and the place behind it are such a pair, the best of the others decides (groups that
+        // do not stay may be among them). From memory: out of the registers it cost every row 0.1 us.
         const int cut = a.k - 1;
         if (__any_sync(all, lane == cut && cut + 1 < want && nkey != kKeyNegInf && lj == nl && bj == nb)) {
             const uint32_t own = __shfl_sync(all, mine, cut);
             const float pl = __shfl_sync(all, lj, cut), pb = __shfl_sync(all, bj, cut);
             uint32_t rest = 0;
-#pragma unroll
-            for (int i = 0; i < NPL; ++i)
-                if (key[i] <= own && !(l[i] == pl && b[i] == pb)) rest = max(rest, key[i]);
+#pragma unroll 4
+            for (int e = lane; e < a.E; e += 32) {
+                const float le = ops_load(a.logits, a.type, row + e), be = a.bias[e];
+                float r = vals_s[warp][e];
+                if (a.groups == 1) r = __fadd_rn(KIND == CLB_SCORE_SOFTMAX ? __fmul_rn(r, by) : r, be);
+                const uint32_t ke = rank_key(r);
+                if (ke <= own && le > -INFINITY && be > -INFINITY && !(le == pl && be == pb)) rest = max(rest, ke);
+            }
             rest = __reduce_max_sync(all, rest);
             const float pv = key_value(own), rv = key_value(rest);
             unsure |= rest > kKeyNegInf && !(pv - rv > 2.0f * (off + kHalfUlp * (fabsf(pv) + fabsf(rv))));
