@@ -4,7 +4,8 @@ experts, the norms with the gated residual step, and the 8-bit integer product.
 Each class holds what stays the same from call to call; `run` takes torch tensors on one
 CUDA device, launches on that device's current stream (or `stream`) and writes into tensors
 of the caller. Rows may lie in a wider buffer: only the last stride has to be 1. Tensors of
-another type, shape, stride or device are refused with ClbError.
+another type, shape, stride or device, and outputs that share memory with an input or with one
+another (but BlockNorm's d_h_out, which may be d_h), are refused with ClbError.
 
 The tensors are checked and the C entry points called by csrc/torch_call.cpp (a decode step
 makes these calls once a layer, with a few microseconds of GPU work each).

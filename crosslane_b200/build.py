@@ -37,7 +37,7 @@ FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-cont
 
 CXX = os.environ.get("CXX", "g++")
 # named for this Python's ABI: another Python does not take it for its own
-TORCH_CALL = os.path.join(HERE, "_torch_call" + sysconfig.get_config_var("EXT_SUFFIX"))
+TORCH_CALL = os.path.join(HERE, "_torch_call" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
 def _torch_call(force):

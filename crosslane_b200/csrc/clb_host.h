@@ -20,14 +20,18 @@ struct Error : std::runtime_error {
     Error(int c, const std::string& m) : std::runtime_error(m), code(c) {}
 };
 
-void require(bool ok, int code, const char* fmt, ...) {
-    if (ok) return;
+[[noreturn]] void refuse(int code, const char* fmt, ...) {
     char buf[480];
     va_list ap;
     va_start(ap, fmt);
     std::vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     throw Error(code, buf);
+}
+// Inline, with the arguments of the message touched on failure alone: an operator's call makes dozens.
+template <class... A>
+inline void require(bool ok, int code, const char* fmt, A... args) {
+    if (__builtin_expect(!ok, 0)) refuse(code, fmt, args...);
 }
 
 void cuda_check(cudaError_t e, const char* what) {
