@@ -112,11 +112,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // once; what bounds it is the latency of one warp's chain for few tokens and the issue slots
 // for many (590 warp instructions a token in the last of these cases), so candidates for the picks are
 // cut down by the lanes' maxima and ranked by counting instead of k passes over the row. Measured on a
-// B200 (device time): 1 x 384, sigmoid and bias, k 6: 3.1 us; 61 x 384 in 8 groups: 3.7 us; 2048 x
+// B200 (device time): 1 x 384, sigmoid and bias, k 6: 2.8 us; 61 x 384 in 8 groups: 3.5 us; 2048 x
 // 384, sqrt-softplus and bias: 5.9 us (7.0 with expf, log1pf and a rounded root for the ranks);
 // 16383 x 256 softmax, k 8: 11.6 us (1.5 TB/s). One pick after the other with all scores in double
-// took 9.9, 15, 19 and 45 us. The form for more than 512 experts spills up to 200 bytes a thread, that for
-// 384 up to 44: 2048 tokens, sigmoid and bias, 512 experts 7.1 us, 544 and 1024 10.4 us.
+// took 9.9, 15, 19 and 45 us. The form for more than 512 experts spills up to 224 bytes a thread, that for
+// 384 up to 60: 2048 tokens, sigmoid and bias, 512 experts 5.6 us, 544 and 1024 10 us.
 template <int NPL, int KIND, bool SCORED>
 __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 5 : 3) k_route_experts(const RouteArgs a) {
     __shared__ unsigned long long cand_s[kRouteWarps][32];                         // key, ~id
@@ -366,7 +366,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 12 ? 6 : NPL <= 16 ? 
         if (lane + 1 < want && nkey != kKeyNegInf && !(lj == nl && bj == nb))
             unsure = !(v - nv > 2.0f * (off + kHalfUlp * (fabsf(v) + fabsf(nv))));
         // Where the last pick and the place behind it are such a pair, the best of the others decides (groups that
-        // do not stay may be among them). From memory: out of the registers it cost every row 0.1 us.
+        // do not stay may be among them). From memory (64 x 384 bf16 with biases of 0: 4.1 us for 3.0): out of the registers it
+        // took 3.3, but 0.1 us from every row without such a pair.
         const int cut = a.k - 1;
         if (__any_sync(all, lane == cut && cut + 1 < want && nkey != kKeyNegInf && lj == nl && bj == nb)) {
             const uint32_t own = __shfl_sync(all, mine, cut);
